@@ -39,10 +39,11 @@ typedef void *rlp_stream_t; /* hipStream_t */
 #define RLP_EUNSUPPORTED (-1001)
 #define RLP_ENOMEM (-1002)  /* unused since ABI version 2 (no library allocations); kept reserved */
 
-#define RLP_ABI_VERSION 3  /* 2: caller-owned rollout / mlp_forward workspaces (round 5);
+#define RLP_ABI_VERSION 4  /* 2: caller-owned rollout / mlp_forward workspaces (round 5);
                               3: per-call mlp_precision of rlp_mfma_forward / rlp_value_fixup,
                                  rlp_selftest_gemm_guard, rlp_reward_norm_statistics /
-                                 rlp_reward_norm_apply / rlp_gae_normalized (round 6) */
+                                 rlp_reward_norm_apply / rlp_gae_normalized (round 6);
+                              4: rlp_linear_attention*, rlp_token_logprob* */
 
 /* ------------------------------------------------------------------------------------------ */
 /* Environment kinds. Each kind is one specific reference env copy (copies diverge). */
@@ -639,12 +640,82 @@ int rlp_sac_update(const rlp_sac_nets *nets, const rlp_sac_cfg *cfg, const float
                    float *work, float *losses, rlp_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------ */
+/* Sequence policies: memory over a rollout segment, token / discrete-action scores            */
+/* ------------------------------------------------------------------------------------------ */
+#define RLP_F32 0
+#define RLP_F16 1
+#define RLP_BF16 2
+
+/* Linear attention with one decay per head, the memory of a policy that sees part of the state:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale * q_t S_t
+ * over B sequences of T tokens and H states of [Dk][Dv] each. q, k and v have Hq, Hk and Hv heads,
+ * each a divisor of H: state h reads head h / (H / Hq) of q, and so on. Element strides of the batch,
+ * token and head axes ([T][B] rollout buffers and slices need no copy); the Dk / Dv axis is
+ * contiguous. Dk, Dv: 1 to 128. log_decay [H] f32 device, <= 0 (-inf: no memory).
+ * reset [B][T] u8 (nullable), strides reset_stride: a token with a nonzero entry begins an episode,
+ * nothing of what came before reaches it, infs and NaNs included.
+ * lengths [B] i32 device (nullable): tokens of each sequence, clamped to [0, T]; rows behind them
+ * are not read, their outputs and gradients are 0.
+ * state / state_out [B][H][Dk][Dv] f32 contiguous (nullable): the state before the first token (0)
+ * and behind the last one. State and sums are f32 whatever dtype is. No atomics: run-to-run
+ * identical. */
+typedef struct rlp_la_cfg {
+    int32_t dtype;             /* of q, k, v, out and their gradients */
+    int32_t B, T, H, Hq, Hk, Hv, Dk, Dv;
+    float scale;
+    int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3];  /* backward: o_stride is d_out's */
+    int64_t dq_stride[3], dk_stride[3], dv_stride[3];            /* backward only */
+    int64_t reset_stride[2];
+} rlp_la_cfg;
+/* Scratch of one call (0: none); it holds nothing between calls. */
+int64_t rlp_linear_attention_workspace_bytes(const rlp_la_cfg *cfg, int backward);
+int rlp_linear_attention(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
+                         const float *log_decay, const uint8_t *reset, const int32_t *lengths,
+                         const float *state, void *out, float *state_out, void *workspace,
+                         int64_t workspace_bytes, rlp_stream_t stream);
+/* Gradients of q, k, v (required; of shared heads the sum over their states) and of state
+ * (nullable) from d_out and d_state_out (nullable: 0). State is recomputed from the inputs. */
+int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
+                                  const float *log_decay, const uint8_t *reset, const int32_t *lengths,
+                                  const float *state, const void *d_out, const float *d_state_out,
+                                  void *dq, void *dk, void *dv, float *d_state, void *workspace,
+                                  int64_t workspace_bytes, rlp_stream_t stream);
+/* One token for every sequence (T = 1): state_out = reset ? 0 : lam state, + k v^T; state_out may be
+ * state. reset [B], stride reset_stride[0]. */
+int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
+                              const float *log_decay, const uint8_t *reset, const float *state,
+                              float *state_out, void *out, rlp_stream_t stream);
+
+/* Log-probabilities of given tokens (or discrete actions) with the entropy and the top alternatives
+ * of their distributions: per row of `vocab` logits (element stride row_stride, contiguous inside)
+ *   x = logits / temperature,  lse = log sum exp x,
+ *   logp = x[token] - lse,  entropy = lse - sum softmax(x) x,
+ *   top_tokens / top_logp [rows][top_k]: the top_k largest logits, ties to the lower token.
+ * A logit of -inf has probability 0. A row without any other: logp -inf, entropy 0, top_logp -inf,
+ * gradient 0. A row with NaN or +inf: NaN (NaN is no alternative; where fewer than top_k logits are
+ * numbers, the rest of top_tokens is -1 and of top_logp NaN). token < 0 marks a padded row, whose
+ * logits are not read: logp, entropy and top_logp 0, top_tokens -1, gradient 0. token >= vocab: logp
+ * and gradient NaN. top_k: 0 (no alternatives, top_* unused) to min(vocab, 32). vocab < 2^31.
+ * stats [rows][3] f32 (nullable): what the backward needs of the row sums. */
+int64_t rlp_token_logprob_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype);
+int rlp_token_logprob(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                      const int64_t *tokens, float temperature, int top_k, float *logp, float *entropy,
+                      float *stats, float *top_logp, int64_t *top_tokens, void *workspace,
+                      int64_t workspace_bytes, rlp_stream_t stream);
+/* d_logits (row stride d_row_stride, dtype) of d_logp and d_entropy ([rows] f32, nullable: 0):
+ *   (d_logp (1[v = token] - p) - d_entropy p (log p + entropy)) / temperature */
+int rlp_token_logprob_backward(const void *logits, int dtype, int64_t rows, int64_t vocab,
+                               int64_t row_stride, const int64_t *tokens, float temperature,
+                               const float *stats, const float *d_logp, const float *d_entropy,
+                               void *d_logits, int64_t d_row_stride, rlp_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------ */
 const char *rlp_last_error_string(void);
 int rlp_abi_version(void);
 /* sizeof of the ABI structs as compiled into the library (0 cartpole, 1 angleonly, 2 soi, 3 ugv,
  * 4 uav, 5 mlp_desc, 6 rollout_cfg, 7 rollout_bufs, 8 ppo2_loss_cfg, 9 adam_cfg, 10 replay,
- * 11 ugv_oa, 12 dense_net, 13 ddpg_nets, 14 ddpg_cfg, 15 sac_nets, 16 sac_cfg): FFI bindings
- * verify their mirrors with it. */
+ * 11 ugv_oa, 12 dense_net, 13 ddpg_nets, 14 ddpg_cfg, 15 sac_nets, 16 sac_cfg, 17 la_cfg): FFI
+ * bindings verify their mirrors with it. */
 int64_t rlp_struct_size(int which);
 /* Test hook of the launch-status plumbing: runs the dense GEMM launcher with `nprobs` problems,
  * which must be outside its accepted range [1, 6], through a call chain that drops the launcher's

@@ -416,6 +416,19 @@ def timeout_flag(kind):
             RLP_ENV_UAV_HOVER_OUTER_LOOP: 1, RLP_ENV_UGV_OBSTACLE_AVOIDANCE: 2}[kind]
 
 
+RLP_F32, RLP_F16, RLP_BF16 = 0, 1, 2
+
+
+class LACfg(C.Structure):  # rlp_la_cfg
+    _fields_ = [("dtype", C.c_int32), ("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32),
+                ("Hq", C.c_int32), ("Hk", C.c_int32), ("Hv", C.c_int32), ("Dk", C.c_int32),
+                ("Dv", C.c_int32), ("scale", C.c_float),
+                ("q_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("o_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3),
+                ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
+                ("reset_stride", C.c_int64 * 2)]
+
+
 def check_struct_sizes():
     """Sizes as seen by the C compiler (tests compare with librlp's rlp_struct_size())."""
     return {"cartpole": C.sizeof(CartPoleParams), "angleonly": C.sizeof(AngleOnlyParams),
@@ -426,7 +439,7 @@ def check_struct_sizes():
             "replay": C.sizeof(Replay), "ugv_oa": C.sizeof(UGVOAParams),
             "dense_net": C.sizeof(DenseNet), "ddpg_nets": C.sizeof(DDPGNets),
             "ddpg_cfg": C.sizeof(DDPGCfg), "sac_nets": C.sizeof(SACNets),
-            "sac_cfg": C.sizeof(SACCfg)}
+            "sac_cfg": C.sizeof(SACCfg), "la_cfg": C.sizeof(LACfg)}
 
 
 _ = math  # keep import for callers doing deg arithmetic

@@ -11,7 +11,7 @@ import torch  # import first: its libamdhip64 is the runtime librlp.so binds to 
 from . import _abi
 
 _LIB_NAME = "librlp.so"
-ABI_VERSION = 3  # include/rlp.h RLP_ABI_VERSION
+ABI_VERSION = 4  # include/rlp.h RLP_ABI_VERSION
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _lib = None
 
@@ -78,6 +78,15 @@ def _declare(lib):
         "rlp_ddpg_update": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
         "rlp_sac_workspace": (i64, [vp, i32]),
         "rlp_sac_update": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "rlp_linear_attention_workspace_bytes": (i64, [vp, i32]),
+        "rlp_linear_attention": (i32, [vp] * 11 + [i64, vp]),
+        "rlp_linear_attention_backward": (i32, [vp] * 15 + [i64, vp]),
+        "rlp_linear_attention_step": (i32, [vp] * 10),
+        "rlp_token_logprob_workspace_bytes": (i64, [i64, i64, i32, i32]),
+        "rlp_token_logprob": (i32, [vp, i32, i64, i64, i64, vp, C.c_float, i32, vp, vp, vp, vp, vp, vp,
+                                    i64, vp]),
+        "rlp_token_logprob_backward": (i32, [vp, i32, i64, i64, i64, vp, C.c_float, vp, vp, vp, vp, i64,
+                                             vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)

@@ -190,6 +190,7 @@ int64_t rlp_struct_size(int which) {
     case 14: return sizeof(rlp_ddpg_cfg);
     case 15: return sizeof(rlp_sac_nets);
     case 16: return sizeof(rlp_sac_cfg);
+    case 17: return sizeof(rlp_la_cfg);
     }
     return -1;
 }

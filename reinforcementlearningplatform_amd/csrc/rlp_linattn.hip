@@ -1,0 +1,614 @@
+// rlp_linattn.hip — linear attention with one decay per head (rlp_linear_attention*): the memory of
+// a sequence policy over rollout segments and prompts, forward, backward and for one token.
+//
+//   S_t = lam_h S_{t-1} + k_t v_t^T     (S_{t-1} dropped where an episode begins at token t)
+//   o_t = scale * q_t S_t
+//
+// Every direction is the same sum with its operands in other roles,
+//   out_i = sum_{j <= i} lam^(i-j) (x_i . y_j) z_j   over the pairs of one episode:
+//   forward  x = q,  y = k,  z = v;            dq  x = do, y = v,  z = k;
+//   dv       x = k,  y = q,  z = do, reversed; dk  x = v,  y = do, z = q, reversed in time,
+// so one kernel computes all of them. It walks a sequence in chunks: within a chunk the decayed,
+// masked products P = X Y^T times Z, before it lam^(i+1) x_i S with the state S = sum_j y_j z_j^T
+// of what came before, S [dx][dz] held in the MFMA accumulators of the block for the whole walk.
+#include "rlp_common.hpp"
+
+namespace rlp {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
+
+// One walk over the sequences: operand strides in elements (batch, token, head), D contiguous.
+struct WalkArgs {
+    const void *x, *y, *z;
+    void *out;
+    int64_t xb, xt, xh, yb, yt, yh, zb, zt, zh, ob, ot, oh;
+    int gx, gy, gz;          // states per x / y / z head (shared heads)
+    const float *log_decay;  // [H]
+    const uint8_t *reset;    // nullable
+    int64_t rb, rt;
+    const int32_t *lengths;  // nullable
+    const float *init;       // nullable: state in; element (a, n) at bh * dx * dz + a * ia + n * in
+    float *fin;              // nullable: state out, same layout as init
+    int64_t ia, in;
+    float *seg;              // [B * H][nseg][dx * dz] states of the segments (nseg > 1)
+    float *segf;             // [B * H][nseg] the segment's decay, -1 where it holds a reset
+    int B, T, H, dx, dz;
+    int nseg, seglen;
+    int mode;                // 0 one walk, 1 only the segments' own states, 2 outputs from seg
+    int rev;                 // walk from the last token to the first
+    int e0;                  // decay of the carried state at a chunk's token i: lam^(i + e0)
+    float s1, s2, s3;        // factors of P, of x_i S and of the state's increments
+    int out_f32;             // out is f32 (a partial of a shared head), not T
+};
+
+// Token at position p of the walk, and whether the walk's link into position p is cut: walking
+// forward by an episode that begins at p's token, backward by one that begins at the token behind.
+__device__ __forceinline__ bool cut_at(const WalkArgs &a, int b, int p, int len) {
+    if (!a.reset) return false;
+    if (!a.rev) return a.reset[b * a.rb + p * a.rt] != 0;
+    return p > 0 && a.reset[b * a.rb + (int64_t)(len - p) * a.rt] != 0;
+}
+
+// lam^n, n >= 0; lam = 0 (log_decay = -inf) included
+__device__ __forceinline__ float decay_pow(float lam2, int n) {
+    return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(lam2 * (float)n);
+}
+
+// Highest set bit of m at or below i (the chunk position where i's episode begins), -1: none.
+__device__ __forceinline__ int begin_of(uint32_t m, int i) {
+    const uint32_t below = m & (0xFFFFFFFFu >> (31 - i));
+    return below ? 31 - __builtin_clz(below) : -1;
+}
+
+// C rows of D = 32 * DB columns into LDS as f32; rows >= n and columns >= d are 0. 16-byte loads
+// (any alignment), the last columns of an odd d one by one. Returns whether a value is inf or NaN.
+template <typename T, int DB, int C, int NT>
+__device__ __forceinline__ bool stage(float (*dst)[32 * DB + 4], const T *src, int64_t st, int n, int d,
+                                      bool look) {
+    constexpr int VE = 16 / sizeof(T);
+    constexpr int VR = 32 * DB / VE;  // vectors per row
+    bool bad = false;
+#pragma unroll
+    for (int it = 0; it < (C * VR + NT - 1) / NT; ++it) {
+        const int id = it * NT + (int)threadIdx.x;
+        if (C * VR % NT != 0 && id >= C * VR) break;
+        const int row = id / VR, c = id % VR * VE;
+        float f[VE];
+#pragma unroll
+        for (int e = 0; e < VE; ++e) f[e] = 0.0f;
+        if (row < n) {
+            const T *p = src + row * st + c;
+            if (c + VE <= d) {
+                T v[VE];
+                __builtin_memcpy(v, p, 16);
+#pragma unroll
+                for (int e = 0; e < VE; ++e) f[e] = to_f32(v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    if (c + e < d) f[e] = to_f32(p[e]);
+            }
+            if (look) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) bad |= (__float_as_uint(f[e]) & 0x7F800000u) == 0x7F800000u;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VE; e += 4)
+            *(floatx4 *)&dst[row][c + e] = (floatx4){f[e], f[e + 1], f[e + 2], f[e + 3]};
+    }
+    return bad;
+}
+
+// The walk in exact f32 products (v_mfma_f32_32x32x2_f32 / 16x16x4_f32). A block of NW waves owns
+// one (batch, head, segment); wave w owns columns [32 w, 32 w + 32) of the state and the output, so
+// no wave ever needs another's state. S sits in accumulators as [a][n] with n on the lane; an
+// accumulator register is an operand of x S as it stands, because the order of the contraction
+// over a is free: step r of block ab takes rows a = 32 ab + 8 (r >> 2) + 4 (lane >> 5) + (r & 3).
+template <typename T, int DXB, int NW>
+__global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
+    constexpr int C = 32, DX = 32 * DXB, DZ = 32 * NW, NT = 64 * NW;
+    __shared__ __align__(16) float xs[C][DX + 4];
+    __shared__ __align__(16) float ys[C][DX + 4];
+    __shared__ __align__(16) float zs[C][DZ + 4];
+    __shared__ __align__(16) float ps[C][C + 4];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    const int p0 = g * a.seglen, p1 = min(len, p0 + a.seglen);
+    const float lam2 = a.log_decay[h] * kLog2e;
+    const int64_t tok0 = a.rev ? len - 1 : 0, dir = a.rev ? -1 : 1;
+    const T *x = (const T *)a.x + b * a.xb + (h / a.gx) * a.xh + tok0 * a.xt;
+    const T *y = (const T *)a.y + b * a.yb + (h / a.gy) * a.yh + tok0 * a.yt;
+    const T *z = (const T *)a.z + b * a.zb + (h / a.gz) * a.zh + tok0 * a.zt;
+    const int64_t out0 = b * a.ob + h * a.oh + tok0 * a.ot;
+    const bool want_out = a.mode != 1;
+    const int col = 32 * w + l31;
+    auto put = [&](int64_t at, float v) {
+        if (a.out_f32) ((float *)a.out)[at] = v;
+        else ((T *)a.out)[at] = (T)v;
+    };
+
+    floatx16 S[DXB];
+    {
+        const float *src = nullptr;
+        int64_t ia = a.ia, in = a.in;
+        if (a.mode == 0 && a.init) src = a.init + (int64_t)bh * a.dx * a.dz;
+        if (a.mode == 2) src = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, ia = a.dz, in = 1;
+#pragma unroll
+        for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
+                S[ab][r] = src && row < a.dx && col < a.dz ? src[row * ia + col * in] : 0.0f;
+            }
+    }
+    bool seg_cut = false;
+    for (int pos = p0; pos < p1;) {
+        int n = min(C, p1 - pos);
+        uint32_t cuts = (uint32_t)__ballot(lane < n && cut_at(a, b, pos + lane, len));
+        __syncthreads();  // the chunk before is done with the tiles
+        const bool look = (cuts & ~1u) != 0;
+        bool bad = false;
+        if (want_out) stage<T, DXB, C, NT>(xs, x + pos * dir * a.xt, dir * a.xt, n, a.dx, false);
+        bad |= stage<T, DXB, C, NT>(ys, y + pos * dir * a.yt, dir * a.yt, n, a.dx, look);
+        bad |= stage<T, NW, C, NT>(zs, z + pos * dir * a.zt, dir * a.zt, n, a.dz, look);
+        bool alone = false;
+        if (look) alone = __syncthreads_or(bad);
+        else __syncthreads();
+        if (alone) {
+            // An inf or NaN of one episode would reach the next through 0 * x in the products: this
+            // chunk ends where the next episode begins, the rows behind it are cleared.
+            n = __builtin_ctz(cuts & ~1u);
+            cuts &= 1u;
+            for (int id = threadIdx.x; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0.0f;
+            for (int id = threadIdx.x; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0.0f;
+            __syncthreads();
+        }
+        if (want_out) {
+            // P = s1 lam^(i-j) X Y^T of the pairs j <= i of one episode: the three 16 x 16 tiles on
+            // and below the diagonal over the waves
+            for (int q = w; q < 3; q += NW) {
+                const int ri = q > 0, ci = q > 1;
+                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+                const float *xa = &xs[16 * ri + (lane & 15)][lane >> 4];
+                const float *yb = &ys[16 * ci + (lane & 15)][lane >> 4];
+#pragma unroll
+                for (int kk = 0; kk < DX; kk += 4) mfma16(xa[kk], yb[kk], acc);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = 16 * ri + 4 * (lane >> 4) + r, j = 16 * ci + (lane & 15);
+                    const bool pair = j <= i && j >= begin_of(cuts, i);
+                    ps[i][j] = pair ? acc[r] * (a.s1 * decay_pow(lam2, i - j)) : 0.0f;
+                }
+            }
+            if (w == 0)
+                for (int r = 0; r < 4; ++r) ps[4 * (lane >> 4) + r][16 + (lane & 15)] = 0.0f;
+            __syncthreads();
+            floatx16 o;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[r] = 0.0f;
+#pragma unroll
+            for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const floatx4 xv = *(const floatx4 *)&xs[l31][32 * ab + 8 * r4 + 4 * half];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        o = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[r], S[ab][4 * r4 + r], o, 0, 0, 0);
+                }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = 8 * (r >> 2) + 4 * half + (r & 3);
+                o[r] = begin_of(cuts, i) < 0 ? o[r] * (a.s2 * decay_pow(lam2, i + a.e0)) : 0.0f;
+            }
+#pragma unroll
+            for (int kk = 0; kk < C; kk += 2)
+                o = __builtin_amdgcn_mfma_f32_32x32x2f32(ps[l31][kk + half], zs[kk + half][col], o, 0, 0, 0);
+            if (col < a.dz) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 8 * (r >> 2) + 4 * half + (r & 3);
+                    if (i < n) put(out0 + (pos + i) * dir * a.ot + col, o[r]);
+                }
+            }
+        }
+        // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T over the episode that goes out
+        const int last = begin_of(cuts, n - 1);
+        const float keep = decay_pow(lam2, n);
+#pragma unroll
+        for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[ab][r] = cuts ? 0.0f : S[ab][r] * keep;
+#pragma unroll
+        for (int kk = 0; kk < C; kk += 2) {
+            const int j = kk + half;
+            const float wz = j < n && j >= last ? zs[j][col] * (a.s3 * decay_pow(lam2, n - a.e0 - j)) : 0.0f;
+#pragma unroll
+            for (int ab = 0; ab < DXB; ++ab)
+                S[ab] = __builtin_amdgcn_mfma_f32_32x32x2f32(ys[j][32 * ab + l31], wz, S[ab], 0, 0, 0);
+        }
+        seg_cut |= cuts != 0;
+        pos += n;
+    }
+    // rows behind the sequence's end are 0
+    if (want_out)
+        for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
+            for (int c = threadIdx.x; c < a.dz; c += NT) put(b * a.ob + h * a.oh + t * a.ot + c, 0.0f);
+    float *dst = nullptr;
+    int64_t da = a.ia, dn = a.in;
+    if (a.mode == 0 && a.fin) dst = a.fin + (int64_t)bh * a.dx * a.dz;
+    if (a.mode == 1) dst = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, da = a.dz, dn = 1;
+    if (dst) {
+        // walking backward, what is left belongs to the state before token 0
+        const bool drop = a.mode == 0 && a.rev && a.reset && len > 0 && a.reset[b * a.rb] != 0;
+#pragma unroll
+        for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
+                if (row < a.dx && col < a.dz) dst[row * da + col * dn] = drop ? 0.0f : S[ab][r];
+            }
+    }
+    if (a.mode == 1 && threadIdx.x == 0)
+        a.segf[(int64_t)bh * a.nseg + g] = seg_cut ? -1.0f : decay_pow(lam2, max(p1 - p0, 0));
+}
+
+// Joins the segments of a split sequence: seg[g] becomes the state that comes into segment g.
+__global__ __launch_bounds__(256) void la_join_kernel(WalkArgs a) {
+    const int bh = blockIdx.x, b = bh / a.H, e = blockIdx.y * 256 + threadIdx.x;
+    if (e >= a.dx * a.dz) return;
+    const int64_t size = (int64_t)a.dx * a.dz, at = bh * size + (e / a.dz) * a.ia + (e % a.dz) * a.in;
+    float carry = a.init ? a.init[at] : 0.0f;
+    float *seg = a.seg + bh * a.nseg * size + e;
+    const float *f = a.segf + (int64_t)bh * a.nseg;
+    for (int g = 0; g < a.nseg; ++g, seg += size) {
+        const float u = *seg;
+        *seg = carry;
+        carry = f[g] < 0.0f ? u : f[g] * carry + u;
+    }
+    if (a.fin) {
+        const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+        const bool drop = a.rev && a.reset && len > 0 && a.reset[b * a.rb] != 0;
+        a.fin[at] = drop ? 0.0f : carry;
+    }
+}
+
+// Gradient of a shared head: the sum of its states' f32 partials [B][T][H][D], in head order.
+template <typename T>
+__global__ __launch_bounds__(256) void la_share_kernel(const float *part, T *out, int64_t ob, int64_t ot,
+                                                       int64_t oh, int B, int T_, int Hs, int group, int D) {
+    const int64_t total = (int64_t)B * T_ * Hs * D;
+    for (int64_t id = blockIdx.x * 256LL + threadIdx.x; id < total; id += gridDim.x * 256LL) {
+        const int d = id % D;
+        int64_t rest = id / D;
+        const int hs = rest % Hs;
+        rest /= Hs;
+        const int t = rest % T_, b = (int)(rest / T_);
+        const float *p = part + ((((int64_t)b * T_ + t) * Hs + hs) * group) * D + d;
+        float s = 0.0f;
+        for (int k = 0; k < group; ++k) s += p[(int64_t)k * D];
+        out[b * ob + t * ot + hs * oh + d] = (T)s;
+    }
+}
+
+// One token for every sequence: reads and writes each state once. A block owns 32 columns of one
+// (batch, head) state: 8 lanes of 4 columns x 32 rows at a time.
+struct StepArgs {
+    const void *q, *k, *v;
+    void *out;
+    int64_t qb, qh, kb, kh, vb, vh, ob, oh;
+    int gq, gk, gv;
+    const float *log_decay;
+    const float *state;
+    float *state_out;
+    const uint8_t *reset;
+    int64_t rb;
+    float scale;
+    int H, dk, dv;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void la_step_kernel(StepArgs a) {
+    __shared__ float part[32][33];
+    const int64_t bh = blockIdx.x;
+    const int b = (int)(bh / a.H), h = (int)(bh % a.H);
+    const int c0 = blockIdx.y * 32 + (threadIdx.x & 7) * 4, r0 = threadIdx.x >> 3;
+    const T *q = (const T *)a.q + b * a.qb + (h / a.gq) * a.qh;
+    const T *k = (const T *)a.k + b * a.kb + (h / a.gk) * a.kh;
+    const T *v = (const T *)a.v + b * a.vb + (h / a.gv) * a.vh;
+    const bool drop = a.reset && a.reset[b * a.rb] != 0;
+    const float lam = __builtin_amdgcn_exp2f(a.log_decay[h] * kLog2e);
+    float vc[4], o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vc[e] = c0 + e < a.dv ? to_f32(v[c0 + e]) : 0.0f;
+    const int64_t base = bh * a.dk * a.dv;
+    for (int r = r0; r < a.dk; r += 32) {
+        const float kr = to_f32(k[r]), qr = to_f32(q[r]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (c0 + e >= a.dv) continue;
+            const int64_t at = base + (int64_t)r * a.dv + c0 + e;
+            const float s = (drop ? 0.0f : lam * a.state[at]) + kr * vc[e];
+            a.state_out[at] = s;
+            o[e] += qr * s;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[r0][(threadIdx.x & 7) * 4 + e] = o[e];
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int c = blockIdx.y * 32 + threadIdx.x;
+        float s = 0.0f;
+        for (int r = 0; r < 32; ++r) s += part[r][threadIdx.x];
+        if (c < a.dv) ((T *)a.out)[b * a.ob + h * a.oh + c] = (T)(a.scale * s);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------
+constexpr int kMaxD = 128;
+
+// A sequence is split where batch x heads alone leave most CUs idle; a segment has 256 tokens at
+// least, so that the extra read of y and z for its state stays below the walk itself.
+int segments(int64_t bh, int T, int *seglen) {
+    *seglen = T > 0 ? T : 1;
+    if (bh >= 512 || T < 512) return 1;
+    const int want = (int)((1024 + bh - 1) / bh);
+    int len = (T + want - 1) / want;
+    len = (len + 63) / 64 * 64;
+    if (len < 256) len = 256;
+    *seglen = len;
+    return (T + len - 1) / len;
+}
+
+int64_t segment_floats(int64_t bh, int T, int Dk, int Dv) {
+    int len;
+    const int64_t ns = segments(bh, T, &len);
+    return ns > 1 ? bh * ns * ((int64_t)Dk * Dv + 1) : 0;
+}
+
+template <typename T, int DXB>
+void launch_walk(const WalkArgs &a, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)a.B * a.H), a.nseg);
+    if (a.dz <= 32) la_walk_kernel<T, DXB, 1><<<grid, 64, 0, s>>>(a);
+    else if (a.dz <= 64) la_walk_kernel<T, DXB, 2><<<grid, 128, 0, s>>>(a);
+    else la_walk_kernel<T, DXB, 4><<<grid, 256, 0, s>>>(a);
+}
+
+template <typename T>
+void launch_walk(const WalkArgs &a, hipStream_t s) {
+    if (a.dx <= 32) launch_walk<T, 1>(a, s);
+    else if (a.dx <= 64) launch_walk<T, 2>(a, s);
+    else launch_walk<T, 4>(a, s);
+}
+
+template <typename T>
+void walk(WalkArgs a, float *ws, hipStream_t s) {
+    const int64_t bh = (int64_t)a.B * a.H;
+    a.nseg = segments(bh, a.T, &a.seglen);
+    if (a.nseg > 1) {
+        a.seg = ws;
+        a.segf = ws + bh * a.nseg * a.dx * a.dz;
+        a.mode = 1;
+        launch_walk<T>(a, s);
+        la_join_kernel<<<dim3((unsigned)bh, (a.dx * a.dz + 255) / 256), 256, 0, s>>>(a);
+        a.mode = 2;
+    }
+    launch_walk<T>(a, s);
+}
+
+WalkArgs base_args(const rlp_la_cfg &c, const float *log_decay, const uint8_t *reset, const int32_t *lengths) {
+    WalkArgs a = {};
+    a.B = c.B, a.T = c.T, a.H = c.H;
+    a.log_decay = log_decay, a.reset = reset, a.lengths = lengths;
+    a.rb = c.reset_stride[0], a.rt = c.reset_stride[1];
+    return a;
+}
+
+void set(const void *&p, int64_t &b, int64_t &t, int64_t &h, const void *src, const int64_t *st) {
+    p = src, b = st[0], t = st[1], h = st[2];
+}
+
+template <typename T>
+void forward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, const float *log_decay,
+             const uint8_t *reset, const int32_t *lengths, const float *init, void *out, float *fin,
+             float *ws, hipStream_t s) {
+    WalkArgs a = base_args(c, log_decay, reset, lengths);
+    set(a.x, a.xb, a.xt, a.xh, q, c.q_stride);
+    set(a.y, a.yb, a.yt, a.yh, k, c.k_stride);
+    set(a.z, a.zb, a.zt, a.zh, v, c.v_stride);
+    a.gx = c.H / c.Hq, a.gy = c.H / c.Hk, a.gz = c.H / c.Hv;
+    a.out = out, a.ob = c.o_stride[0], a.ot = c.o_stride[1], a.oh = c.o_stride[2];
+    a.dx = c.Dk, a.dz = c.Dv;
+    a.init = init, a.fin = fin, a.ia = c.Dv, a.in = 1;
+    a.e0 = 1, a.s1 = a.s2 = c.scale, a.s3 = 1.0f;
+    walk<T>(a, ws, s);
+}
+
+template <typename T>
+void share(const rlp_la_cfg &c, const float *part, void *out, const int64_t *st, int Hs, int D, hipStream_t s) {
+    const int64_t total = (int64_t)c.B * c.T * Hs * D;
+    if (total == 0) return;
+    const int64_t blocks = (total + 255) / 256;
+    la_share_kernel<T><<<(unsigned)(blocks < 16384 ? blocks : 16384), 256, 0, s>>>(
+        part, (T *)out, st[0], st[1], st[2], c.B, c.T, Hs, c.H / Hs, D);
+}
+
+template <typename T>
+void backward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, const float *log_decay,
+              const uint8_t *reset, const int32_t *lengths, const float *init, const void *d_out,
+              const float *d_fin, void *dq, void *dk, void *dv, float *d_init, float *ws, hipStream_t s) {
+    const int64_t bh = (int64_t)c.B * c.H;
+    float *part = ws + segment_floats(bh, c.T, c.Dk, c.Dv);
+    // a gradient of unshared heads goes straight out, of shared heads through f32 partials
+    auto target = [&](WalkArgs &a, void *out, const int64_t *st, int Hs, int D) {
+        if (Hs == c.H) {
+            a.out = out, a.ob = st[0], a.ot = st[1], a.oh = st[2];
+        } else {
+            a.out = part, a.out_f32 = 1;
+            a.oh = D, a.ot = (int64_t)c.H * D, a.ob = a.ot * c.T;
+        }
+    };
+    if (dq) {
+        WalkArgs a = base_args(c, log_decay, reset, lengths);
+        set(a.x, a.xb, a.xt, a.xh, d_out, c.o_stride);
+        set(a.y, a.yb, a.yt, a.yh, v, c.v_stride);
+        set(a.z, a.zb, a.zt, a.zh, k, c.k_stride);
+        a.gx = 1, a.gy = c.H / c.Hv, a.gz = c.H / c.Hk;
+        a.dx = c.Dv, a.dz = c.Dk;
+        a.init = init, a.ia = 1, a.in = c.Dv;  // S transposed
+        a.e0 = 1, a.s1 = a.s2 = c.scale, a.s3 = 1.0f;
+        target(a, dq, c.dq_stride, c.Hq, c.Dk);
+        walk<T>(a, ws, s);
+        if (c.Hq != c.H) share<T>(c, part, dq, c.dq_stride, c.Hq, c.Dk, s);
+    }
+    if (dv || d_init) {
+        WalkArgs a = base_args(c, log_decay, reset, lengths);
+        set(a.x, a.xb, a.xt, a.xh, k, c.k_stride);
+        set(a.y, a.yb, a.yt, a.yh, q, c.q_stride);
+        set(a.z, a.zb, a.zt, a.zh, d_out, c.o_stride);
+        a.gx = c.H / c.Hk, a.gy = c.H / c.Hq, a.gz = 1;
+        a.dx = c.Dk, a.dz = c.Dv;
+        a.init = d_fin, a.fin = d_init, a.ia = c.Dv, a.in = 1;
+        a.rev = 1, a.e0 = 0, a.s1 = c.scale, a.s2 = 1.0f, a.s3 = c.scale;
+        target(a, dv, c.dv_stride, c.Hv, c.Dv);
+        walk<T>(a, ws, s);
+        if (c.Hv != c.H) share<T>(c, part, dv, c.dv_stride, c.Hv, c.Dv, s);
+    }
+    if (dk) {
+        WalkArgs a = base_args(c, log_decay, reset, lengths);
+        set(a.x, a.xb, a.xt, a.xh, v, c.v_stride);
+        set(a.y, a.yb, a.yt, a.yh, d_out, c.o_stride);
+        set(a.z, a.zb, a.zt, a.zh, q, c.q_stride);
+        a.gx = c.H / c.Hv, a.gy = 1, a.gz = c.H / c.Hq;
+        a.dx = c.Dv, a.dz = c.Dk;
+        a.init = d_fin, a.ia = 1, a.in = c.Dv;  // R transposed
+        a.rev = 1, a.e0 = 0, a.s1 = c.scale, a.s2 = 1.0f, a.s3 = c.scale;
+        target(a, dk, c.dk_stride, c.Hk, c.Dk);
+        walk<T>(a, ws, s);
+        if (c.Hk != c.H) share<T>(c, part, dk, c.dk_stride, c.Hk, c.Dk, s);
+    }
+}
+
+int check_cfg(const rlp_la_cfg *c, const char *who) {
+    RLP_REQUIRE(c, "%s: null cfg", who);
+    RLP_REQUIRE(c->dtype == RLP_F32 || c->dtype == RLP_F16 || c->dtype == RLP_BF16, "%s: dtype %d", who, c->dtype);
+    RLP_REQUIRE(c->B >= 0 && c->T >= 0 && c->H >= 1, "%s: B %d, T %d, H %d", who, c->B, c->T, c->H);
+    RLP_REQUIRE(c->Hq >= 1 && c->Hk >= 1 && c->Hv >= 1 && c->H % c->Hq == 0 && c->H % c->Hk == 0 &&
+                    c->H % c->Hv == 0,
+                "%s: %d states for %d / %d / %d heads of q / k / v (each has to divide it)", who, c->H,
+                c->Hq, c->Hk, c->Hv);
+    RLP_REQUIRE(c->Dk >= 1 && c->Dk <= kMaxD && c->Dv >= 1 && c->Dv <= kMaxD,
+                "%s: Dk %d, Dv %d (1 to %d)", who, c->Dk, c->Dv, kMaxD);
+    RLP_REQUIRE((int64_t)c->B * c->H <= 0x7FFFFFFFLL, "%s: B x H too large", who);
+    return RLP_OK;
+}
+
+int64_t workspace_bytes(const rlp_la_cfg &c, bool backward) {
+    const int64_t bh = (int64_t)c.B * c.H;
+    int64_t f = segment_floats(bh, c.T, c.Dk, c.Dv);
+    if (backward) {
+        int D = 0;
+        if (c.Hq != c.H || c.Hk != c.H) D = c.Dk;
+        if (c.Hv != c.H && c.Dv > D) D = c.Dv;
+        f += bh * c.T * D;
+    }
+    return f * 4;
+}
+
+template <typename F>
+void by_type(int dtype, F &&f) {
+    if (dtype == RLP_F32) f((float *)nullptr);
+    else if (dtype == RLP_F16) f((_Float16 *)nullptr);
+    else f((__bf16 *)nullptr);
+}
+
+}  // namespace
+}  // namespace rlp
+
+using namespace rlp;
+
+extern "C" {
+
+int64_t rlp_linear_attention_workspace_bytes(const rlp_la_cfg *cfg, int backward) {
+    const int rc = check_cfg(cfg, "rlp_linear_attention_workspace_bytes");
+    return rc != RLP_OK ? rc : workspace_bytes(*cfg, backward != 0);
+}
+
+int rlp_linear_attention(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
+                         const float *log_decay, const uint8_t *reset, const int32_t *lengths,
+                         const float *state, void *out, float *state_out, void *workspace,
+                         int64_t workspace_bytes_, rlp_stream_t stream) {
+    take_pending();
+    const int rc = check_cfg(cfg, "rlp_linear_attention");
+    if (rc != RLP_OK) return rc;
+    if (cfg->B == 0 || (cfg->T == 0 && !state_out)) return RLP_OK;
+    RLP_REQUIRE(log_decay && (cfg->T == 0 || (q && k && v && out)), "rlp_linear_attention: null argument");
+    const int64_t need = workspace_bytes(*cfg, false);
+    RLP_REQUIRE(need == 0 || (workspace && workspace_bytes_ >= need),
+                "rlp_linear_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes_,
+                (long long)need);
+    by_type(cfg->dtype, [&](auto *t) {
+        forward<std::remove_pointer_t<decltype(t)>>(*cfg, q, k, v, log_decay, reset, lengths, state, out,
+                                                    state_out, (float *)workspace, as_stream(stream));
+    });
+    RLP_CHECK_LAUNCH("rlp_linear_attention");
+    return RLP_OK;
+}
+
+int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
+                                  const float *log_decay, const uint8_t *reset, const int32_t *lengths,
+                                  const float *state, const void *d_out, const float *d_state_out,
+                                  void *dq, void *dk, void *dv, float *d_state, void *workspace,
+                                  int64_t workspace_bytes_, rlp_stream_t stream) {
+    take_pending();
+    const int rc = check_cfg(cfg, "rlp_linear_attention_backward");
+    if (rc != RLP_OK) return rc;
+    if (cfg->B == 0 || (cfg->T == 0 && !d_state)) return RLP_OK;
+    RLP_REQUIRE(log_decay && (cfg->T == 0 || (q && k && v && d_out && dq && dk && dv)),
+                "rlp_linear_attention_backward: null argument");
+    const int64_t need = workspace_bytes(*cfg, true);
+    RLP_REQUIRE(need == 0 || (workspace && workspace_bytes_ >= need),
+                "rlp_linear_attention_backward: workspace of %lld bytes, %lld needed",
+                (long long)workspace_bytes_, (long long)need);
+    by_type(cfg->dtype, [&](auto *t) {
+        backward<std::remove_pointer_t<decltype(t)>>(*cfg, q, k, v, log_decay, reset, lengths, state, d_out,
+                                                     d_state_out, dq, dk, dv, d_state, (float *)workspace,
+                                                     as_stream(stream));
+    });
+    RLP_CHECK_LAUNCH("rlp_linear_attention_backward");
+    return RLP_OK;
+}
+
+int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
+                              const float *log_decay, const uint8_t *reset, const float *state,
+                              float *state_out, void *out, rlp_stream_t stream) {
+    take_pending();
+    const int rc = check_cfg(cfg, "rlp_linear_attention_step");
+    if (rc != RLP_OK) return rc;
+    RLP_REQUIRE(cfg->T == 1, "rlp_linear_attention_step: T = %d (one token)", cfg->T);
+    if (cfg->B == 0) return RLP_OK;
+    RLP_REQUIRE(q && k && v && log_decay && state && state_out && out, "rlp_linear_attention_step: null argument");
+    StepArgs a = {};
+    a.q = q, a.k = k, a.v = v, a.out = out, a.log_decay = log_decay, a.state = state, a.state_out = state_out;
+    a.qb = cfg->q_stride[0], a.qh = cfg->q_stride[2], a.kb = cfg->k_stride[0], a.kh = cfg->k_stride[2];
+    a.vb = cfg->v_stride[0], a.vh = cfg->v_stride[2], a.ob = cfg->o_stride[0], a.oh = cfg->o_stride[2];
+    a.gq = cfg->H / cfg->Hq, a.gk = cfg->H / cfg->Hk, a.gv = cfg->H / cfg->Hv;
+    a.reset = reset, a.rb = cfg->reset_stride[0];
+    a.scale = cfg->scale, a.H = cfg->H, a.dk = cfg->Dk, a.dv = cfg->Dv;
+    const dim3 grid((unsigned)((int64_t)cfg->B * cfg->H), (cfg->Dv + 31) / 32);
+    by_type(cfg->dtype, [&](auto *t) {
+        la_step_kernel<std::remove_pointer_t<decltype(t)>><<<grid, 256, 0, as_stream(stream)>>>(a);
+    });
+    RLP_CHECK_LAUNCH("rlp_linear_attention_step");
+    return RLP_OK;
+}
+
+}  // extern "C"

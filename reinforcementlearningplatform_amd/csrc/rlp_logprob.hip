@@ -1,0 +1,552 @@
+// rlp_logprob.hip — log-probabilities of given tokens / discrete actions with the entropy and the
+// top alternatives (rlp_token_logprob), and the gradient of the logits.
+//
+// One pass over the logits: with m the largest so far, s = sum 2^y and w = sum 2^y y of
+// y = (l - m) log2(e) / temperature, rescaled when m grows,
+//   logp = ln 2 (y_token - log2 s),   entropy = ln 2 (log2 s - w / s).
+// y is formed from the difference l - m, not from scaled logits, so a row of the type's lowest
+// values is the uniform row it should be and large logits lose nothing. Sums are f32.
+#include "rlp_common.hpp"
+
+namespace rlp {
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kMaxTop = 32;
+constexpr int kNoIndex = 0x7FFFFFFF;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
+__device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+struct ScoreArgs {
+    const void *logits;
+    int64_t rows, stride;
+    int vocab;
+    const int64_t *tokens;
+    float c, inv_t;  // log2(e) / temperature, 1 / temperature
+    int k;
+    float *logp, *entropy, *stats, *top_logp;
+    int64_t *top_tokens;
+    int slices, slice_len;  // parts of a row (one block each), joined by score_join_kernel
+    float *parts;           // [rows][slices][3 + 2 k]: m, s, w, then (value, token) descending
+};
+
+struct Sums {
+    float m, s, w;  // m -inf: nothing but -inf so far
+};
+
+__device__ __forceinline__ float base_of(float m) { return m == neg_inf() ? 0.0f : m; }
+
+// The sums of two parts about their common maximum. -200: 2^-200 is 0 in f32, so a clamped y leaves
+// 0 where 0 * -inf would leave NaN.
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+    Sums r;
+    r.m = fmaxf(a.m, b.m);
+    const float base = base_of(r.m);
+    const float ya = (a.m - base) * c, yb = (b.m - base) * c;
+    const float ea = __builtin_amdgcn_exp2f(ya), eb = __builtin_amdgcn_exp2f(yb);
+    r.s = ea * a.s + eb * b.s;
+    r.w = ea * (a.w + fmaxf(ya, -200.0f) * a.s) + eb * (b.w + fmaxf(yb, -200.0f) * b.s);
+    return r;
+}
+
+template <int G>
+__device__ __forceinline__ Sums join_lanes(Sums v, float c) {
+#pragma unroll
+    for (int d = G / 2; d > 0; d >>= 1) {
+        Sums o = {__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.w, d)};
+        v = join(v, o, c);
+    }
+    return v;
+}
+
+// Row results from its sums (one lane). lt: the token's logit.
+__device__ __forceinline__ float log2_sum(const Sums &v) {
+    return v.s == 0.0f ? __builtin_inff() : __builtin_amdgcn_logf(v.s);
+}
+// not ln 2 times a log2, which overflows for a logit of the type's lowest value
+__device__ __forceinline__ float logp_of(const Sums &v, float l, float inv_t) {
+    return v.s == 0.0f ? neg_inf() : (l - base_of(v.m)) * inv_t - kLn2 * log2_sum(v);
+}
+__device__ __forceinline__ void write_row(const ScoreArgs &a, int64_t row, int64_t tok, float lt, const Sums &v) {
+    const float l2 = log2_sum(v);
+    const float ent = v.s == 0.0f ? 0.0f : kLn2 * (l2 - v.w / v.s);
+    a.logp[row] = tok >= a.vocab ? __builtin_nanf("") : logp_of(v, lt, a.inv_t);
+    a.entropy[row] = ent;
+    if (a.stats) {
+        a.stats[3 * row] = base_of(v.m);
+        a.stats[3 * row + 1] = l2;
+        a.stats[3 * row + 2] = ent;
+    }
+}
+__device__ __forceinline__ void write_padded(const ScoreArgs &a, int64_t row) {
+    a.logp[row] = a.entropy[row] = 0.0f;
+    if (a.stats) a.stats[3 * row] = a.stats[3 * row + 1] = a.stats[3 * row + 2] = 0.0f;
+    for (int i = 0; i < a.k; ++i) {
+        a.top_logp[row * a.k + i] = 0.0f;
+        a.top_tokens[row * a.k + i] = -1;
+    }
+}
+__device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t row, int i, const Sums &v, float val, int id) {
+    const bool none = id == kNoIndex;
+    a.top_logp[row * a.k + i] = none ? __builtin_nanf("") : logp_of(v, val, a.inv_t);
+    a.top_tokens[row * a.k + i] = none ? -1 : id;
+}
+
+__device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+
+// Rows of up to G * E logits, G lanes a row, all of it in registers: lane g holds tokens g + G e.
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
+    const int g = threadIdx.x % G;
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (row >= a.rows) return;
+    const int64_t tok = a.tokens[row];
+    if (tok < 0) {
+        if (g == 0) write_padded(a, row);
+        return;
+    }
+    const T *l = (const T *)a.logits + row * a.stride;
+    float x[E];
+    Sums v = {neg_inf(), 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = g + G * e < a.vocab ? to_f32(l[g + G * e]) : neg_inf();
+        v.m = fmaxf(v.m, x[e]);
+    }
+    const float lt = tok < a.vocab ? to_f32(l[tok]) : 0.0f;
+#pragma unroll
+    for (int d = G / 2; d > 0; d >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, d));
+    const float base = base_of(v.m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float y = (x[e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
+        v.s += p;
+        v.w += p * fmaxf(y, -200.0f);
+    }
+#pragma unroll
+    for (int d = G / 2; d > 0; d >>= 1) {
+        v.s += __shfl_xor(v.s, d);
+        v.w += __shfl_xor(v.w, d);
+    }
+    if (g == 0) write_row(a, row, tok, lt, v);
+    uint32_t open = 0;  // own tokens that are still to choose from
+#pragma unroll
+    for (int e = 0; e < E; ++e) open |= (g + G * e < a.vocab && x[e] == x[e] ? 1u : 0u) << e;
+    for (int i = 0; i < a.k; ++i) {
+        float bv = neg_inf();
+        int bi = kNoIndex;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if ((open >> e & 1) && ahead(x[e], g + G * e, bv, bi)) bv = x[e], bi = g + G * e;
+#pragma unroll
+        for (int d = G / 2; d > 0; d >>= 1) {
+            const float ov = __shfl_xor(bv, d);
+            const int oi = __shfl_xor(bi, d);
+            if (ahead(ov, oi, bv, bi)) bv = ov, bi = oi;
+        }
+        if (bi != kNoIndex && bi % G == g) open &= ~(1u << (bi / G));
+        if (g == 0) write_top(a, row, i, v, bv, bi);
+    }
+}
+
+// The k best (value, token) of what a wave has seen, descending over its lanes; ties to the lower
+// token. Lanes behind the last entry hold (-inf, none).
+struct TopList {
+    float v;
+    int i;
+    __device__ void clear() { v = neg_inf(), i = kNoIndex; }
+    __device__ void insert(float nv, int ni) {  // nv, ni: the same in all lanes
+        const int lane = threadIdx.x & 63;
+        const int at = __popcll(__ballot(ahead(v, i, nv, ni)));
+        // the entries behind move up one lane (DPP wave_shr:1)
+        const float uv = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x138, 0xF, 0xF, false));
+        const int ui = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xF, 0xF, false);
+        v = lane < at ? v : lane == at ? nv : uv;
+        i = lane < at ? i : lane == at ? ni : ui;
+    }
+    __device__ float worst_v(int k) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), k - 1)); }
+    __device__ int worst_i(int k) const { return __builtin_amdgcn_readlane(i, k - 1); }
+};
+
+// The k-th largest of a wave's 64 values: bit by bit on whole numbers of the same order.
+__device__ __forceinline__ float kth_largest(float x, int k) {
+    const uint32_t b = __float_as_uint(x);
+    const uint32_t key = b & 0x80000000u ? ~b : b | 0x80000000u;
+    uint32_t lo = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t t = lo | 1u << bit;
+        if (__popcll(__ballot(key >= t)) >= k) lo = t;
+    }
+    return __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
+}
+
+// Longer rows: W waves a row, one pass. A wave takes tiles of 64 lanes x U 16-byte vectors (any
+// alignment), W tiles apart, the next tile loaded ahead. Alternatives: each wave keeps its own list
+// and a lower bound of the row's k-th value, shared between the row's waves through LDS; a tile is
+// searched only where a vector's maximum reaches the bound.
+template <typename T, int W, bool TOP>
+__global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
+    constexpr int VE = 16 / sizeof(T), U = 4, TILE = 64 * VE * U;
+    __shared__ float bound_s[4];
+    __shared__ Sums sums_s[4];
+    __shared__ float lv_s[4][kMaxTop];
+    __shared__ int li_s[4][kMaxTop];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W;
+    const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
+    const int slice = blockIdx.y;
+    if (TOP) {
+        if (lane == 0 && w == 0) bound_s[wave] = neg_inf();
+        if (W > 1) __syncthreads();
+    }
+    const int64_t tok = row < a.rows ? a.tokens[row] : -1;
+    const bool padded = tok < 0;  // the same for all W waves of the row
+    const T *l = (const T *)a.logits + row * a.stride;
+    const int v0 = slice * a.slice_len, v1 = min(a.vocab, v0 + a.slice_len);
+    float lt = 0.0f;
+    if (!padded && tok < a.vocab) lt = to_f32(l[tok]);
+    Sums sum = {neg_inf(), 0.0f, 0.0f};
+    TopList list;
+    list.clear();
+    volatile float *bound = &bound_s[wave / W * W];
+
+    auto load = [&](T(&t)[U][VE], int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = at + (u * 64 + lane) * VE;
+            if (i + VE <= v1) {
+                __builtin_memcpy(t[u], l + i, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) t[u][e] = i + e < v1 ? l[i + e] : (T)neg_inf();
+            }
+        }
+    };
+    if (!padded) {
+        T cur[U][VE], nxt[U][VE];
+        int at = v0 + w * TILE;
+        if (at < v1) load(cur, at);
+        for (; at < v1; at += W * TILE) {
+            const bool more = at + W * TILE < v1;
+            if (more) load(nxt, at + W * TILE);
+            float x[U][VE], um[U], tm = neg_inf();
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                um[u] = neg_inf();
+#pragma unroll
+                for (int e = 0; e < VE; ++e) {
+                    x[u][e] = to_f32(cur[u][e]);
+                    um[u] = fmaxf(um[u], x[u][e]);
+                }
+                tm = fmaxf(tm, um[u]);
+            }
+            {
+                const float m = fmaxf(sum.m, tm), base = base_of(m);
+                const float y0 = (sum.m - base) * a.c, e0 = __builtin_amdgcn_exp2f(y0);
+                sum.w = e0 * (sum.w + fmaxf(y0, -200.0f) * sum.s);
+                sum.s *= e0;
+                sum.m = m;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        const float y = (x[u][e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
+                        sum.s += p;
+                        sum.w += p * fmaxf(y, -200.0f);
+                    }
+            }
+            if (TOP) {
+                float lv = list.worst_v(a.k);
+                int li = list.worst_i(a.k);
+                float lim = fmaxf(lv, *bound);
+                const int n = __popcll(__ballot(tm >= lim));
+                if (n > 0) {
+                    // many lanes: at least k values reach the k-th largest of the lanes' maxima
+                    if (n > a.k) lim = fmaxf(lim, kth_largest(tm, a.k));
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (!__any(um[u] >= lim)) continue;
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) {
+                            const int id = at + (u * 64 + lane) * VE + e;
+                            uint64_t pick = __ballot(x[u][e] >= lim && id < v1 && ahead(x[u][e], id, lv, li));
+                            while (pick) {
+                                const int from = __builtin_ctzll(pick);
+                                pick &= pick - 1;
+                                const float nv = __uint_as_float(
+                                    __builtin_amdgcn_readlane(__float_as_uint(x[u][e]), from));
+                                list.insert(nv, at + (u * 64 + from) * VE + e);
+                            }
+                            lv = list.worst_v(a.k), li = list.worst_i(a.k);
+                        }
+                    }
+                    if (W > 1 && lane == 0 && lv > *bound) *bound = lv;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VE; ++e) cur[u][e] = nxt[u][e];
+        }
+        sum = join_lanes<64>(sum, a.c);
+    }
+    if (W > 1) {
+        if (lane == 0) sums_s[wave] = sum;
+        if (TOP && lane < a.k) lv_s[wave][lane] = list.v, li_s[wave][lane] = list.i;
+        __syncthreads();
+        if (w != 0) return;
+        for (int o = 1; o < W; ++o) {
+            sum = join(sum, sums_s[wave + o], a.c);
+            if (!TOP) continue;
+            const float ov = lane < a.k ? lv_s[wave + o][lane] : neg_inf();
+            const int oi = lane < a.k ? li_s[wave + o][lane] : kNoIndex;
+            for (int i = 0; i < a.k; ++i) {
+                const float nv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ov), i));
+                const int ni = __builtin_amdgcn_readlane(oi, i);
+                if (!ahead(nv, ni, list.worst_v(a.k), list.worst_i(a.k))) break;
+                list.insert(nv, ni);
+            }
+        }
+    }
+    if (row >= a.rows) return;
+    if (a.slices > 1) {
+        float *part = a.parts + (row * a.slices + slice) * (3 + 2 * a.k);
+        if (lane == 0) part[0] = sum.m, part[1] = sum.s, part[2] = sum.w;
+        if (TOP && lane < a.k) {
+            part[3 + 2 * lane] = list.v;
+            part[4 + 2 * lane] = __int_as_float(list.i);
+        }
+        return;
+    }
+    if (padded) {
+        if (lane == 0) write_padded(a, row);
+        return;
+    }
+    if (lane == 0) write_row(a, row, tok, lt, sum);
+    if (TOP && lane < a.k) write_top(a, row, lane, sum, list.v, list.i);
+}
+
+// Joins the slices (at most 64) of a row: one wave a row, one slice a lane.
+template <typename T>
+__global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = blockIdx.x * 4LL + (threadIdx.x >> 6);
+    if (row >= a.rows) return;
+    const int64_t tok = a.tokens[row];
+    if (tok < 0) {
+        if (lane == 0) write_padded(a, row);
+        return;
+    }
+    const float lt = tok < a.vocab ? to_f32(((const T *)a.logits)[row * a.stride + tok]) : 0.0f;
+    const float *part = a.parts + (row * a.slices + min(lane, a.slices - 1)) * (3 + 2 * a.k);
+    const bool on = lane < a.slices;
+    Sums sum = {on ? part[0] : neg_inf(), on ? part[1] : 0.0f, on ? part[2] : 0.0f};
+    sum = join_lanes<64>(sum, a.c);
+    if (lane == 0) write_row(a, row, tok, lt, sum);
+    if (a.k == 0) return;
+    TopList list;
+    list.clear();
+    for (int i = 0; i < a.k; ++i) {  // every slice's i-th entry
+        const float v = on ? part[3 + 2 * i] : neg_inf();
+        const int id = on ? __float_as_int(part[4 + 2 * i]) : kNoIndex;
+        uint64_t pick = __ballot(ahead(v, id, list.worst_v(a.k), list.worst_i(a.k)));
+        if (!pick) break;  // the slices' further entries are no better
+        while (pick) {
+            const int from = __builtin_ctzll(pick);
+            pick &= pick - 1;
+            list.insert(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), from)),
+                        __builtin_amdgcn_readlane(id, from));
+        }
+    }
+    if (lane < a.k) write_top(a, row, lane, sum, list.v, list.i);
+}
+
+struct GradArgs {
+    const void *logits;
+    void *d_logits;
+    int64_t rows, stride, d_stride;
+    int vocab, span;  // span: logits of a row per block in y
+    const int64_t *tokens;
+    float c, inv_t;
+    const float *stats, *d_logp, *d_entropy;
+};
+
+// d logit = (g (1[token] - p) - h p (log p + entropy)) / temperature; L lanes a row, 16 bytes each.
+template <typename T>
+__global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
+    constexpr int VE = 16 / sizeof(T);
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (row >= a.rows) return;
+    const int64_t tok = a.tokens[row];
+    const bool padded = tok < 0;
+    const T *l = (const T *)a.logits + row * a.stride;
+    T *d = (T *)a.d_logits + row * a.d_stride;
+    const float m = a.stats[3 * row], l2 = a.stats[3 * row + 1], ent = a.stats[3 * row + 2];
+    float g = a.d_logp ? a.d_logp[row] * a.inv_t : 0.0f;
+    const float h = a.d_entropy ? a.d_entropy[row] * a.inv_t : 0.0f;
+    if (l2 == __builtin_inff()) g = 0.0f;  // nothing but -inf
+    if (tok >= a.vocab) g = __builtin_nanf("");
+    const int v0 = blockIdx.y * a.span, v1 = min(a.vocab, v0 + a.span);
+    for (int i = v0 + threadIdx.x % L * VE; i < v1; i += L * VE) {
+        const bool full = i + VE <= v1;
+        T x[VE] = {}, r[VE];
+        if (!padded) {
+            if (full) {
+                __builtin_memcpy(x, l + i, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) x[e] = i + e < v1 ? l[i + e] : (T)neg_inf();
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            const float y = (to_f32(x[e]) - m) * a.c - l2, p = __builtin_amdgcn_exp2f(y);
+            const float lp = kLn2 * fmaxf(y, -200.0f);
+            float v = -p * (g + h * (lp + ent));
+            if (i + e == tok) v += g;
+            r[e] = (T)(padded ? 0.0f : v);
+        }
+        if (full) {
+            __builtin_memcpy(d + i, r, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e)
+                if (i + e < v1) d[i + e] = r[e];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------
+constexpr int kSmallVocab = 512;
+
+// Few long rows: each over several blocks of at least one tile per wave.
+int slices_of(int64_t rows, int64_t vocab, int dtype, int *len) {
+    *len = (int)vocab;
+    if (rows >= 512 || vocab <= kSmallVocab) return 1;
+    const int64_t tile = 4 * (dtype == RLP_F32 ? 1024 : 2048);  // four waves' tiles
+    int64_t want = (1024 + rows - 1) / rows;
+    const int64_t most = (vocab + tile - 1) / tile;
+    if (want > most) want = most;
+    if (want > 64) want = 64;
+    if (want <= 1) return 1;
+    const int64_t each = ((vocab + want - 1) / want + tile - 1) / tile * tile;
+    *len = (int)each;
+    return (int)((vocab + each - 1) / each);
+}
+
+template <typename T>
+void launch_score(const ScoreArgs &a, hipStream_t s) {
+    auto blocks = [&](int per) { return (unsigned)((a.rows + per - 1) / per); };
+    if (a.vocab <= 32) score_small_kernel<T, 4, 8><<<blocks(64), 256, 0, s>>>(a);
+    else if (a.vocab <= 128) score_small_kernel<T, 16, 8><<<blocks(16), 256, 0, s>>>(a);
+    else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64, 8><<<blocks(4), 256, 0, s>>>(a);
+    else if (a.slices == 1 && a.vocab <= 8192) {
+        if (a.k) score_rows_kernel<T, 1, true><<<blocks(4), 256, 0, s>>>(a);
+        else score_rows_kernel<T, 1, false><<<blocks(4), 256, 0, s>>>(a);
+    } else {
+        const dim3 grid((unsigned)a.rows, a.slices);
+        if (a.k) score_rows_kernel<T, 4, true><<<grid, 256, 0, s>>>(a);
+        else score_rows_kernel<T, 4, false><<<grid, 256, 0, s>>>(a);
+        if (a.slices > 1) score_join_kernel<T><<<blocks(4), 256, 0, s>>>(a);
+    }
+}
+
+template <typename T>
+void launch_grad(GradArgs a, hipStream_t s) {
+    constexpr int VE = 16 / sizeof(T);
+    int L = 1;
+    while (L < 256 && L * VE < a.vocab) L *= 2;
+    const int64_t blocks = (a.rows + 256 / L - 1) / (256 / L);
+    // a block takes 4 vectors a lane of a long row; at most 65535 blocks in y
+    a.span = 256 * VE * 4;
+    int64_t ny = ((int64_t)a.vocab + a.span - 1) / a.span;
+    while (ny > 65535) a.span *= 2, ny = ((int64_t)a.vocab + a.span - 1) / a.span;
+    score_grad_kernel<T><<<dim3((unsigned)blocks, (unsigned)ny), 256, 0, s>>>(a, L);
+}
+
+int check_rows(const char *who, int dtype, int64_t rows, int64_t vocab, int64_t stride, float temperature) {
+    RLP_REQUIRE(dtype == RLP_F32 || dtype == RLP_F16 || dtype == RLP_BF16, "%s: dtype %d", who, dtype);
+    RLP_REQUIRE(rows >= 0 && rows <= 0x7FFFFFFFLL, "%s: %lld rows", who, (long long)rows);
+    RLP_REQUIRE(vocab >= 1 && vocab < 0x7FFF0000LL, "%s: vocab %lld", who, (long long)vocab);
+    RLP_REQUIRE(stride >= 0, "%s: row stride %lld", who, (long long)stride);
+    RLP_REQUIRE(temperature > 0.0f && temperature <= 3.402823466e38f, "%s: temperature %g (a positive number)",
+                who, temperature);
+    return RLP_OK;
+}
+
+}  // namespace
+}  // namespace rlp
+
+using namespace rlp;
+
+extern "C" {
+
+int64_t rlp_token_logprob_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype) {
+    const int rc = check_rows("rlp_token_logprob_workspace_bytes", dtype, rows, vocab, 0, 1.0f);
+    if (rc != RLP_OK) return rc;
+    RLP_REQUIRE(top_k >= 0 && top_k <= kMaxTop && top_k <= vocab,
+                "rlp_token_logprob_workspace_bytes: top_k %d (0 to min(vocab, %d))", top_k, kMaxTop);
+    int len;
+    const int n = slices_of(rows, vocab, dtype, &len);
+    return n > 1 ? rows * n * (3 + 2 * top_k) * 4 : 0;
+}
+
+int rlp_token_logprob(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                      const int64_t *tokens, float temperature, int top_k, float *logp, float *entropy,
+                      float *stats, float *top_logp, int64_t *top_tokens, void *workspace,
+                      int64_t workspace_bytes, rlp_stream_t stream) {
+    take_pending();
+    const int rc = check_rows("rlp_token_logprob", dtype, rows, vocab, row_stride, temperature);
+    if (rc != RLP_OK) return rc;
+    RLP_REQUIRE(top_k >= 0 && top_k <= kMaxTop && top_k <= vocab,
+                "rlp_token_logprob: top_k %d (0 to min(vocab, %d))", top_k, kMaxTop);
+    if (rows == 0) return RLP_OK;
+    RLP_REQUIRE(logits && tokens && logp && entropy && (top_k == 0 || (top_logp && top_tokens)),
+                "rlp_token_logprob: null argument");
+    const int64_t need = rlp_token_logprob_workspace_bytes(rows, vocab, top_k, dtype);
+    RLP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
+                "rlp_token_logprob: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                (long long)need);
+    ScoreArgs a = {};
+    a.logits = logits, a.rows = rows, a.stride = row_stride, a.vocab = (int)vocab, a.tokens = tokens;
+    a.c = (float)(1.4426950408889634 / (double)temperature), a.inv_t = 1.0f / temperature, a.k = top_k;
+    a.logp = logp, a.entropy = entropy, a.stats = stats, a.top_logp = top_logp, a.top_tokens = top_tokens;
+    a.slices = slices_of(rows, vocab, dtype, &a.slice_len);
+    a.parts = (float *)workspace;
+    hipStream_t s = as_stream(stream);
+    if (dtype == RLP_F32) launch_score<float>(a, s);
+    else if (dtype == RLP_F16) launch_score<_Float16>(a, s);
+    else launch_score<__bf16>(a, s);
+    RLP_CHECK_LAUNCH("rlp_token_logprob");
+    return RLP_OK;
+}
+
+int rlp_token_logprob_backward(const void *logits, int dtype, int64_t rows, int64_t vocab,
+                               int64_t row_stride, const int64_t *tokens, float temperature,
+                               const float *stats, const float *d_logp, const float *d_entropy,
+                               void *d_logits, int64_t d_row_stride, rlp_stream_t stream) {
+    take_pending();
+    const int rc = check_rows("rlp_token_logprob_backward", dtype, rows, vocab, row_stride, temperature);
+    if (rc != RLP_OK) return rc;
+    RLP_REQUIRE(rows <= 1 || d_row_stride >= vocab, "rlp_token_logprob_backward: rows of d_logits overlap");
+    if (rows == 0) return RLP_OK;
+    RLP_REQUIRE(logits && tokens && stats && d_logits, "rlp_token_logprob_backward: null argument");
+    GradArgs a = {};
+    a.logits = logits, a.d_logits = d_logits, a.rows = rows, a.stride = row_stride, a.d_stride = d_row_stride;
+    a.vocab = (int)vocab, a.tokens = tokens;
+    a.c = (float)(1.4426950408889634 / (double)temperature), a.inv_t = 1.0f / temperature;
+    a.stats = stats, a.d_logp = d_logp, a.d_entropy = d_entropy;
+    hipStream_t s = as_stream(stream);
+    if (dtype == RLP_F32) launch_grad<float>(a, s);
+    else if (dtype == RLP_F16) launch_grad<_Float16>(a, s);
+    else launch_grad<__bf16>(a, s);
+    RLP_CHECK_LAUNCH("rlp_token_logprob_backward");
+    return RLP_OK;
+}
+
+}  // extern "C"

@@ -505,3 +505,324 @@ def sac_update(nets, cfg, s, a, r, s_next, dw, noise, work, losses):
                                ptr(dw), ptr(noise), ptr(work), ptr(losses), stream_ptr()),
           "rlp_sac_update")
     return losses
+
+
+# ---------------------------------------------------------------------------------------------
+# Sequence policies (include/rlp.h: rlp_linear_attention*, rlp_token_logprob*)
+# ---------------------------------------------------------------------------------------------
+_DTYPES = {torch.float32: _abi.RLP_F32, torch.float16: _abi.RLP_F16, torch.bfloat16: _abi.RLP_BF16}
+
+
+def _on_gpu(what, **tensors):
+    """All tensors on one ROCm device (returned); None entries are skipped."""
+    dev = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RLPError(f"{what}: {name} is not on the GPU (librlp takes device tensors only)")
+        if dev is not None and t.device != dev:
+            raise RLPError(f"{what}: {name} is on {t.device}, the others on {dev}")
+        dev = t.device
+    return dev
+
+
+def _dtype_of(what, t):
+    if t.dtype not in _DTYPES:
+        raise RLPError(f"{what}: dtype {t.dtype} (float32, float16 or bfloat16)")
+    return _DTYPES[t.dtype]
+
+
+def _raw(t):
+    return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+def _rows(x):
+    """x with its last axis contiguous; every other axis may have any stride."""
+    return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+def _like_order(ref, B, T, H, D):
+    """An empty [B][T][H][D] tensor in ref's order of the batch and token axes (rollout buffers are
+    time-major)."""
+    if ref.dim() == 4 and B > 1 and T > 1 and ref.stride(0) < ref.stride(1):
+        return torch.empty((T, B, H, D), dtype=ref.dtype, device=ref.device).transpose(0, 1)
+    return torch.empty((B, T, H, D), dtype=ref.dtype, device=ref.device)
+
+
+def _la_flags(what, reset, lengths, B, T):
+    if reset is not None:
+        if reset.dtype == torch.bool:
+            reset = reset.view(torch.uint8)
+        want = (B,) if T is None else (B, T)
+        if reset.dtype != torch.uint8 or tuple(reset.shape) != want:
+            raise RLPError(f"{what}: reset {reset.dtype} {tuple(reset.shape)}, uint8 or bool {want} needed")
+    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,)):
+        raise RLPError(f"{what}: lengths {lengths.dtype} {tuple(lengths.shape)}, int32 ({B},) needed")
+    return reset, None if lengths is None else lengths.contiguous()
+
+
+def _la_cfg(what, q, k, v, log_decay, scale, state):
+    """rlp_la_cfg of q, k, v [B][T][heads][D] after the checks that need no device."""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise RLPError(f"{what}: {name} of {t.dim()} axes")
+        if t.dtype != q.dtype:
+            raise RLPError(f"{what}: {name} is {t.dtype}, q {q.dtype}")
+    B, T, Hq, Dk = q.shape
+    if k.shape[:2] != q.shape[:2] or v.shape[:2] != q.shape[:2] or k.shape[3] != Dk:
+        raise RLPError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    Hk, Hv, Dv = k.shape[2], v.shape[2], v.shape[3]
+    if log_decay.dim() != 1 or log_decay.dtype != torch.float32:
+        raise RLPError(f"{what}: log_decay {log_decay.dtype} {tuple(log_decay.shape)}, float32 (heads,) needed")
+    H = log_decay.shape[0]
+    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (B, H, Dk, Dv)):
+        raise RLPError(f"{what}: state {state.dtype} {tuple(state.shape)}, float32 {(B, H, Dk, Dv)} needed")
+    c = _abi.LACfg()
+    c.dtype = _dtype_of(what, q)
+    c.B, c.T, c.H, c.Hq, c.Hk, c.Hv, c.Dk, c.Dv = B, T, H, Hq, Hk, Hv, Dk, Dv
+    c.scale = float(Dk ** -0.5 if scale is None else scale)
+    need = int(lib().rlp_linear_attention_workspace_bytes(C.byref(c), 0))
+    check(need if need < 0 else 0, what)
+    return c
+
+
+def _set_strides(c, **tensors):
+    for name, t in tensors.items():
+        if t is not None:
+            setattr(c, name + "_stride", type(getattr(c, name + "_stride"))(*t.stride()[:3]))
+
+
+def _la_workspace(c, backward, dev):
+    need = int(lib().rlp_linear_attention_workspace_bytes(C.byref(c), int(backward)))
+    check(need if need < 0 else 0, "rlp_linear_attention_workspace_bytes")
+    return torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None, need
+
+
+def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=None, lengths=None,
+                             return_state=False):
+    """rlp_linear_attention without autograd (arguments as linear_attention): (out, state or None)."""
+    what = "linear_attention"
+    c = _la_cfg(what, q, k, v, log_decay, scale, state)
+    reset, lengths = _la_flags(what, reset, lengths, c.B, c.T)
+    dev = _on_gpu(what, q=q, k=k, v=v, log_decay=log_decay, state=state, reset=reset, lengths=lengths)
+    with torch.cuda.device(dev):
+        q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+        state = state.contiguous() if state is not None else None
+        out = _like_order(q, c.B, c.T, c.H, c.Dv)
+        last = torch.empty((c.B, c.H, c.Dk, c.Dv), dtype=torch.float32, device=dev) if return_state else None
+        _set_strides(c, q=q, k=k, v=v, o=out)
+        if reset is not None:
+            c.reset_stride[:] = reset.stride()
+        ws, need = _la_workspace(c, False, dev)
+        check(lib().rlp_linear_attention(C.byref(c), _raw(q), _raw(k), _raw(v), _raw(log_decay),
+                                         _raw(reset), _raw(lengths), _raw(state), _raw(out), _raw(last),
+                                         _raw(ws), need, stream_ptr()), "rlp_linear_attention")
+    return out, last
+
+
+def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, state=None, reset=None,
+                              lengths=None):
+    """rlp_linear_attention_backward: (dq, dk, dv, gradient of state or None) from the gradients of
+    linear_attention's out and state (d_state None: 0)."""
+    what = "linear_attention_backward"
+    c = _la_cfg(what, q, k, v, log_decay, scale, state)
+    reset, lengths = _la_flags(what, reset, lengths, c.B, c.T)
+    if tuple(d_out.shape) != (c.B, c.T, c.H, c.Dv) or d_out.dtype != q.dtype:
+        raise RLPError(f"{what}: d_out {d_out.dtype} {tuple(d_out.shape)}")
+    if d_state is not None and (d_state.dtype != torch.float32 or
+                                tuple(d_state.shape) != (c.B, c.H, c.Dk, c.Dv)):
+        raise RLPError(f"{what}: d_state {d_state.dtype} {tuple(d_state.shape)}")
+    dev = _on_gpu(what, q=q, k=k, v=v, log_decay=log_decay, state=state, reset=reset, lengths=lengths,
+                  d_out=d_out, d_state=d_state)
+    with torch.cuda.device(dev):
+        q, k, v, d_out, log_decay = _rows(q), _rows(k), _rows(v), _rows(d_out), log_decay.contiguous()
+        first = torch.empty((c.B, c.H, c.Dk, c.Dv), dtype=torch.float32, device=dev) \
+            if state is not None else None
+        state = state.contiguous() if state is not None else None
+        d_state = d_state.contiguous() if d_state is not None else None
+        dq, dk = _like_order(q, c.B, c.T, c.Hq, c.Dk), _like_order(k, c.B, c.T, c.Hk, c.Dk)
+        dv = _like_order(v, c.B, c.T, c.Hv, c.Dv)
+        _set_strides(c, q=q, k=k, v=v, o=d_out, dq=dq, dk=dk, dv=dv)
+        if reset is not None:
+            c.reset_stride[:] = reset.stride()
+        ws, need = _la_workspace(c, True, dev)
+        check(lib().rlp_linear_attention_backward(
+            C.byref(c), _raw(q), _raw(k), _raw(v), _raw(log_decay), _raw(reset), _raw(lengths),
+            _raw(state), _raw(d_out), _raw(d_state), _raw(dq), _raw(dk), _raw(dv), _raw(first), _raw(ws),
+            need, stream_ptr()), "rlp_linear_attention_backward")
+    return dq, dk, dv, first
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, scale, state, reset, lengths, return_state):
+        out, last = linear_attention_forward(q, k, v, log_decay, scale, state, reset, lengths, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, reset, lengths)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return (out, last) if return_state else out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, d_state=None):
+        q, k, v, log_decay, state, reset, lengths = ctx.saved_tensors
+        if d_out is None:
+            if d_state is None:
+                return (None,) * 9
+            d_out = _like_order(q, q.shape[0], q.shape[1], log_decay.shape[0], v.shape[3]).zero_()
+        dq, dk, dv, first = linear_attention_backward(d_out, d_state, q, k, v, log_decay, ctx.scale, state,
+                                                      reset, lengths)
+        return dq, dk, dv, None, None, first, None, None, None
+
+
+def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, lengths=None,
+                     return_state=False):
+    """Linear attention with one decay per head, a policy's memory over a rollout segment or a prompt:
+    S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, out_t = scale * q_t S_t (include/rlp.h
+    rlp_linear_attention). Differentiable in q, k, v and state.
+
+    q, k [B][T][heads][Dk], v [B][T][heads][Dv] (float32, float16 or bfloat16; 1 to 128 wide; each may
+    have fewer heads than log_decay [H], which its heads divide; any strides, so a time-major buffer
+    [T][n] goes in as x.transpose(0, 1)). log_decay: float32, <= 0, a constant of the layer.
+    scale: None for Dk ** -0.5. state: float32 [B][H][Dk][Dv] before the first token (None: 0).
+    reset: uint8 / bool [B][T], nonzero where a token begins an episode (the done flags of the step
+    before). lengths: int32 [B] on the device, tokens of a padded batch; rows behind them give 0.
+    Returns out [B][T][H][Dv], with return_state also the float32 state behind the last token.
+
+    In a captured HIP graph, capture forward and backward together, with no graph of the same leaves
+    alive from outside the capture (torch keeps one accumulation node per leaf and its stream)."""
+    if torch.is_grad_enabled() and log_decay.requires_grad:
+        raise RLPError("linear_attention: log_decay has no gradient (pass it detached)")
+    return _LinearAttention.apply(q, k, v, log_decay, scale, state, reset, lengths, bool(return_state))
+
+
+def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, state_out=None, out=None):
+    """linear_attention for one token of every sequence, for acting: q, k [B][heads][Dk],
+    v [B][heads][Dv], state float32 [B][H][Dk][Dv] contiguous, updated in place or written to state_out;
+    reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv]. Not differentiable."""
+    what = "linear_attention_step"
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RLPError(f"{what}: not differentiable (call it under torch.no_grad, or linear_attention)")
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 3:
+            raise RLPError(f"{what}: {name} of {t.dim()} axes")
+    c = _la_cfg(what, q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), log_decay, scale, state)
+    reset, _ = _la_flags(what, reset, None, c.B, None)
+    state_out = state if state_out is None else state_out
+    shape = (c.B, c.H, c.Dv)
+    if state_out.shape != state.shape or state_out.dtype != torch.float32:
+        raise RLPError(f"{what}: state_out {state_out.dtype} {tuple(state_out.shape)}")
+    if not state.is_contiguous() or not state_out.is_contiguous():
+        raise RLPError(f"{what}: state and state_out have to be contiguous")
+    lo, n = state.data_ptr(), 4 * state.numel()
+    if state_out.data_ptr() != lo and abs(state_out.data_ptr() - lo) < n:
+        raise RLPError(f"{what}: state_out overlaps state (pass state itself for an update in place)")
+    if out is not None and (tuple(out.shape) != shape or out.dtype != q.dtype or not out.is_contiguous()):
+        raise RLPError(f"{what}: out {out.dtype} {tuple(out.shape)}, contiguous {q.dtype} {shape} needed")
+    dev = _on_gpu(what, q=q, k=k, v=v, log_decay=log_decay, state=state, state_out=state_out, reset=reset,
+                  out=out)
+    with torch.cuda.device(dev):
+        q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+        out = torch.empty(shape, dtype=q.dtype, device=dev) if out is None else out
+        for name, t in (("q", q), ("k", k), ("v", v), ("o", out)):
+            getattr(c, name + "_stride")[:] = (t.stride(0), 0, t.stride(1))
+        if reset is not None:
+            c.reset_stride[0] = reset.stride(0)
+        check(lib().rlp_linear_attention_step(C.byref(c), _raw(q), _raw(k), _raw(v), _raw(log_decay),
+                                              _raw(reset), _raw(state), _raw(state_out), _raw(out),
+                                              stream_ptr()), "rlp_linear_attention_step")
+    return out
+
+
+def token_logprob_forward(logits, tokens, temperature=1.0, top_k=0):
+    """rlp_token_logprob without autograd on logits [rows][vocab], tokens [rows] int64: (logp, entropy,
+    stats, top_logp, top_tokens); stats feeds token_logprob_backward, top_* are None for top_k 0."""
+    what = "token_logprob"
+    if logits.dim() != 2 or tuple(tokens.shape) != (logits.shape[0],) or tokens.dtype != torch.int64:
+        raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
+    dev, dt, top_k = _on_gpu(what, logits=logits, tokens=tokens), _dtype_of(what, logits), int(top_k)
+    rows, vocab = logits.shape
+    need = int(lib().rlp_token_logprob_workspace_bytes(rows, vocab, top_k, dt))
+    check(need if need < 0 else 0, what)
+    with torch.cuda.device(dev):
+        logits, tokens = _rows(logits), tokens.contiguous()
+        f32 = dict(dtype=torch.float32, device=dev)
+        logp, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
+        stats = torch.empty((rows, 3), **f32)
+        top_logp = torch.empty((rows, top_k), **f32) if top_k else None
+        top_tokens = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+        check(lib().rlp_token_logprob(_raw(logits), dt, rows, vocab, logits.stride(0), _raw(tokens),
+                                      float(temperature), top_k, _raw(logp), _raw(entropy), _raw(stats),
+                                      _raw(top_logp), _raw(top_tokens), _raw(ws), need, stream_ptr()),
+              "rlp_token_logprob")
+    return logp, entropy, stats, top_logp, top_tokens
+
+
+def token_logprob_backward(d_logp, d_entropy, logits, tokens, stats, temperature=1.0):
+    """rlp_token_logprob_backward: the gradient of logits from those of logp and entropy (None: 0)."""
+    what = "token_logprob_backward"
+    rows, vocab = logits.shape
+    for name, t in (("d_logp", d_logp), ("d_entropy", d_entropy)):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (rows,)):
+            raise RLPError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, float32 ({rows},) needed")
+    if tuple(stats.shape) != (rows, 3) or stats.dtype != torch.float32 or tokens.dtype != torch.int64 or \
+            tuple(tokens.shape) != (rows,):
+        raise RLPError(f"{what}: stats {tuple(stats.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
+    dev, dt = _on_gpu(what, logits=logits, tokens=tokens, stats=stats, d_logp=d_logp,
+                      d_entropy=d_entropy), _dtype_of(what, logits)
+    with torch.cuda.device(dev):
+        logits, tokens, stats = _rows(logits), tokens.contiguous(), stats.contiguous()
+        d_logp = d_logp.contiguous() if d_logp is not None else None
+        d_entropy = d_entropy.contiguous() if d_entropy is not None else None
+        d_logits = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+        check(lib().rlp_token_logprob_backward(_raw(logits), dt, rows, vocab, logits.stride(0), _raw(tokens),
+                                               float(temperature), _raw(stats), _raw(d_logp),
+                                               _raw(d_entropy), _raw(d_logits), vocab, stream_ptr()),
+              "rlp_token_logprob_backward")
+    return d_logits
+
+
+class _TokenLogprob(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, temperature, top_k):
+        logp, entropy, stats, top_logp, top_tokens = token_logprob_forward(logits, tokens, temperature, top_k)
+        ctx.save_for_backward(logits, tokens, stats)
+        ctx.temperature = temperature
+        ctx.set_materialize_grads(False)
+        if not top_k:
+            return logp, entropy
+        ctx.mark_non_differentiable(top_logp, top_tokens)
+        return logp, entropy, top_logp, top_tokens
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_logp, d_entropy, *_):
+        if d_logp is None and d_entropy is None:
+            return None, None, None, None
+        logits, tokens, stats = ctx.saved_tensors
+        return token_logprob_backward(d_logp, d_entropy, logits, tokens, stats, ctx.temperature), None, None, None
+
+
+def token_logprob(logits, tokens, temperature=1.0, top_k=0):
+    """Log-probability of the given tokens (discrete actions) and the entropy of their distributions
+    softmax(logits / temperature): the two terms of a PPO2 actor loss over tokens (include/rlp.h
+    rlp_token_logprob). Differentiable in logits.
+
+    logits [...][vocab] float32, float16 or bfloat16; tokens [...] int64 or int32, negative: a padded
+    row (0 everywhere, no gradient). -inf logits are actions that are not allowed.
+    Returns (logp, entropy), float32 of tokens' shape; with top_k (1 to 32) also the top_k most
+    probable tokens, (logp, entropy, top_logp, top_tokens [...][top_k]), ties to the lower token; those
+    two carry no gradient."""
+    what = "token_logprob"
+    if logits.dim() < 1 or tuple(tokens.shape) != tuple(logits.shape[:-1]):
+        raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tuple(tokens.shape)}")
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise RLPError(f"{what}: tokens {tokens.dtype} (int64 or int32)")
+    shape, vocab = tuple(tokens.shape), logits.shape[-1]
+    if vocab < 1:
+        raise RLPError(f"{what}: no logits in a row")
+    res = _TokenLogprob.apply(logits.reshape(-1, vocab), tokens.reshape(-1).long(), float(temperature),
+                              int(top_k))
+    return tuple(r.view(shape if r.dim() == 1 else shape + (int(top_k),)) for r in res)

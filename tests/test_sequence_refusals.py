@@ -1,0 +1,154 @@
+"""Refusals of the sequence-policy operators (linear attention, token log-probabilities): bad arguments
+come back as RLPError / a status code on the host, before any launch."""
+import ctypes as C
+
+import pytest
+import torch
+
+from reinforcementlearningplatform_amd import _abi, _native
+from reinforcementlearningplatform_amd import kernels as K
+from reinforcementlearningplatform_amd._native import RLPError
+
+DEV = C.c_void_p(1 << 20)  # never dereferenced: the calls must fail before any launch
+
+
+def la(**over):
+    c = _abi.LACfg()
+    for name, v in dict(dtype=0, B=2, T=8, H=4, Hq=4, Hk=4, Hv=4, Dk=16, Dv=16, scale=1.0, **over).items():
+        setattr(c, name, v)
+    return c
+
+
+def la_forward(c, q=DEV, ld=DEV, out=DEV, ws=None, nb=0):
+    return _native.lib().rlp_linear_attention(C.byref(c), q, DEV, DEV, ld, None, None, None, out, None, ws,
+                                              nb, None)
+
+
+@pytest.mark.parametrize("over, word", [
+    (dict(dtype=3), b"dtype"), (dict(B=-1), b"B -1"), (dict(T=-1), b"T -1"), (dict(H=0), b"H 0"),
+    (dict(Hq=3), b"divide"), (dict(Hk=0), b"divide"), (dict(Hv=8), b"divide"), (dict(Dk=0), b"Dk 0"),
+    (dict(Dk=129), b"Dk 129"), (dict(Dv=129), b"Dv 129"), (dict(B=1 << 30, H=4, T=1), b"too large")])
+def test_linear_attention_cfg_is_checked(over, word):
+    base = dict(dtype=0, B=2, T=8, H=4, Hq=4, Hk=4, Hv=4, Dk=16, Dv=16, scale=1.0)
+    c = _abi.LACfg()
+    for name, v in {**base, **over}.items():
+        setattr(c, name, v)
+    lib = _native.lib()
+    assert la_forward(c) == _abi.RLP_EINVAL and word in lib.rlp_last_error_string()
+    assert lib.rlp_linear_attention_workspace_bytes(C.byref(c), 1) == _abi.RLP_EINVAL
+    assert lib.rlp_linear_attention_backward(C.byref(c), *[DEV] * 14, 1 << 40, None) == _abi.RLP_EINVAL
+    c.T = 1 if c.T == 8 else c.T
+    assert lib.rlp_linear_attention_step(C.byref(c), *[DEV] * 8, None) == _abi.RLP_EINVAL
+
+
+def test_linear_attention_nulls_and_workspace():
+    lib = _native.lib()
+    c = la()
+    assert la_forward(c, q=None) == _abi.RLP_EINVAL and b"null" in lib.rlp_last_error_string()
+    assert la_forward(c, ld=None) == _abi.RLP_EINVAL
+    assert la_forward(c, out=None) == _abi.RLP_EINVAL
+    assert lib.rlp_linear_attention(None, *[DEV] * 10, 0, None) == _abi.RLP_EINVAL
+    assert lib.rlp_linear_attention_step(C.byref(c), *[DEV] * 8, None) == _abi.RLP_EINVAL   # T = 8
+    assert b"one token" in lib.rlp_last_error_string()
+    # long sequences of few heads are split: their segments' states need scratch
+    c = la()
+    c.B, c.T = 1, 4096
+    need = lib.rlp_linear_attention_workspace_bytes(C.byref(c), 0)
+    assert need > 0
+    assert la_forward(c, ws=DEV, nb=need - 1) == _abi.RLP_EINVAL
+    assert b"workspace" in lib.rlp_last_error_string()
+    assert la_forward(c, ws=None, nb=0) == _abi.RLP_EINVAL
+    # shared heads: the backward's f32 partials on top
+    c.Hq = 1
+    assert lib.rlp_linear_attention_workspace_bytes(C.byref(c), 1) >= need + 4 * 4096 * 4 * 16
+    c = la()
+    c.B = 0
+    assert la_forward(c) == 0 and lib.rlp_linear_attention_workspace_bytes(C.byref(c), 1) == 0
+
+
+@pytest.mark.parametrize("over, word", [
+    (dict(dtype=7), b"dtype"), (dict(rows=-1), b"rows"), (dict(vocab=0), b"vocab"),
+    (dict(vocab=1 << 31), b"vocab"), (dict(stride=-1), b"stride"), (dict(temperature=0.0), b"temperature"),
+    (dict(temperature=-1.0), b"temperature"), (dict(temperature=float("nan")), b"temperature"),
+    (dict(temperature=float("inf")), b"temperature"), (dict(top=-1), b"top_k"), (dict(top=33), b"top_k"),
+    (dict(vocab=5, top=6), b"top_k"), (dict(logits=None), b"null"), (dict(top_tokens=None, top=2), b"null")])
+def test_token_logprob_arguments_are_checked(over, word):
+    a = {**dict(logits=DEV, dtype=0, rows=4, vocab=100, stride=100, temperature=1.0, top=0, top_tokens=DEV),
+         **over}
+    lib = _native.lib()
+    rc = lib.rlp_token_logprob(a["logits"], a["dtype"], a["rows"], a["vocab"], a["stride"], DEV,
+                               a["temperature"], a["top"], DEV, DEV, DEV, DEV, a["top_tokens"], None, 0, None)
+    assert rc == _abi.RLP_EINVAL and word in lib.rlp_last_error_string()
+
+
+def test_token_logprob_workspace_and_backward_rows():
+    lib = _native.lib()
+    need = lib.rlp_token_logprob_workspace_bytes(8, 50257, 20, _abi.RLP_BF16)
+    assert need > 0
+    for ws, nb in ((None, 0), (DEV, need - 1)):
+        assert lib.rlp_token_logprob(DEV, _abi.RLP_BF16, 8, 50257, 50257, DEV, 1.0, 20, DEV, DEV, DEV, DEV, DEV,
+                                     ws, nb, None) == _abi.RLP_EINVAL
+        assert b"workspace" in lib.rlp_last_error_string()
+    assert lib.rlp_token_logprob_workspace_bytes(8, 18, 4, 0) == 0
+    assert lib.rlp_token_logprob_workspace_bytes(65536, 50257, 4, 0) == 0
+    assert lib.rlp_token_logprob_backward(DEV, 0, 4, 100, 100, DEV, 1.0, DEV, DEV, DEV, DEV, 99, None) \
+        == _abi.RLP_EINVAL and b"overlap" in lib.rlp_last_error_string()
+    assert lib.rlp_token_logprob_backward(DEV, 0, 4, 100, 100, DEV, 1.0, None, DEV, DEV, DEV, 100, None) \
+        == _abi.RLP_EINVAL
+    assert lib.rlp_token_logprob(DEV, 0, 0, 100, 100, DEV, 1.0, 0, DEV, DEV, None, None, None, None, 0,
+                                 None) == 0   # no rows: nothing launched
+
+
+def qkv(B=2, T=8, H=2, D=4, dtype=torch.float32):
+    return [torch.zeros(B, T, H, D, dtype=dtype) for _ in range(3)] + [torch.zeros(H)]
+
+
+def test_linear_attention_wrapper_refusals():
+    q, k, v, ld = qkv()
+    for args, kw, word in [
+            ((q, k, v, ld), {}, "not on the GPU"),
+            ((q.double(), k.double(), v.double(), ld), {}, "dtype"),
+            ((q, k.half(), v, ld), {}, "k is"),
+            ((q[0], k, v, ld), {}, "axes"),
+            ((q, k[:, :4], v, ld), {}, "q "),
+            ((q, k[..., :3], v, ld), {}, "q "),
+            ((q, k, v, ld.double()), {}, "log_decay"),
+            ((q, k, v, torch.zeros(3)), {}, "divide"),
+            ((q, k, v, ld), dict(state=torch.zeros(2, 2, 4, 5)), "state"),
+            ((q, k, v, ld), dict(state=torch.zeros(2, 2, 4, 4).half()), "state"),
+            ((q, k, v, ld), dict(reset=torch.zeros(8, 2, dtype=torch.uint8)), "reset"),
+            ((q, k, v, ld), dict(reset=torch.zeros(2, 8)), "reset"),
+            ((q, k, v, ld), dict(lengths=torch.zeros(2, dtype=torch.int64)), "lengths"),
+            ((q, k, v, ld.clone().requires_grad_()), {}, "log_decay")]:
+        with pytest.raises(RLPError, match=word):
+            K.linear_attention(*args, **kw)
+
+
+def test_linear_attention_step_wrapper_refusals():
+    q, k, v, ld = [t[:, 0] if t.dim() == 4 else t for t in qkv()]
+    st = torch.zeros(2, 2, 4, 4)
+    big = torch.zeros(3, 2, 4, 4)
+    for args, kw, word in [
+            ((q, k, v, ld, st), {}, "not on the GPU"),
+            ((q.unsqueeze(1), k, v, ld, st), {}, "axes"),
+            ((q, k, v, ld, st.half()), {}, "state"),
+            ((q, k, v, ld, st.transpose(2, 3)), {}, "contiguous"),
+            ((q, k, v, ld, st), dict(state_out=torch.zeros(2, 2, 4, 3)), "state_out"),
+            ((q, k, v, ld, big[:2]), dict(state_out=big[1:]), "overlaps"),
+            ((q, k, v, ld, st), dict(reset=torch.zeros(2, 1, dtype=torch.uint8)), "reset"),
+            ((q, k, v, ld, st), dict(out=torch.zeros(2, 2, 5)), "out"),
+            ((q.clone().requires_grad_(), k, v, ld, st), {}, "not differentiable")]:
+        with pytest.raises(RLPError, match=word):
+            K.linear_attention_step(*args, **kw)
+
+
+def test_token_logprob_wrapper_refusals():
+    l, t = torch.zeros(3, 5), torch.zeros(3, dtype=torch.int64)
+    for args, kw, word in [
+            ((l, t), {}, "not on the GPU"),
+            ((l, t[:2]), {}, "tokens"),
+            ((l, t.float()), {}, "int64"),
+            ((torch.zeros(3, 0), t), {}, "no logits"),
+            ((l.double(), t), {}, "GPU|dtype")]:
+        with pytest.raises(RLPError, match=word):
+            K.token_logprob(*args, **kw)
