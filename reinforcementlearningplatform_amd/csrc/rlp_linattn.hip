@@ -11,6 +11,8 @@
 // so one kernel computes all of them. It walks a sequence in chunks: within a chunk the decayed,
 // masked products P = X Y^T times Z, before it lam^(i+1) x_i S with the state S = sum_j y_j z_j^T
 // of what came before, S [dx][dz] held in the MFMA accumulators of the block for the whole walk.
+#include <type_traits>
+
 #include "rlp_common.hpp"
 
 namespace rlp {
@@ -59,6 +61,15 @@ __device__ __forceinline__ float decay_pow(float lam2, int n) {
     return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(lam2 * (float)n);
 }
 
+// The value as if computed anew: keeps what a loop derives from lane numbers and powers inside the loop.
+// Hoisted, those invariants (addresses, comparisons, products of powers) took 200 registers more than a
+// wave has and went to scratch.
+template <typename T>
+__device__ __forceinline__ T anew(T v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // Highest set bit of m at or below i (the chunk position where i's episode begins), -1: none.
 __device__ __forceinline__ int begin_of(uint32_t m, int i) {
     const uint32_t below = m & (0xFFFFFFFFu >> (31 - i));
@@ -68,11 +79,10 @@ __device__ __forceinline__ int begin_of(uint32_t m, int i) {
 // C rows of D = 32 * DB columns into LDS as f32; rows >= n and columns >= d are 0. 16-byte loads
 // (any alignment), the last columns of an odd d one by one. Returns whether a value is inf or NaN.
 template <typename T, int DB, int C, int NT>
-__device__ __forceinline__ bool stage(float (*dst)[32 * DB + 4], const T *src, int64_t st, int n, int d,
-                                      bool look) {
+__device__ __forceinline__ bool stage(float (*dst)[32 * DB + 4], const T *src, int64_t st, int n, int d) {
     constexpr int VE = 16 / sizeof(T);
     constexpr int VR = 32 * DB / VE;  // vectors per row
-    bool bad = false;
+    uint32_t most = 0;
 #pragma unroll
     for (int it = 0; it < (C * VR + NT - 1) / NT; ++it) {
         const int id = it * NT + (int)threadIdx.x;
@@ -93,16 +103,14 @@ __device__ __forceinline__ bool stage(float (*dst)[32 * DB + 4], const T *src, i
                 for (int e = 0; e < VE; ++e)
                     if (c + e < d) f[e] = to_f32(p[e]);
             }
-            if (look) {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) bad |= (__float_as_uint(f[e]) & 0x7F800000u) == 0x7F800000u;
-            }
+            for (int e = 0; e < VE; ++e) most = max(most, __float_as_uint(f[e]) & 0x7FFFFFFFu);
         }
 #pragma unroll
         for (int e = 0; e < VE; e += 4)
             *(floatx4 *)&dst[row][c + e] = (floatx4){f[e], f[e + 1], f[e + 2], f[e + 3]};
     }
-    return bad;
+    return most >= 0x7F800000u;
 }
 
 // The walk in exact f32 products (v_mfma_f32_32x32x2_f32 / 16x16x4_f32). A block of NW waves owns
@@ -117,6 +125,7 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
     __shared__ __align__(16) float ys[C][DX + 4];
     __shared__ __align__(16) float zs[C][DZ + 4];
     __shared__ __align__(16) float ps[C][C + 4];
+    __shared__ int bad_s, first_s;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -149,23 +158,33 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
             }
     }
     bool seg_cut = false;
+    if (threadIdx.x == 0) bad_s = -1;
     for (int pos = p0; pos < p1;) {
         int n = min(C, p1 - pos);
         uint32_t cuts = (uint32_t)__ballot(lane < n && cut_at(a, b, pos + lane, len));
         __syncthreads();  // the chunk before is done with the tiles
-        const bool look = (cuts & ~1u) != 0;
-        bool bad = false;
-        if (want_out) stage<T, DXB, C, NT>(xs, x + pos * dir * a.xt, dir * a.xt, n, a.dx, false);
-        bad |= stage<T, DXB, C, NT>(ys, y + pos * dir * a.yt, dir * a.yt, n, a.dx, look);
-        bad |= stage<T, NW, C, NT>(zs, z + pos * dir * a.zt, dir * a.zt, n, a.dz, look);
-        bool alone = false;
-        if (look) alone = __syncthreads_or(bad);
-        else __syncthreads();
-        if (alone) {
-            // An inf or NaN of one episode would reach the next through 0 * x in the products: this
-            // chunk ends where the next episode begins, the rows behind it are cleared.
-            n = __builtin_ctz(cuts & ~1u);
-            cuts &= 1u;
+        if (want_out) stage<T, DXB, C, NT>(xs, x + pos * dir * a.xt, dir * a.xt, n, a.dx);
+        bool bad = stage<T, DXB, C, NT>(ys, y + pos * dir * a.yt, dir * a.yt, n, a.dx);
+        bad |= stage<T, NW, C, NT>(zs, z + pos * dir * a.zt, dir * a.zt, n, a.dz);
+        if (bad) bad_s = pos;
+        __syncthreads();
+        if (bad_s == pos) {
+            // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
+            // chunk ends before a row that holds one, and such a row's chunk before the next episode.
+            if (threadIdx.x == 0) first_s = n;
+            __syncthreads();
+            bool head = false;
+            for (int j = 0; j < n; ++j) {
+                bool b2 = false;
+                for (int c = threadIdx.x; c < DX; c += NT) b2 |= (__float_as_uint(ys[j][c]) & 0x7F800000u) == 0x7F800000u;
+                for (int c = threadIdx.x; c < DZ; c += NT) b2 |= (__float_as_uint(zs[j][c]) & 0x7F800000u) == 0x7F800000u;
+                if (j == 0) head = __syncthreads_or(b2);
+                else if (b2) atomicMin(&first_s, j);
+            }
+            __syncthreads();
+            n = first_s;
+            if (head && (cuts & ~1u)) n = min(n, (int)__builtin_ctz(cuts & ~1u));
+            cuts &= 0xFFFFFFFFu >> (32 - n);
             for (int id = threadIdx.x; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0.0f;
             for (int id = threadIdx.x; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0.0f;
             __syncthreads();
@@ -246,6 +265,394 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
     if (a.mode == 1) dst = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, da = a.dz, dn = 1;
     if (dst) {
         // walking backward, what is left belongs to the state before token 0
+        const bool drop = a.mode == 0 && a.rev && a.reset && len > 0 && a.reset[b * a.rb] != 0;
+#pragma unroll
+        for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
+                if (row < a.dx && col < a.dz) dst[row * da + col * dn] = drop ? 0.0f : S[ab][r];
+            }
+    }
+    if (a.mode == 1 && threadIdx.x == 0)
+        a.segf[(int64_t)bh * a.nseg + g] = seg_cut ? -1.0f : decay_pow(lam2, max(p1 - p0, 0));
+}
+
+// ------------------------------------------------------------------------------------------
+// The walk on bfloat16 operands
+// ------------------------------------------------------------------------------------------
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {  // two roundings to nearest even
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){a, b}, bf16x2));
+}
+__device__ __forceinline__ float lo_half(uint32_t v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float hi_half(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
+
+// Eight f32 values as the sum of N bf16 operands: each piece takes what the pieces before left over,
+// so two pieces hold a value to 2^-16 and three to 2^-24 of itself.
+template <int N>
+__device__ __forceinline__ void split8(const float *v, bf16x8 (&out)[N]) {
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rest[e] = v[e];
+#pragma unroll
+    for (int p = 0; p < N; ++p) {
+        uintx4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[e] = pack2(rest[2 * e], rest[2 * e + 1]);
+            if (p + 1 < N) {
+                rest[2 * e] -= lo_half(w[e]);
+                rest[2 * e + 1] -= hi_half(w[e]);
+            }
+        }
+        out[p] = __builtin_bit_cast(bf16x8, w);
+    }
+}
+
+__device__ __forceinline__ floatx16 mfma_bf16(bf16x8 a, bf16x8 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int begin_of64(uint64_t m, int i) {
+    const uint64_t below = m & (~0ull >> (63 - i));
+    return below ? 63 - __builtin_clzll(below) : -1;
+}
+
+// 64 rows of D bf16 columns on their way from global memory to LDS: 16 bytes a thread and step.
+template <int D, int NT>
+struct Rows16 {
+    static constexpr int VR = D / 8, N = 64 * VR / NT;
+    uintx4 v[N];
+    // d: a multiple of 8, so a vector is wholly inside the row or behind it
+    __device__ __forceinline__ void load(const __bf16 *src, int64_t st, int n, int d, int tid) {
+        const int row = tid / VR, c = tid % VR * 8;
+        const __bf16 *p = src + row * st + c;
+        const bool in = c < d;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            v[k] = (uintx4){0, 0, 0, 0};
+            if (in && row + k * (NT / VR) < n) __builtin_memcpy(&v[k], p + k * (NT / VR) * st, 16);
+        }
+    }
+    // PERM: within 16 columns the order 0-3, 8-11, 4-7, 12-15, in which a half wave's 8 columns are
+    // 16 bytes and match the rows of an accumulator (see the kernel).
+    template <bool PERM, int P>
+    __device__ __forceinline__ void store(unsigned short (*dst)[P], int tid) const {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int id = k * NT + tid, row = id / VR, c = id % VR * 8;
+            if (PERM) {
+                const int at = (c & ~15) + (c & 8) / 2;
+                *(uintx2 *)&dst[row][at] = (uintx2){v[k][0], v[k][1]};
+                *(uintx2 *)&dst[row][at + 8] = (uintx2){v[k][2], v[k][3]};
+            } else {
+                *(uintx4 *)&dst[row][c] = v[k];
+            }
+        }
+    }
+    __device__ __forceinline__ bool not_finite() const {
+        ushortx2 m = {0, 0};
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(ushortx2, v[k][e] & 0x7FFF7FFFu));
+        return m[0] >= 0x7F80 || m[1] >= 0x7F80;
+    }
+};
+
+// Four rows j0 + 4 (lane >> 5) .. + 3 of column c0 + (lane & 31): the transposing LDS read, 16 lanes
+// giving the addresses of 4 rows x 16 columns and getting a column each.
+template <bool PERM, int P>
+__device__ __forceinline__ uintx2 column4(const unsigned short (*t)[P], int j0, int c0, int lane) {
+    const int row = j0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int q = lane & 3, c = c0 + (lane & 16) + 4 * (PERM ? (q >> 1) | (q & 1) << 1 : q);
+    typedef __attribute__((address_space(3))) shortx4 *lds4;
+    return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)&t[row][c]));
+}
+template <bool PERM, int P>
+__device__ __forceinline__ uintx4 column16(const unsigned short (*t)[P], int j0, int c0, int lane) {
+    const uintx2 a = column4<PERM>(t, j0, c0, lane), b = column4<PERM>(t, j0 + 8, c0, lane);
+    return (uintx4){a[0], a[1], b[0], b[1]};
+}
+
+// la_walk_kernel for bf16 operands on v_mfma_f32_32x32x16_bf16, 64 tokens a chunk. Products of the
+// operands are exact in f32; what is not an operand is split into bf16 pieces where it meets the
+// matrix cores: P and S for the output into two (2^-16, below the output's own rounding), the
+// weighted z of the state's sum into three (2^-24), so that the state stays an f32 state.
+//
+// A 32x32 accumulator holds rows 8 (r >> 2) + 4 (lane >> 5) + (r & 3) of column lane & 31, so eight of
+// its registers are the operand of 16 rows in the order 0-3, 8-11 | 4-7, 12-15 of the half waves. With
+// the other operand read in that order (the order of a contraction is free) S goes from accumulator
+// to operand without leaving its wave, and so does P, computed transposed as Y X^T.
+template <int DXB, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void la_walk_bf16_kernel(WalkArgs a) {
+    constexpr int C = 64, DX = 32 * DXB, DZ = 32 * NW, NT = 64 * NW;
+    __shared__ __align__(16) unsigned short xs[C][DX + 16];
+    __shared__ __align__(16) unsigned short ys[C][DX + 16];
+    __shared__ __align__(16) unsigned short zs[C][DZ + 16];
+    __shared__ __align__(16) uintx4 ps[3][2][2][64];
+    __shared__ int bad_s, first_s;
+    int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    const int p0 = g * a.seglen, p1 = min(len, p0 + a.seglen);
+    const float lam2 = a.log_decay[h] * kLog2e;
+    const int64_t tok0 = a.rev ? len - 1 : 0, dir = a.rev ? -1 : 1;
+    const __bf16 *x = (const __bf16 *)a.x + b * a.xb + (h / a.gx) * a.xh + tok0 * a.xt;
+    const __bf16 *y = (const __bf16 *)a.y + b * a.yb + (h / a.gy) * a.yh + tok0 * a.yt;
+    const __bf16 *z = (const __bf16 *)a.z + b * a.zb + (h / a.gz) * a.zh + tok0 * a.zt;
+    const int64_t out0 = b * a.ob + h * a.oh + tok0 * a.ot;
+    const bool want_out = a.mode != 1;
+    const int c0 = 32 * w;
+    int col = c0 + l31;
+    auto put = [&](int64_t at, float v) {
+        if (a.out_f32) ((float *)a.out)[at] = v;
+        else ((__bf16 *)a.out)[at] = (__bf16)v;
+    };
+
+    // powers of lam of an output's rows i = 8 m + 4 half + r
+    float row_m[4], pow_r[4];
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        row_m[m] = a.s2 * decay_pow(lam2, 8 * m + 4 * half + a.e0);
+        pow_r[m] = decay_pow(lam2, m);
+    }
+    const float pow8 = decay_pow(lam2, 8), pow32 = decay_pow(lam2, 32);
+
+    floatx16 S[DXB];
+    {
+        const float *src = nullptr;
+        int64_t ia = a.ia, in = a.in;
+        if (a.mode == 0 && a.init) src = a.init + (int64_t)bh * a.dx * a.dz;
+        if (a.mode == 2) src = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, ia = a.dz, in = 1;
+#pragma unroll
+        for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
+                S[ab][r] = src && row < a.dx && col < a.dz ? src[row * ia + col * in] : 0.0f;
+            }
+    }
+    bool seg_cut = false;
+    if (threadIdx.x == 0) bad_s = -1;
+    Rows16<DX, NT> rx, ry;
+    Rows16<DZ, NT> rz;
+    auto load = [&](int pos) {
+        const int n = min(C, p1 - pos);
+        if (want_out) rx.load(x + pos * dir * a.xt, dir * a.xt, n, a.dx, tid);
+        ry.load(y + pos * dir * a.yt, dir * a.yt, n, a.dx, tid);
+        rz.load(z + pos * dir * a.zt, dir * a.zt, n, a.dz, tid);
+    };
+    if (p0 < p1) load(p0);
+    for (int pos = p0; pos < p1;) {
+        tid = anew(tid), lane = tid & 63, half = lane >> 5, l31 = lane & 31, col = c0 + l31;
+#pragma unroll
+        for (int m = 0; m < 4; ++m) row_m[m] = anew(row_m[m]), pow_r[m] = anew(pow_r[m]);
+        int n = min(C, p1 - pos);
+        uint64_t cuts = __ballot(lane < n && cut_at(a, b, pos + lane, len));
+        __syncthreads();  // the chunk before is done with the tiles
+        if (want_out) rx.template store<true>(xs, tid);
+        ry.template store<true>(ys, tid);
+        rz.template store<false>(zs, tid);
+        if (ry.not_finite() || rz.not_finite()) bad_s = pos;
+        if (pos + n < p1) load(pos + n);
+        __syncthreads();
+        if (bad_s == pos) {
+            // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
+            // chunk ends before a row that holds one, and such a row's chunk before the next episode.
+            if (threadIdx.x == 0) first_s = n;
+            __syncthreads();
+            bool head = false;
+            for (int j = 0; j < n; ++j) {
+                bool bad = false;
+                for (int c = threadIdx.x; c < DX; c += NT) bad |= (ys[j][c] & 0x7F80) == 0x7F80;
+                for (int c = threadIdx.x; c < DZ; c += NT) bad |= (zs[j][c] & 0x7F80) == 0x7F80;
+                if (j == 0) head = __syncthreads_or(bad);
+                else if (bad) atomicMin(&first_s, j);
+            }
+            __syncthreads();
+            n = first_s;
+            if (head && (cuts & ~1ull)) n = min(n, (int)__builtin_ctzll(cuts & ~1ull));
+            cuts &= ~0ull >> (64 - n);
+            for (int id = threadIdx.x; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0;
+            for (int id = threadIdx.x; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0;
+            if (pos + n < p1) load(pos + n);
+            __syncthreads();
+        }
+        const bool two = n > 32;
+        floatx16 O0, O1;
+        if (want_out) {
+            // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in 32 x 32 blocks (j, i), shared out
+            // over the waves and handed to all of them as operands, two pieces each
+            for (int q = w; q < (two ? 3 : 1); q += NW) {
+                const int jb = 32 * (q >> 1), ib = 32 * ((q + 1) >> 1);
+                floatx16 P;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) P[r] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < 2 * DXB; ++s)
+                    P = mfma_bf16(*(const bf16x8 *)&ys[jb + l31][16 * s + 8 * half],
+                                  *(const bf16x8 *)&xs[ib + l31][16 * s + 8 * half], P);
+                const int d0 = ib - jb + l31 - 4 * half;
+                const int j0 = max(0, begin_of64(cuts, ib + l31) - jb - 4 * half);  // of i's episode
+#pragma unroll
+                for (int js = 0; js < 2; ++js) {
+                    float pv[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int j = 16 * js + 8 * (e >> 2) + (e & 3);
+                        const float f = a.s1 * decay_pow(lam2, max(d0 - j, 0));
+                        pv[e] = j <= d0 && j >= j0 ? P[8 * js + e] * f : 0.0f;  // 0 whatever stood there
+                    }
+                    bf16x8 Pp[2];
+                    split8(pv, Pp);
+                    ps[q][js][0][lane] = __builtin_bit_cast(uintx4, Pp[0]);
+                    ps[q][js][1][lane] = __builtin_bit_cast(uintx4, Pp[1]);
+                }
+            }
+            // x S, decayed to each row, where the row's episode is the one that came in
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O0[r] = O1[r] = 0.0f;
+            auto xS = [&](auto both) {
+#pragma unroll
+                for (int s = 0; s < 2 * DXB; ++s) {
+                    bf16x8 Sp[2];
+                    float sv[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sv[e] = S[s / 2][8 * (s & 1) + e];
+                    split8(sv, Sp);
+                    const bf16x8 X0 = *(const bf16x8 *)&xs[l31][16 * s + 8 * half];
+                    O0 = mfma_bf16(X0, Sp[0], O0);
+                    O0 = mfma_bf16(X0, Sp[1], O0);
+                    if (both) {
+                        const bf16x8 X1 = *(const bf16x8 *)&xs[32 + l31][16 * s + 8 * half];
+                        O1 = mfma_bf16(X1, Sp[0], O1);
+                        O1 = mfma_bf16(X1, Sp[1], O1);
+                    }
+                }
+            };
+            if (two) xS(std::true_type{});
+            else xS(std::false_type{});
+            const int first = cuts ? (int)__builtin_ctzll(cuts) : C;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = 8 * (r >> 2) + 4 * half + (r & 3);
+                const float f = row_m[r >> 2] * pow_r[r & 3];
+                O0[r] = i < first ? O0[r] * f : 0.0f;
+                O1[r] = 32 + i < first ? O1[r] * (f * pow32) : 0.0f;
+            }
+            __syncthreads();  // P is there
+#pragma unroll
+            for (int js = 0; js < 2; ++js) {
+                const bf16x8 Z = __builtin_bit_cast(bf16x8, column16<false>(zs, 16 * js, c0, lane));
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    O0 = mfma_bf16(__builtin_bit_cast(bf16x8, ps[0][js][p][lane]), Z, O0);
+                    if (two) O1 = mfma_bf16(__builtin_bit_cast(bf16x8, ps[1][js][p][lane]), Z, O1);
+                }
+            }
+            if (two) {
+#pragma unroll
+                for (int js = 0; js < 2; ++js) {
+                    const bf16x8 Z = __builtin_bit_cast(bf16x8, column16<false>(zs, 32 + 16 * js, c0, lane));
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        O1 = mfma_bf16(__builtin_bit_cast(bf16x8, ps[2][js][p][lane]), Z, O1);
+                }
+            }
+        }
+        // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T over the episode that goes out
+        const float keep = decay_pow(lam2, n);
+#pragma unroll
+        for (int ab = 0; ab < DXB; ++ab)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[ab][r] = cuts ? 0.0f : S[ab][r] * keep;
+        const bool plain = n == C && !cuts;
+        const int last = begin_of64(cuts, n - 1);
+        float wg = a.s3 * decay_pow(lam2, 5 - a.e0 - 4 * half);  // of the last group's row 3
+#pragma unroll
+        for (int js = 3; js >= 0; --js) {
+            if (16 * js >= n) continue;
+            const uintx4 zv = column16<false>(zs, 16 * js, c0, lane);
+            float wz[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wz[e] = e & 1 ? hi_half(zv[e / 2]) : lo_half(zv[e / 2]);
+            if (plain) {
+#pragma unroll
+                for (int m = 1; m >= 0; --m) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) wz[4 * m + r] *= wg * pow_r[3 - r];
+                    wg *= pow8;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int j = 16 * js + 8 * (e >> 2) + 4 * half + (e & 3);
+                    wz[e] = j < n && j >= last ? wz[e] * (a.s3 * decay_pow(lam2, n - a.e0 - j)) : 0.0f;
+                }
+            }
+            bf16x8 Zp[3];
+            split8(wz, Zp);
+#pragma unroll
+            for (int ab = 0; ab < DXB; ++ab) {
+                const bf16x8 Y = __builtin_bit_cast(bf16x8, column16<true>(ys, 16 * js, 32 * ab, lane));
+                S[ab] = mfma_bf16(Y, Zp[0], S[ab]);
+                S[ab] = mfma_bf16(Y, Zp[1], S[ab]);
+                S[ab] = mfma_bf16(Y, Zp[2], S[ab]);
+            }
+        }
+        if (want_out) {
+            // out through the wave's own columns of the z tile, which it is done with: 16-byte stores
+            if (!a.out_f32) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 8 * (r >> 2) + 4 * half + (r & 3);
+                    zs[i][col] = __builtin_bit_cast(unsigned short, (__bf16)O0[r]);
+                    zs[32 + i][col] = __builtin_bit_cast(unsigned short, (__bf16)O1[r]);
+                }
+                const int row = lane >> 2, c = c0 + (lane & 3) * 8;
+                __bf16 *o = (__bf16 *)a.out + out0 + (pos + row) * dir * a.ot + c;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (c < a.dz && row + 16 * k < n) __builtin_memcpy(o + 16 * k * dir * a.ot, &zs[row + 16 * k][c], 16);
+            } else {
+                for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = 8 * (r >> 2) + 4 * half + (r & 3);
+                        *(float *)&zs[2 * i + (l31 >> 4)][c0 + 2 * (l31 & 15)] = part ? O1[r] : O0[r];
+                    }
+                    const int row = lane >> 3, c = (lane & 7) * 4;
+                    float *o = (float *)a.out + out0 + (pos + 32 * part + row) * dir * a.ot + c0 + c;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (c0 + c < a.dz && 32 * part + row + 8 * k < n)
+                            __builtin_memcpy(o + 8 * k * dir * a.ot, &zs[2 * (row + 8 * k) + (c >> 4)][c0 + 2 * (c & 15)], 16);
+                }
+            }
+        }
+        seg_cut |= cuts != 0;
+        pos += n;
+    }
+    // rows behind the sequence's end are 0
+    if (want_out)
+        for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
+            for (int c = threadIdx.x; c < a.dz; c += NT) put(b * a.ob + h * a.oh + t * a.ot + c, 0.0f);
+    float *dst = nullptr;
+    int64_t da = a.ia, dn = a.in;
+    if (a.mode == 0 && a.fin) dst = a.fin + (int64_t)bh * a.dx * a.dz;
+    if (a.mode == 1) dst = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, da = a.dz, dn = 1;
+    if (dst) {
         const bool drop = a.mode == 0 && a.rev && a.reset && len > 0 && a.reset[b * a.rb] != 0;
 #pragma unroll
         for (int ab = 0; ab < DXB; ++ab)
@@ -377,7 +784,11 @@ int64_t segment_floats(int64_t bh, int T, int Dk, int Dv) {
 template <typename T, int DXB>
 void launch_walk(const WalkArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.B * a.H), a.nseg);
-    if (a.dz <= 32) la_walk_kernel<T, DXB, 1><<<grid, 64, 0, s>>>(a);
+    if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0) {
+        if (a.dz <= 32) la_walk_bf16_kernel<DXB, 1><<<grid, 64, 0, s>>>(a);
+        else if (a.dz <= 64) la_walk_bf16_kernel<DXB, 2><<<grid, 128, 0, s>>>(a);
+        else la_walk_bf16_kernel<DXB, 4><<<grid, 256, 0, s>>>(a);
+    } else if (a.dz <= 32) la_walk_kernel<T, DXB, 1><<<grid, 64, 0, s>>>(a);
     else if (a.dz <= 64) la_walk_kernel<T, DXB, 2><<<grid, 128, 0, s>>>(a);
     else la_walk_kernel<T, DXB, 4><<<grid, 256, 0, s>>>(a);
 }

@@ -237,6 +237,34 @@ def test_la_episodes_are_separate(K, dtype, bad):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("at", [[0], [37], [63, 64], [20, 22, 130]])
+def test_la_later_tokens_are_separate(K, dtype, at):
+    """An inf or NaN reaches no output before it and no gradient behind it, only its own column of v."""
+    s = la_inputs(1, 150, 2, (2, 2, 2), 32, 32, dtype, seed=15)
+    for i, t in enumerate(at):
+        s["v"][0, t, 0, 5 + i] = float("nan")
+    out, last = K.linear_attention(*[s[n].cuda() for n in "qkv"], s["ld"].cuda(), return_state=True)
+    out = out.float().cpu()[0]
+    fin = torch.isfinite(out)
+    want = torch.ones(150, 2, 32, dtype=torch.bool)
+    for i, t in enumerate(at):
+        want[t:, 0, 5 + i] = False
+    assert torch.equal(fin, want)
+    clean = torch.nan_to_num(s["v"])
+    ref = K.linear_attention(s["q"].cuda(), s["k"].cuda(), clean.cuda(), s["ld"].cuda()).float().cpu()[0]
+    # the spoilt chunks are walked in other pieces, so sums may round otherwise
+    assert torch.allclose(out[want], ref[want], rtol=2 * torch.finfo(dtype).eps, atol=1e-2 * ref.abs().mean().item())
+    # backward: d_out of a token reaches the gradients of k and v of that token and those before it
+    do = s["d_out"].clone()
+    do[0, 70, 1, 3] = float("inf")
+    ins = [x.cuda().requires_grad_() for x in (s["q"], s["k"], clean)]
+    _, dk, dv = torch.autograd.grad(K.linear_attention(*ins, s["ld"].cuda()), ins, do.cuda())
+    for d in (dk, dv):
+        assert torch.isfinite(d[0, 71:]).all() and torch.isfinite(d[:, :, 0]).all()
+        assert not torch.isfinite(d[0, 70, 1]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_la_strides(K, dtype):
     """Slices, broadcast batches and bases that are not aligned to anything."""
     s = la_inputs(3, 75, 2, (2, 2, 2), 24, 24, dtype, seed=6)
