@@ -56,9 +56,10 @@ __device__ __forceinline__ bool cut_at(const WalkArgs &a, int b, int p, int len)
     return p > 0 && a.reset[b * a.rb + (int64_t)(len - p) * a.rt] != 0;
 }
 
-// lam^n, n >= 0; lam = 0 (log_decay = -inf) included
+// log2 lam; a log_decay of -inf (no memory) becomes a finite number, so that lam^0 is 1 and lam^1 is 0
+__device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(log_decay * kLog2e, -1e6f); }
 __device__ __forceinline__ float decay_pow(float lam2, int n) {
-    return n == 0 ? 1.0f : __builtin_amdgcn_exp2f(lam2 * (float)n);
+    return __builtin_amdgcn_exp2f(lam2 * (float)n);
 }
 
 // The value as if computed anew: keeps what a loop derives from lane numbers and powers inside the loop.
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
     const int p0 = g * a.seglen, p1 = min(len, p0 + a.seglen);
-    const float lam2 = a.log_decay[h] * kLog2e;
+    const float lam2 = log2_decay(a.log_decay[h]);
     const int64_t tok0 = a.rev ? len - 1 : 0, dir = a.rev ? -1 : 1;
     const T *x = (const T *)a.x + b * a.xb + (h / a.gx) * a.xh + tok0 * a.xt;
     const T *y = (const T *)a.y + b * a.yb + (h / a.gy) * a.yh + tok0 * a.yt;
@@ -288,6 +289,7 @@ typedef short shortx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
 typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+typedef uintx4 uintx4_any __attribute__((aligned(2)));  // 16 bytes at any element's address
 
 __device__ __forceinline__ uint32_t pack2(float a, float b) {  // two roundings to nearest even
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){a, b}, bf16x2));
@@ -317,10 +319,6 @@ __device__ __forceinline__ void split8(const float *v, bf16x8 (&out)[N]) {
     }
 }
 
-__device__ __forceinline__ floatx16 mfma_bf16(bf16x8 a, bf16x8 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
 __device__ __forceinline__ int begin_of64(uint64_t m, int i) {
     const uint64_t below = m & (~0ull >> (63 - i));
     return below ? 63 - __builtin_clzll(below) : -1;
@@ -329,28 +327,33 @@ __device__ __forceinline__ int begin_of64(uint64_t m, int i) {
 // 64 rows of D bf16 columns on their way from global memory to LDS: 16 bytes a thread and step.
 template <int D, int NT>
 struct Rows16 {
-    static constexpr int VR = D / 8, N = 64 * VR / NT;
+    static constexpr int VR = D / 8, N = (64 * VR + NT - 1) / NT;
     uintx4 v[N];
     // d: a multiple of 8, so a vector is wholly inside the row or behind it
     __device__ __forceinline__ void load(const __bf16 *src, int64_t st, int n, int d, int tid) {
         const int row = tid / VR, c = tid % VR * 8;
         const __bf16 *p = src + row * st + c;
-        const bool in = c < d;
+        if (n == 64 && d == D && 64 * VR >= NT) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = *(const uintx4_any *)(p + k * (NT / VR) * st);
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             v[k] = (uintx4){0, 0, 0, 0};
-            if (in && row + k * (NT / VR) < n) __builtin_memcpy(&v[k], p + k * (NT / VR) * st, 16);
+            if (c < d && row + k * (NT / VR) < n) v[k] = *(const uintx4_any *)(p + k * (NT / VR) * st);
         }
     }
-    // PERM: within 16 columns the order 0-3, 8-11, 4-7, 12-15, in which a half wave's 8 columns are
-    // 16 bytes and match the rows of an accumulator (see the kernel).
+    // PERM: of 32 columns the four-column groups in the order 0 4 1 5 2 6 3 7, in which a quarter wave's
+    // eight columns are 16 bytes and match two accumulators' rows (see the kernel).
     template <bool PERM, int P>
     __device__ __forceinline__ void store(unsigned short (*dst)[P], int tid) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int id = k * NT + tid, row = id / VR, c = id % VR * 8;
+            if (64 * VR < NT && row >= 64) break;
             if (PERM) {
-                const int at = (c & ~15) + (c & 8) / 2;
+                const int at = (c & ~31) + (c & 8) * 2 + (c & 16) / 4;
                 *(uintx2 *)&dst[row][at] = (uintx2){v[k][0], v[k][1]};
                 *(uintx2 *)&dst[row][at + 8] = (uintx2){v[k][2], v[k][3]};
             } else {
@@ -369,82 +372,75 @@ struct Rows16 {
     }
 };
 
-// Four rows j0 + 4 (lane >> 5) .. + 3 of column c0 + (lane & 31): the transposing LDS read, 16 lanes
-// giving the addresses of 4 rows x 16 columns and getting a column each.
+// Rows j0 + 4 q .. + 3 of column c0 + (lane & 15), q = lane >> 4: the transposing LDS read, in which 16
+// lanes give the addresses of 4 rows x 16 columns and get a column each. column32: also the rows 16 on,
+// together the operand of 32 rows.
 template <bool PERM, int P>
 __device__ __forceinline__ uintx2 column4(const unsigned short (*t)[P], int j0, int c0, int lane) {
-    const int row = j0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int q = lane & 3, c = c0 + (lane & 16) + 4 * (PERM ? (q >> 1) | (q & 1) << 1 : q);
     typedef __attribute__((address_space(3))) shortx4 *lds4;
+    const int row = j0 + (lane >> 2);
+    const int c = PERM ? (c0 & ~31) + (c0 & 16) / 4 + (lane & 3) * 8 : c0 + (lane & 3) * 4;
     return __builtin_bit_cast(uintx2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)&t[row][c]));
 }
 template <bool PERM, int P>
-__device__ __forceinline__ uintx4 column16(const unsigned short (*t)[P], int j0, int c0, int lane) {
-    const uintx2 a = column4<PERM>(t, j0, c0, lane), b = column4<PERM>(t, j0 + 8, c0, lane);
+__device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0, int c0, int lane) {
+    const uintx2 a = column4<PERM>(t, j0, c0, lane), b = column4<PERM>(t, j0 + 16, c0, lane);
     return (uintx4){a[0], a[1], b[0], b[1]};
 }
 
-// la_walk_kernel for bf16 operands on v_mfma_f32_32x32x16_bf16, 64 tokens a chunk. Products of the
+// la_walk_kernel for bf16 operands on v_mfma_f32_16x16x32_bf16, 64 tokens a chunk. Products of the
 // operands are exact in f32; what is not an operand is split into bf16 pieces where it meets the
 // matrix cores: P and S for the output into two (2^-16, below the output's own rounding), the
 // weighted z of the state's sum into three (2^-24), so that the state stays an f32 state.
 //
-// A 32x32 accumulator holds rows 8 (r >> 2) + 4 (lane >> 5) + (r & 3) of column lane & 31, so eight of
-// its registers are the operand of 16 rows in the order 0-3, 8-11 | 4-7, 12-15 of the half waves. With
+// A 16x16 accumulator holds rows 4 q + r (q = lane >> 4) of column lane & 15, so the accumulators of two
+// row tiles are the operand of 32 rows in the order 4 q .. 4 q + 3, 16 + 4 q .. of the quarter waves. With
 // the other operand read in that order (the order of a contraction is free) S goes from accumulator
 // to operand without leaving its wave, and so does P, computed transposed as Y X^T.
+//
+// 16 columns a wave, not 32: with 32x32 tiles at two waves a SIMD the same work waited on LDS and on
+// its own products (9 us a chunk of 128 x 128); half the registers a wave let four waves run.
 template <int DXB, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void la_walk_bf16_kernel(WalkArgs a) {
-    constexpr int C = 64, DX = 32 * DXB, DZ = 32 * NW, NT = 64 * NW;
-    __shared__ __align__(16) unsigned short xs[C][DX + 16];
-    __shared__ __align__(16) unsigned short ys[C][DX + 16];
-    __shared__ __align__(16) unsigned short zs[C][DZ + 16];
-    __shared__ __align__(16) uintx4 ps[3][2][2][64];
+__global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
+    constexpr int C = 64, DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW, PAD = 16;
+    __shared__ __align__(16) unsigned short xs[C][DX + PAD];
+    __shared__ __align__(16) unsigned short ys[C][DX + PAD];
+    __shared__ __align__(16) unsigned short zs[C][DZ + PAD];
+    __shared__ __align__(16) uintx2 ps[6][2][64][2];  // (token tile, 32 tokens), piece, lane, half
+    __shared__ __align__(16) float into_s[C], from_s[C];
     __shared__ int bad_s, first_s;
-    int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, l31 = lane & 31;
+    int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
     const int p0 = g * a.seglen, p1 = min(len, p0 + a.seglen);
-    const float lam2 = a.log_decay[h] * kLog2e;
+    const float lam2 = log2_decay(a.log_decay[h]);
     const int64_t tok0 = a.rev ? len - 1 : 0, dir = a.rev ? -1 : 1;
     const __bf16 *x = (const __bf16 *)a.x + b * a.xb + (h / a.gx) * a.xh + tok0 * a.xt;
     const __bf16 *y = (const __bf16 *)a.y + b * a.yb + (h / a.gy) * a.yh + tok0 * a.yt;
     const __bf16 *z = (const __bf16 *)a.z + b * a.zb + (h / a.gz) * a.zh + tok0 * a.zt;
     const int64_t out0 = b * a.ob + h * a.oh + tok0 * a.ot;
     const bool want_out = a.mode != 1;
-    const int c0 = 32 * w;
-    int col = c0 + l31;
-    auto put = [&](int64_t at, float v) {
-        if (a.out_f32) ((float *)a.out)[at] = v;
-        else ((__bf16 *)a.out)[at] = (__bf16)v;
-    };
+    const int c0 = 16 * w;
+    int col = c0 + l15;
 
-    // powers of lam of an output's rows i = 8 m + 4 half + r
-    float row_m[4], pow_r[4];
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        row_m[m] = a.s2 * decay_pow(lam2, 8 * m + 4 * half + a.e0);
-        pow_r[m] = decay_pow(lam2, m);
-    }
-    const float pow8 = decay_pow(lam2, 8), pow32 = decay_pow(lam2, 32);
-
-    floatx16 S[DXB];
+    floatx4 S[2 * DXB];
     {
         const float *src = nullptr;
         int64_t ia = a.ia, in = a.in;
         if (a.mode == 0 && a.init) src = a.init + (int64_t)bh * a.dx * a.dz;
         if (a.mode == 2) src = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, ia = a.dz, in = 1;
 #pragma unroll
-        for (int ab = 0; ab < DXB; ++ab)
+        for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
-                S[ab][r] = src && row < a.dx && col < a.dz ? src[row * ia + col * in] : 0.0f;
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * at + 4 * q + r;
+                S[at][r] = src && row < a.dx && col < a.dz ? src[row * ia + col * in] : 0.0f;
             }
     }
     bool seg_cut = false;
-    if (threadIdx.x == 0) bad_s = -1;
+    if (tid == 0) bad_s = -1;
+    for (int id = tid; id < 6 * 2 * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
     Rows16<DX, NT> rx, ry;
     Rows16<DZ, NT> rz;
     auto load = [&](int pos) {
@@ -455,28 +451,35 @@ __global__ __launch_bounds__(64 * NW, 2) void la_walk_bf16_kernel(WalkArgs a) {
     };
     if (p0 < p1) load(p0);
     for (int pos = p0; pos < p1;) {
-        tid = anew(tid), lane = tid & 63, half = lane >> 5, l31 = lane & 31, col = c0 + l31;
-#pragma unroll
-        for (int m = 0; m < 4; ++m) row_m[m] = anew(row_m[m]), pow_r[m] = anew(pow_r[m]);
+        tid = anew(tid), lane = tid & 63, q = lane >> 4, l15 = lane & 15, col = c0 + l15;
         int n = min(C, p1 - pos);
+        // what a token takes from the state that comes in, and what it leaves to the one that goes out: only
+        // tokens of the episodes that came in and that goes out
+        auto factors = [&](uint64_t cuts) {
+            if (tid < C) {
+                into_s[tid] = cuts & (~0ull >> (63 - tid)) ? 0.0f : a.s2 * decay_pow(lam2, tid + a.e0);
+                from_s[tid] = tid < n && tid >= begin_of64(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - tid) : 0.0f;
+            }
+        };
         uint64_t cuts = __ballot(lane < n && cut_at(a, b, pos + lane, len));
         __syncthreads();  // the chunk before is done with the tiles
         if (want_out) rx.template store<true>(xs, tid);
         ry.template store<true>(ys, tid);
         rz.template store<false>(zs, tid);
+        factors(cuts);
         if (ry.not_finite() || rz.not_finite()) bad_s = pos;
         if (pos + n < p1) load(pos + n);
         __syncthreads();
         if (bad_s == pos) {
             // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
             // chunk ends before a row that holds one, and such a row's chunk before the next episode.
-            if (threadIdx.x == 0) first_s = n;
+            if (tid == 0) first_s = n;
             __syncthreads();
             bool head = false;
             for (int j = 0; j < n; ++j) {
                 bool bad = false;
-                for (int c = threadIdx.x; c < DX; c += NT) bad |= (ys[j][c] & 0x7F80) == 0x7F80;
-                for (int c = threadIdx.x; c < DZ; c += NT) bad |= (zs[j][c] & 0x7F80) == 0x7F80;
+                for (int c = tid; c < DX; c += NT) bad |= (ys[j][c] & 0x7F80) == 0x7F80;
+                for (int c = tid; c < DZ; c += NT) bad |= (zs[j][c] & 0x7F80) == 0x7F80;
                 if (j == 0) head = __syncthreads_or(bad);
                 else if (bad) atomicMin(&first_s, j);
             }
@@ -484,161 +487,133 @@ __global__ __launch_bounds__(64 * NW, 2) void la_walk_bf16_kernel(WalkArgs a) {
             n = first_s;
             if (head && (cuts & ~1ull)) n = min(n, (int)__builtin_ctzll(cuts & ~1ull));
             cuts &= ~0ull >> (64 - n);
-            for (int id = threadIdx.x; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0;
-            for (int id = threadIdx.x; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0;
+            for (int id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0;
+            for (int id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0;
             if (pos + n < p1) load(pos + n);
+            factors(cuts);
             __syncthreads();
         }
-        const bool two = n > 32;
-        floatx16 O0, O1;
+        floatx4 O[4];
+        uintx4 zv[2];  // z rows 32 js .. of the wave's columns: the operand of P Z, weighted that of S
+#pragma unroll
+        for (int js = 0; js < 2; ++js) zv[js] = column32<false>(zs, 32 * js, c0, lane);
         if (want_out) {
-            // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in 32 x 32 blocks (j, i), shared out
-            // over the waves and handed to all of them as operands, two pieces each
-            for (int q = w; q < (two ? 3 : 1); q += NW) {
-                const int jb = 32 * (q >> 1), ib = 32 * ((q + 1) >> 1);
-                floatx16 P;
+            // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in ten 16 x 16 tiles (j, i), shared
+            // out over the waves and handed to all of them as operands, two pieces each
+            for (int t = w; t < 10; t += NW) {
+                const int it = (t > 0) + (t > 2) + (t > 5), jt = t - it * (it + 1) / 2;
+                floatx4 P = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int r = 0; r < 16; ++r) P[r] = 0.0f;
+                for (int s = 0; s < DXB; ++s)
+                    P = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)&ys[16 * jt + l15][32 * s + 8 * q],
+                                                                *(const bf16x8 *)&xs[16 * it + l15][32 * s + 8 * q],
+                                                                P, 0, 0, 0);
+                const int d0 = 16 * (it - jt) + l15 - 4 * q;
+                const int j0 = cuts ? begin_of64(cuts, 16 * it + l15) - 16 * jt - 4 * q : -C;  // of i's episode
+                float pv[4];
 #pragma unroll
-                for (int s = 0; s < 2 * DXB; ++s)
-                    P = mfma_bf16(*(const bf16x8 *)&ys[jb + l31][16 * s + 8 * half],
-                                  *(const bf16x8 *)&xs[ib + l31][16 * s + 8 * half], P);
-                const int d0 = ib - jb + l31 - 4 * half;
-                const int j0 = max(0, begin_of64(cuts, ib + l31) - jb - 4 * half);  // of i's episode
+                for (int r = 0; r < 4; ++r) {
+                    pv[r] = P[r] * (a.s1 * decay_pow(lam2, d0 - r));
+                    pv[r] = r <= d0 && r >= j0 ? pv[r] : 0.0f;  // 0 whatever stood there
+                }
+                const uintx2 hi = {pack2(pv[0], pv[1]), pack2(pv[2], pv[3])};
+                const int slot = it + (it == 3) + (jt >> 1);
+                ps[slot][0][lane][jt & 1] = hi;
+                ps[slot][1][lane][jt & 1] = (uintx2){pack2(pv[0] - lo_half(hi[0]), pv[1] - hi_half(hi[0])),
+                                                     pack2(pv[2] - lo_half(hi[1]), pv[3] - hi_half(hi[1]))};
+            }
+            // x S, decayed to each row
 #pragma unroll
-                for (int js = 0; js < 2; ++js) {
-                    float pv[8];
+            for (int it = 0; it < 4; ++it) O[it] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int j = 16 * js + 8 * (e >> 2) + (e & 3);
-                        const float f = a.s1 * decay_pow(lam2, max(d0 - j, 0));
-                        pv[e] = j <= d0 && j >= j0 ? P[8 * js + e] * f : 0.0f;  // 0 whatever stood there
-                    }
-                    bf16x8 Pp[2];
-                    split8(pv, Pp);
-                    ps[q][js][0][lane] = __builtin_bit_cast(uintx4, Pp[0]);
-                    ps[q][js][1][lane] = __builtin_bit_cast(uintx4, Pp[1]);
+            for (int s = 0; s < DXB; ++s) {
+                bf16x8 Sp[2];
+                float sv[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sv[e] = S[2 * s + (e >> 2)][e & 3];
+                split8(sv, Sp);
+#pragma unroll
+                for (int it = 0; it < 4; ++it) {
+                    const bf16x8 X = *(const bf16x8 *)&xs[16 * it + l15][32 * s + 8 * q];
+                    O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[0], O[it], 0, 0, 0);
+                    O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[1], O[it], 0, 0, 0);
                 }
             }
-            // x S, decayed to each row, where the row's episode is the one that came in
 #pragma unroll
-            for (int r = 0; r < 16; ++r) O0[r] = O1[r] = 0.0f;
-            auto xS = [&](auto both) {
+            for (int it = 0; it < 4; ++it) {
+                const floatx4 f = *(const floatx4 *)&into_s[16 * it + 4 * q];
 #pragma unroll
-                for (int s = 0; s < 2 * DXB; ++s) {
-                    bf16x8 Sp[2];
-                    float sv[8];
+                for (int r = 0; r < 4; ++r) O[it][r] *= f[r];
+                if (cuts) {  // not 0 * inf
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sv[e] = S[s / 2][8 * (s & 1) + e];
-                    split8(sv, Sp);
-                    const bf16x8 X0 = *(const bf16x8 *)&xs[l31][16 * s + 8 * half];
-                    O0 = mfma_bf16(X0, Sp[0], O0);
-                    O0 = mfma_bf16(X0, Sp[1], O0);
-                    if (both) {
-                        const bf16x8 X1 = *(const bf16x8 *)&xs[32 + l31][16 * s + 8 * half];
-                        O1 = mfma_bf16(X1, Sp[0], O1);
-                        O1 = mfma_bf16(X1, Sp[1], O1);
-                    }
+                    for (int r = 0; r < 4; ++r) O[it][r] = f[r] != 0.0f ? O[it][r] : 0.0f;
                 }
-            };
-            if (two) xS(std::true_type{});
-            else xS(std::false_type{});
-            const int first = cuts ? (int)__builtin_ctzll(cuts) : C;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = 8 * (r >> 2) + 4 * half + (r & 3);
-                const float f = row_m[r >> 2] * pow_r[r & 3];
-                O0[r] = i < first ? O0[r] * f : 0.0f;
-                O1[r] = 32 + i < first ? O1[r] * (f * pow32) : 0.0f;
             }
             __syncthreads();  // P is there
 #pragma unroll
-            for (int js = 0; js < 2; ++js) {
-                const bf16x8 Z = __builtin_bit_cast(bf16x8, column16<false>(zs, 16 * js, c0, lane));
+            for (int it = 0; it < 4; ++it)
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    O0 = mfma_bf16(__builtin_bit_cast(bf16x8, ps[0][js][p][lane]), Z, O0);
-                    if (two) O1 = mfma_bf16(__builtin_bit_cast(bf16x8, ps[1][js][p][lane]), Z, O1);
-                }
-            }
-            if (two) {
-#pragma unroll
-                for (int js = 0; js < 2; ++js) {
-                    const bf16x8 Z = __builtin_bit_cast(bf16x8, column16<false>(zs, 32 + 16 * js, c0, lane));
+                for (int js = 0; js < (it >> 1) + 1; ++js)
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
-                        O1 = mfma_bf16(__builtin_bit_cast(bf16x8, ps[2][js][p][lane]), Z, O1);
-                }
-            }
+                        O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            *(const bf16x8 *)&ps[it + (it == 3) + js][p][lane], __builtin_bit_cast(bf16x8, zv[js]), O[it],
+                            0, 0, 0);
         }
-        // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T over the episode that goes out
-        const float keep = decay_pow(lam2, n);
+        // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T
+        {
+            const float keep = decay_pow(lam2, n);
 #pragma unroll
-        for (int ab = 0; ab < DXB; ++ab)
+            for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[ab][r] = cuts ? 0.0f : S[ab][r] * keep;
-        const bool plain = n == C && !cuts;
-        const int last = begin_of64(cuts, n - 1);
-        float wg = a.s3 * decay_pow(lam2, 5 - a.e0 - 4 * half);  // of the last group's row 3
+                for (int r = 0; r < 4; ++r) S[at][r] *= keep;
+        }
+        if (cuts) {
 #pragma unroll
-        for (int js = 3; js >= 0; --js) {
-            if (16 * js >= n) continue;
-            const uintx4 zv = column16<false>(zs, 16 * js, c0, lane);
+            for (int at = 0; at < 2 * DXB; ++at) S[at] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int js = 0; js < 2; ++js) {
             float wz[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) wz[e] = e & 1 ? hi_half(zv[e / 2]) : lo_half(zv[e / 2]);
-            if (plain) {
-#pragma unroll
-                for (int m = 1; m >= 0; --m) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) wz[4 * m + r] *= wg * pow_r[3 - r];
-                    wg *= pow8;
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int j = 16 * js + 8 * (e >> 2) + 4 * half + (e & 3);
-                    wz[e] = j < n && j >= last ? wz[e] * (a.s3 * decay_pow(lam2, n - a.e0 - j)) : 0.0f;
-                }
+            for (int m = 0; m < 2; ++m) {
+                const floatx4 f = *(const floatx4 *)&from_s[32 * js + 16 * m + 4 * q];
+                wz[4 * m] = lo_half(zv[js][2 * m]) * f[0], wz[4 * m + 1] = hi_half(zv[js][2 * m]) * f[1];
+                wz[4 * m + 2] = lo_half(zv[js][2 * m + 1]) * f[2], wz[4 * m + 3] = hi_half(zv[js][2 * m + 1]) * f[3];
             }
             bf16x8 Zp[3];
             split8(wz, Zp);
 #pragma unroll
-            for (int ab = 0; ab < DXB; ++ab) {
-                const bf16x8 Y = __builtin_bit_cast(bf16x8, column16<true>(ys, 16 * js, 32 * ab, lane));
-                S[ab] = mfma_bf16(Y, Zp[0], S[ab]);
-                S[ab] = mfma_bf16(Y, Zp[1], S[ab]);
-                S[ab] = mfma_bf16(Y, Zp[2], S[ab]);
+            for (int at = 0; at < 2 * DXB; ++at) {
+                const bf16x8 Y = __builtin_bit_cast(bf16x8, column32<true>(ys, 32 * js, 16 * at, lane));
+#pragma unroll
+                for (int p = 0; p < 3; ++p) S[at] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Y, Zp[p], S[at], 0, 0, 0);
             }
         }
         if (want_out) {
             // out through the wave's own columns of the z tile, which it is done with: 16-byte stores
             if (!a.out_f32) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = 8 * (r >> 2) + 4 * half + (r & 3);
-                    zs[i][col] = __builtin_bit_cast(unsigned short, (__bf16)O0[r]);
-                    zs[32 + i][col] = __builtin_bit_cast(unsigned short, (__bf16)O1[r]);
-                }
-                const int row = lane >> 2, c = c0 + (lane & 3) * 8;
+                for (int it = 0; it < 4; ++it)
+#pragma unroll
+                    for (int r = 0; r < 4; r += 2) {
+                        const uint32_t o = pack2(O[it][r], O[it][r + 1]);
+                        zs[16 * it + 4 * q + r][col] = (unsigned short)o;
+                        zs[16 * it + 4 * q + r + 1][col] = (unsigned short)(o >> 16);
+                    }
+                const int row = lane >> 1, c = c0 + (lane & 1) * 8;
                 __bf16 *o = (__bf16 *)a.out + out0 + (pos + row) * dir * a.ot + c;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (c < a.dz && row + 16 * k < n) __builtin_memcpy(o + 16 * k * dir * a.ot, &zs[row + 16 * k][c], 16);
+                for (int k = 0; k < 2; ++k)
+                    if (c < a.dz && row + 32 * k < n) *(uintx4_any *)(o + 32 * k * dir * a.ot) = *(uintx4 *)&zs[row + 32 * k][c];
             } else {
-                for (int part = 0; part < 2; ++part) {
+                float *o = (float *)a.out + out0 + (pos + 4 * q) * dir * a.ot + col;
+                if (col < a.dz)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = 8 * (r >> 2) + 4 * half + (r & 3);
-                        *(float *)&zs[2 * i + (l31 >> 4)][c0 + 2 * (l31 & 15)] = part ? O1[r] : O0[r];
-                    }
-                    const int row = lane >> 3, c = (lane & 7) * 4;
-                    float *o = (float *)a.out + out0 + (pos + 32 * part + row) * dir * a.ot + c0 + c;
+                    for (int it = 0; it < 4; ++it)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (c0 + c < a.dz && 32 * part + row + 8 * k < n)
-                            __builtin_memcpy(o + 8 * k * dir * a.ot, &zs[2 * (row + 8 * k) + (c >> 4)][c0 + 2 * (c & 15)], 16);
-                }
+                        for (int r = 0; r < 4; ++r)
+                            if (16 * it + 4 * q + r < n) o[(16 * it + r) * dir * a.ot] = O[it][r];
             }
         }
         seg_cut |= cuts != 0;
@@ -647,7 +622,11 @@ __global__ __launch_bounds__(64 * NW, 2) void la_walk_bf16_kernel(WalkArgs a) {
     // rows behind the sequence's end are 0
     if (want_out)
         for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
-            for (int c = threadIdx.x; c < a.dz; c += NT) put(b * a.ob + h * a.oh + t * a.ot + c, 0.0f);
+            for (int c = tid; c < a.dz; c += NT) {
+                const int64_t at = b * a.ob + h * a.oh + t * a.ot + c;
+                if (a.out_f32) ((float *)a.out)[at] = 0.0f;
+                else ((__bf16 *)a.out)[at] = (__bf16)0.0f;
+            }
     float *dst = nullptr;
     int64_t da = a.ia, dn = a.in;
     if (a.mode == 0 && a.fin) dst = a.fin + (int64_t)bh * a.dx * a.dz;
@@ -655,14 +634,14 @@ __global__ __launch_bounds__(64 * NW, 2) void la_walk_bf16_kernel(WalkArgs a) {
     if (dst) {
         const bool drop = a.mode == 0 && a.rev && a.reset && len > 0 && a.reset[b * a.rb] != 0;
 #pragma unroll
-        for (int ab = 0; ab < DXB; ++ab)
+        for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (row < a.dx && col < a.dz) dst[row * da + col * dn] = drop ? 0.0f : S[ab][r];
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * at + 4 * q + r;
+                if (row < a.dx && col < a.dz) dst[row * da + col * dn] = drop ? 0.0f : S[at][r];
             }
     }
-    if (a.mode == 1 && threadIdx.x == 0)
+    if (a.mode == 1 && tid == 0)
         a.segf[(int64_t)bh * a.nseg + g] = seg_cut ? -1.0f : decay_pow(lam2, max(p1 - p0, 0));
 }
 
@@ -674,10 +653,16 @@ __global__ __launch_bounds__(256) void la_join_kernel(WalkArgs a) {
     float carry = a.init ? a.init[at] : 0.0f;
     float *seg = a.seg + bh * a.nseg * size + e;
     const float *f = a.segf + (int64_t)bh * a.nseg;
-    for (int g = 0; g < a.nseg; ++g, seg += size) {
-        const float u = *seg;
-        *seg = carry;
-        carry = f[g] < 0.0f ? u : f[g] * carry + u;
+    for (int g = 0; g < a.nseg; g += 8) {
+        float u[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k] = g + k < a.nseg ? seg[(g + k) * size] : 0.0f;  // in flight together
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (g + k >= a.nseg) break;
+            seg[(g + k) * size] = carry;
+            carry = f[g + k] < 0.0f ? u[k] : f[g + k] * carry + u[k];
+        }
     }
     if (a.fin) {
         const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -785,9 +770,9 @@ template <typename T, int DXB>
 void launch_walk(const WalkArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.B * a.H), a.nseg);
     if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0) {
-        if (a.dz <= 32) la_walk_bf16_kernel<DXB, 1><<<grid, 64, 0, s>>>(a);
-        else if (a.dz <= 64) la_walk_bf16_kernel<DXB, 2><<<grid, 128, 0, s>>>(a);
-        else la_walk_bf16_kernel<DXB, 4><<<grid, 256, 0, s>>>(a);
+        if (a.dz <= 32) la_walk_bf16_kernel<DXB, 2><<<grid, 128, 0, s>>>(a);
+        else if (a.dz <= 64) la_walk_bf16_kernel<DXB, 4><<<grid, 256, 0, s>>>(a);
+        else la_walk_bf16_kernel<DXB, 8><<<grid, 512, 0, s>>>(a);
     } else if (a.dz <= 32) la_walk_kernel<T, DXB, 1><<<grid, 64, 0, s>>>(a);
     else if (a.dz <= 64) la_walk_kernel<T, DXB, 2><<<grid, 128, 0, s>>>(a);
     else la_walk_kernel<T, DXB, 4><<<grid, 256, 0, s>>>(a);
