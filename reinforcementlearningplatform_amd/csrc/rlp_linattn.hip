@@ -18,6 +18,15 @@
 namespace rlp {
 namespace {
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
+typedef uintx4 uintx4_any __attribute__((aligned(2)));  // 16 bytes at any element's address
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
@@ -77,57 +86,87 @@ __device__ __forceinline__ int begin_of(uint32_t m, int i) {
     return below ? 31 - __builtin_clz(below) : -1;
 }
 
-// C rows of D = 32 * DB columns into LDS as f32; rows >= n and columns >= d are 0. 16-byte loads
-// (any alignment), the last columns of an odd d one by one. Returns whether a value is inf or NaN.
-template <typename T, int DB, int C, int NT>
-__device__ __forceinline__ bool stage(float (*dst)[32 * DB + 4], const T *src, int64_t st, int n, int d) {
-    constexpr int VE = 16 / sizeof(T);
-    constexpr int VR = 32 * DB / VE;  // vectors per row
-    uint32_t most = 0;
+// 32 rows of D columns of T on their way from global memory to f32 rows in LDS: 16 bytes a thread and
+// step at any alignment; rows >= n and columns >= d become 0.
+template <typename T, int D, int NT>
+struct Rows32 {
+    static constexpr int VE = 16 / sizeof(T), VR = D / VE, N = (32 * VR + NT - 1) / NT;
+    uintx4 v[N];
+    __device__ __forceinline__ void load(const T *src, int64_t st, int n, int d, int tid) {
+        const int row = tid / VR, c = tid % VR * VE;
+        const T *p = src + row * st + c;
+        if (n == 32 && d == D && 32 * VR % NT == 0) {
 #pragma unroll
-    for (int it = 0; it < (C * VR + NT - 1) / NT; ++it) {
-        const int id = it * NT + (int)threadIdx.x;
-        if (C * VR % NT != 0 && id >= C * VR) break;
-        const int row = id / VR, c = id % VR * VE;
-        float f[VE];
+            for (int k = 0; k < N; ++k) v[k] = *(const uintx4_any *)(p + k * (NT / VR) * st);
+            return;
+        }
 #pragma unroll
-        for (int e = 0; e < VE; ++e) f[e] = 0.0f;
-        if (row < n) {
-            const T *p = src + row * st + c;
+        for (int k = 0; k < N; ++k) {
+            v[k] = (uintx4){0, 0, 0, 0};
+            if (row + k * (NT / VR) >= n) continue;
+            const T *pk = p + k * (NT / VR) * st;
             if (c + VE <= d) {
-                T v[VE];
-                __builtin_memcpy(v, p, 16);
+                v[k] = *(const uintx4_any *)pk;
+            } else if constexpr (sizeof(T) == 4) {
+                if (c < d) v[k][0] = *(const uint32_t *)pk;
+                if (c + 1 < d) v[k][1] = *(const uint32_t *)(pk + 1);
+                if (c + 2 < d) v[k][2] = *(const uint32_t *)(pk + 2);
+            } else {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) f[e] = to_f32(v[e]);
+                for (int e = 0; e < 7; ++e)
+                    if (c + e < d) v[k][e / 2] |= (uint32_t)__builtin_bit_cast(unsigned short, pk[e]) << (16 * (e & 1));
+            }
+        }
+    }
+    // Also says whether a value is inf or NaN.
+    __device__ __forceinline__ bool store(float (*dst)[D + 4], int tid) const {
+        uint32_t most = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int id = k * NT + tid, row = id / VR, c = id % VR * VE;
+            if (32 * VR % NT != 0 && row >= 32) break;
+            float f[VE];
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) f[e] = __uint_as_float(v[k][e]);
             } else {
 #pragma unroll
                 for (int e = 0; e < VE; ++e)
-                    if (c + e < d) f[e] = to_f32(p[e]);
+                    f[e] = to_f32(__builtin_bit_cast(T, (unsigned short)(v[k][e / 2] >> (16 * (e & 1)))));
             }
 #pragma unroll
             for (int e = 0; e < VE; ++e) most = max(most, __float_as_uint(f[e]) & 0x7FFFFFFFu);
-        }
 #pragma unroll
-        for (int e = 0; e < VE; e += 4)
-            *(floatx4 *)&dst[row][c + e] = (floatx4){f[e], f[e + 1], f[e + 2], f[e + 3]};
+            for (int e = 0; e < VE; e += 4)
+                *(floatx4 *)&dst[row][c + e] = (floatx4){f[e], f[e + 1], f[e + 2], f[e + 3]};
+        }
+        return most >= 0x7F800000u;
     }
-    return most >= 0x7F800000u;
+};
+
+__device__ __forceinline__ floatx4 mfma_f32(float a, float b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// The walk in exact f32 products (v_mfma_f32_32x32x2_f32 / 16x16x4_f32). A block of NW waves owns
-// one (batch, head, segment); wave w owns columns [32 w, 32 w + 32) of the state and the output, so
-// no wave ever needs another's state. S sits in accumulators as [a][n] with n on the lane; an
-// accumulator register is an operand of x S as it stands, because the order of the contraction
-// over a is free: step r of block ab takes rows a = 32 ab + 8 (r >> 2) + 4 (lane >> 5) + (r & 3).
+// The walk in exact f32 products (v_mfma_f32_16x16x4_f32), 32 tokens a chunk, for every type. A block
+// of NW waves owns one (batch, head, segment); wave w owns columns [16 w, 16 w + 16) of the state and
+// the output, so no wave ever needs another's state.
+//
+// A 16x16 accumulator holds rows 4 q + r (q = lane >> 4) of column lane & 15 in register r, and an
+// operand one value of row q of four. With the order of a contraction free, register r of an
+// accumulator is the operand of rows q -> 4 q + r as it stands: S goes from accumulator to operand
+// without leaving its wave, and so does P, computed transposed as Y X^T and shared out over the waves.
 template <typename T, int DXB, int NW>
-__global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
-    constexpr int C = 32, DX = 32 * DXB, DZ = 32 * NW, NT = 64 * NW;
+__global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_kernel(WalkArgs a) {
+    constexpr int C = 32, DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW;
     __shared__ __align__(16) float xs[C][DX + 4];
     __shared__ __align__(16) float ys[C][DX + 4];
     __shared__ __align__(16) float zs[C][DZ + 4];
-    __shared__ __align__(16) float ps[C][C + 4];
+    __shared__ __align__(16) floatx4 ps[3][64];
+    __shared__ __align__(16) float into_s[C], from_s[C];
     __shared__ int bad_s, first_s;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, half = lane >> 5, l31 = lane & 31;
+    int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
     const int p0 = g * a.seglen, p1 = min(len, p0 + a.seglen);
@@ -138,120 +177,168 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
     const T *z = (const T *)a.z + b * a.zb + (h / a.gz) * a.zh + tok0 * a.zt;
     const int64_t out0 = b * a.ob + h * a.oh + tok0 * a.ot;
     const bool want_out = a.mode != 1;
-    const int col = 32 * w + l31;
-    auto put = [&](int64_t at, float v) {
-        if (a.out_f32) ((float *)a.out)[at] = v;
-        else ((T *)a.out)[at] = (T)v;
-    };
+    const int c0 = 16 * w;
+    int col = c0 + l15;
 
-    floatx16 S[DXB];
+    floatx4 S[2 * DXB];
     {
         const float *src = nullptr;
         int64_t ia = a.ia, in = a.in;
         if (a.mode == 0 && a.init) src = a.init + (int64_t)bh * a.dx * a.dz;
         if (a.mode == 2) src = a.seg + ((int64_t)bh * a.nseg + g) * a.dx * a.dz, ia = a.dz, in = 1;
 #pragma unroll
-        for (int ab = 0; ab < DXB; ++ab)
+        for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
-                S[ab][r] = src && row < a.dx && col < a.dz ? src[row * ia + col * in] : 0.0f;
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * at + 4 * q + r;
+                S[at][r] = src && row < a.dx && col < a.dz ? src[row * ia + col * in] : 0.0f;
             }
     }
     bool seg_cut = false;
-    if (threadIdx.x == 0) bad_s = -1;
+    if (tid == 0) bad_s = -1;
+    Rows32<T, DX, NT> rx, ry;
+    Rows32<T, DZ, NT> rz;
+    auto load = [&](int pos) {
+        const int n = min(C, p1 - pos);
+        if (want_out) rx.load(x + pos * dir * a.xt, dir * a.xt, n, a.dx, tid);
+        ry.load(y + pos * dir * a.yt, dir * a.yt, n, a.dx, tid);
+        rz.load(z + pos * dir * a.zt, dir * a.zt, n, a.dz, tid);
+    };
+    if (p0 < p1) load(p0);
     for (int pos = p0; pos < p1;) {
+        tid = anew(tid), lane = tid & 63, q = lane >> 4, l15 = lane & 15, col = c0 + l15;
         int n = min(C, p1 - pos);
+        // what a token takes from the state that comes in, and what it leaves to the one that goes out: only
+        // tokens of the episodes that came in and that goes out
+        auto factors = [&](uint32_t cuts) {
+            if (tid < C) {
+                into_s[tid] = cuts & (~0u >> (31 - tid)) ? 0.0f : a.s2 * decay_pow(lam2, tid + a.e0);
+                from_s[tid] = tid < n && tid >= begin_of(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - tid) : 0.0f;
+            }
+        };
         uint32_t cuts = (uint32_t)__ballot(lane < n && cut_at(a, b, pos + lane, len));
         __syncthreads();  // the chunk before is done with the tiles
-        if (want_out) stage<T, DXB, C, NT>(xs, x + pos * dir * a.xt, dir * a.xt, n, a.dx);
-        bool bad = stage<T, DXB, C, NT>(ys, y + pos * dir * a.yt, dir * a.yt, n, a.dx);
-        bad |= stage<T, NW, C, NT>(zs, z + pos * dir * a.zt, dir * a.zt, n, a.dz);
+        if (want_out) rx.store(xs, tid);
+        bool bad = ry.store(ys, tid);
+        bad |= rz.store(zs, tid);
         if (bad) bad_s = pos;
+        factors(cuts);
+        if (pos + n < p1) load(pos + n);
         __syncthreads();
         if (bad_s == pos) {
             // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
             // chunk ends before a row that holds one, and such a row's chunk before the next episode.
-            if (threadIdx.x == 0) first_s = n;
+            if (tid == 0) first_s = n;
             __syncthreads();
             bool head = false;
             for (int j = 0; j < n; ++j) {
-                bool b2 = false;
-                for (int c = threadIdx.x; c < DX; c += NT) b2 |= (__float_as_uint(ys[j][c]) & 0x7F800000u) == 0x7F800000u;
-                for (int c = threadIdx.x; c < DZ; c += NT) b2 |= (__float_as_uint(zs[j][c]) & 0x7F800000u) == 0x7F800000u;
-                if (j == 0) head = __syncthreads_or(b2);
-                else if (b2) atomicMin(&first_s, j);
+                bool here = false;
+                for (int c = tid; c < DX; c += NT) here |= (__float_as_uint(ys[j][c]) & 0x7F800000u) == 0x7F800000u;
+                for (int c = tid; c < DZ; c += NT) here |= (__float_as_uint(zs[j][c]) & 0x7F800000u) == 0x7F800000u;
+                if (j == 0) head = __syncthreads_or(here);
+                else if (here) atomicMin(&first_s, j);
             }
             __syncthreads();
             n = first_s;
             if (head && (cuts & ~1u)) n = min(n, (int)__builtin_ctz(cuts & ~1u));
-            cuts &= 0xFFFFFFFFu >> (32 - n);
-            for (int id = threadIdx.x; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0.0f;
-            for (int id = threadIdx.x; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0.0f;
+            cuts &= ~0u >> (32 - n);
+            for (int id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0.0f;
+            for (int id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0.0f;
+            if (pos + n < p1) load(pos + n);
+            factors(cuts);
             __syncthreads();
         }
-        if (want_out) {
-            // P = s1 lam^(i-j) X Y^T of the pairs j <= i of one episode: the three 16 x 16 tiles on
-            // and below the diagonal over the waves
-            for (int q = w; q < 3; q += NW) {
-                const int ri = q > 0, ci = q > 1;
-                floatx4 acc = {0.f, 0.f, 0.f, 0.f};
-                const float *xa = &xs[16 * ri + (lane & 15)][lane >> 4];
-                const float *yb = &ys[16 * ci + (lane & 15)][lane >> 4];
+        floatx4 zv[2], O[2];  // zv: z rows 16 jt + 4 q + r of the wave's columns
 #pragma unroll
-                for (int kk = 0; kk < DX; kk += 4) mfma16(xa[kk], yb[kk], acc);
+        for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) zv[jt][r] = zs[16 * jt + 4 * q + r][col];
+        if (want_out) {
+            // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode: tiles (j, i) on and above the diagonal
+            for (int t = w; t < 3; t += NW) {
+                const int it = t > 0, jt = t > 1;
+                floatx4 P = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int at = 0; at < 2 * DXB; ++at) {
+                    const floatx4 yv = *(const floatx4 *)&ys[16 * jt + l15][16 * at + 4 * q];
+                    const floatx4 xv = *(const floatx4 *)&xs[16 * it + l15][16 * at + 4 * q];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) P = mfma_f32(yv[r], xv[r], P);
+                }
+                const int d0 = 16 * (it - jt) + l15 - 4 * q;
+                const int j0 = cuts ? begin_of(cuts, 16 * it + l15) - 16 * jt - 4 * q : -C;  // of i's episode
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * ri + 4 * (lane >> 4) + r, j = 16 * ci + (lane & 15);
-                    const bool pair = j <= i && j >= begin_of(cuts, i);
-                    ps[i][j] = pair ? acc[r] * (a.s1 * decay_pow(lam2, i - j)) : 0.0f;
+                    P[r] *= a.s1 * decay_pow(lam2, d0 - r);
+                    P[r] = r <= d0 && r >= j0 ? P[r] : 0.0f;  // 0 whatever stood there
                 }
+                ps[t][lane] = P;
             }
-            if (w == 0)
-                for (int r = 0; r < 4; ++r) ps[4 * (lane >> 4) + r][16 + (lane & 15)] = 0.0f;
-            __syncthreads();
-            floatx16 o;
+            // x S, decayed to each row
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[r] = 0.0f;
+            for (int it = 0; it < 2; ++it) O[it] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int ab = 0; ab < DXB; ++ab)
+            for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const floatx4 xv = *(const floatx4 *)&xs[l31][32 * ab + 8 * r4 + 4 * half];
+                for (int it = 0; it < 2; ++it) {
+                    const floatx4 xv = *(const floatx4 *)&xs[16 * it + l15][16 * at + 4 * q];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        o = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[r], S[ab][4 * r4 + r], o, 0, 0, 0);
+                    for (int r = 0; r < 4; ++r) O[it] = mfma_f32(xv[r], S[at][r], O[it]);
                 }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = 8 * (r >> 2) + 4 * half + (r & 3);
-                o[r] = begin_of(cuts, i) < 0 ? o[r] * (a.s2 * decay_pow(lam2, i + a.e0)) : 0.0f;
+            for (int it = 0; it < 2; ++it) {
+                const floatx4 f = *(const floatx4 *)&into_s[16 * it + 4 * q];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) O[it][r] *= f[r];
+                if (cuts) {  // not 0 * inf
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) O[it][r] = f[r] != 0.0f ? O[it][r] : 0.0f;
+                }
+            }
+            __syncthreads();  // P is there
+            const floatx4 p00 = ps[0][lane], p01 = ps[1][lane], p11 = ps[2][lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                O[0] = mfma_f32(p00[r], zv[0][r], O[0]);
+                O[1] = mfma_f32(p01[r], zv[0][r], O[1]);
             }
 #pragma unroll
-            for (int kk = 0; kk < C; kk += 2)
-                o = __builtin_amdgcn_mfma_f32_32x32x2f32(ps[l31][kk + half], zs[kk + half][col], o, 0, 0, 0);
+            for (int r = 0; r < 4; ++r) O[1] = mfma_f32(p11[r], zv[1][r], O[1]);
             if (col < a.dz) {
+                const int64_t at0 = out0 + (pos + 4 * q) * dir * a.ot + col;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = 8 * (r >> 2) + 4 * half + (r & 3);
-                    if (i < n) put(out0 + (pos + i) * dir * a.ot + col, o[r]);
-                }
+                for (int it = 0; it < 2; ++it)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (16 * it + 4 * q + r >= n) continue;
+                        const int64_t at = at0 + (16 * it + r) * dir * a.ot;
+                        if (a.out_f32) ((float *)a.out)[at] = O[it][r];
+                        else ((T *)a.out)[at] = (T)O[it][r];
+                    }
             }
         }
-        // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T over the episode that goes out
-        const int last = begin_of(cuts, n - 1);
-        const float keep = decay_pow(lam2, n);
+        // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T
+        {
+            const float keep = decay_pow(lam2, n);
 #pragma unroll
-        for (int ab = 0; ab < DXB; ++ab)
+            for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[ab][r] = cuts ? 0.0f : S[ab][r] * keep;
+                for (int r = 0; r < 4; ++r) S[at][r] *= keep;
+        }
+        if (cuts) {
 #pragma unroll
-        for (int kk = 0; kk < C; kk += 2) {
-            const int j = kk + half;
-            const float wz = j < n && j >= last ? zs[j][col] * (a.s3 * decay_pow(lam2, n - a.e0 - j)) : 0.0f;
+            for (int at = 0; at < 2 * DXB; ++at) S[at] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
-            for (int ab = 0; ab < DXB; ++ab)
-                S[ab] = __builtin_amdgcn_mfma_f32_32x32x2f32(ys[j][32 * ab + l31], wz, S[ab], 0, 0, 0);
+        for (int jt = 0; jt < 2; ++jt) {
+            const floatx4 f = *(const floatx4 *)&from_s[16 * jt + 4 * q];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float wz = zv[jt][r] * f[r];
+#pragma unroll
+                for (int at = 0; at < 2 * DXB; ++at)
+                    S[at] = mfma_f32(ys[16 * jt + 4 * q + r][16 * at + l15], wz, S[at]);
+            }
         }
         seg_cut |= cuts != 0;
         pos += n;
@@ -259,7 +346,11 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
     // rows behind the sequence's end are 0
     if (want_out)
         for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
-            for (int c = threadIdx.x; c < a.dz; c += NT) put(b * a.ob + h * a.oh + t * a.ot + c, 0.0f);
+            for (int c = tid; c < a.dz; c += NT) {
+                const int64_t at = b * a.ob + h * a.oh + t * a.ot + c;
+                if (a.out_f32) ((float *)a.out)[at] = 0.0f;
+                else ((T *)a.out)[at] = (T)0.0f;
+            }
     float *dst = nullptr;
     int64_t da = a.ia, dn = a.in;
     if (a.mode == 0 && a.fin) dst = a.fin + (int64_t)bh * a.dx * a.dz;
@@ -268,29 +359,20 @@ __global__ __launch_bounds__(64 * NW) void la_walk_kernel(WalkArgs a) {
         // walking backward, what is left belongs to the state before token 0
         const bool drop = a.mode == 0 && a.rev && a.reset && len > 0 && a.reset[b * a.rb] != 0;
 #pragma unroll
-        for (int ab = 0; ab < DXB; ++ab)
+        for (int at = 0; at < 2 * DXB; ++at)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int row = 32 * ab + 8 * (r >> 2) + 4 * half + (r & 3);
-                if (row < a.dx && col < a.dz) dst[row * da + col * dn] = drop ? 0.0f : S[ab][r];
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * at + 4 * q + r;
+                if (row < a.dx && col < a.dz) dst[row * da + col * dn] = drop ? 0.0f : S[at][r];
             }
     }
-    if (a.mode == 1 && threadIdx.x == 0)
+    if (a.mode == 1 && tid == 0)
         a.segf[(int64_t)bh * a.nseg + g] = seg_cut ? -1.0f : decay_pow(lam2, max(p1 - p0, 0));
 }
 
 // ------------------------------------------------------------------------------------------
 // The walk on bfloat16 operands
 // ------------------------------------------------------------------------------------------
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx2 __attribute__((ext_vector_type(2)));
-typedef short shortx4 __attribute__((ext_vector_type(4)));
-typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
-typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
-typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
-typedef uintx4 uintx4_any __attribute__((aligned(2)));  // 16 bytes at any element's address
-
 __device__ __forceinline__ uint32_t pack2(float a, float b) {  // two roundings to nearest even
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2){a, b}, bf16x2));
 }
@@ -769,13 +851,16 @@ int64_t segment_floats(int64_t bh, int T, int Dk, int Dv) {
 template <typename T, int DXB>
 void launch_walk(const WalkArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.B * a.H), a.nseg);
-    if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0) {
-        if (a.dz <= 32) la_walk_bf16_kernel<DXB, 2><<<grid, 128, 0, s>>>(a);
-        else if (a.dz <= 64) la_walk_bf16_kernel<DXB, 4><<<grid, 256, 0, s>>>(a);
-        else la_walk_bf16_kernel<DXB, 8><<<grid, 512, 0, s>>>(a);
-    } else if (a.dz <= 32) la_walk_kernel<T, DXB, 1><<<grid, 64, 0, s>>>(a);
-    else if (a.dz <= 64) la_walk_kernel<T, DXB, 2><<<grid, 128, 0, s>>>(a);
-    else la_walk_kernel<T, DXB, 4><<<grid, 256, 0, s>>>(a);
+    auto go = [&](auto nw) {
+        constexpr int NW = decltype(nw)::value;
+        if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0)
+            la_walk_bf16_kernel<DXB, NW><<<grid, 64 * NW, 0, s>>>(a);
+        else
+            la_walk_kernel<T, DXB, NW><<<grid, 64 * NW, 0, s>>>(a);
+    };
+    if (a.dz <= 32) go(std::integral_constant<int, 2>{});
+    else if (a.dz <= 64) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
 }
 
 template <typename T>
