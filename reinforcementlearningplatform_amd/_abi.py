@@ -6,6 +6,7 @@ SURVEY.md §8a "Per-copy constants"); the citing path:line is relative to the re
 """
 import ctypes as C
 import math
+import struct
 
 import numpy as np
 
@@ -427,6 +428,9 @@ class LACfg(C.Structure):  # rlp_la_cfg
                 ("o_stride", C.c_int64 * 3), ("dq_stride", C.c_int64 * 3),
                 ("dk_stride", C.c_int64 * 3), ("dv_stride", C.c_int64 * 3),
                 ("reset_stride", C.c_int64 * 2)]
+
+
+LA_CFG_PACK = struct.Struct("=9if23q")  # LACfg's bytes in one call (acting pays for every attribute set)
 
 
 def check_struct_sizes():

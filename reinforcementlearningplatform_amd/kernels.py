@@ -3,6 +3,7 @@
 All tensors live on the ROCm device. Nothing here falls back to the CPU.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -508,116 +509,109 @@ def sac_update(nets, cfg, s, a, r, s_next, dw, noise, work, losses):
 
 
 # ---------------------------------------------------------------------------------------------
-# Sequence policies (include/rlp.h: rlp_linear_attention*, rlp_token_logprob*)
+# Sequence policies (include/rlp.h: rlp_linear_attention*, rlp_token_logprob*). Acting calls these once
+# a step, so the wrappers count their microseconds: one packed cfg, plain integers for pointers.
 # ---------------------------------------------------------------------------------------------
 _DTYPES = {torch.float32: _abi.RLP_F32, torch.float16: _abi.RLP_F16, torch.bfloat16: _abi.RLP_BF16}
 
 
-def _on_gpu(what, **tensors):
-    """All tensors on one ROCm device (returned); None entries are skipped."""
-    dev = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RLPError(f"{what}: {name} is not on the GPU (librlp takes device tensors only)")
-        if dev is not None and t.device != dev:
-            raise RLPError(f"{what}: {name} is on {t.device}, the others on {dev}")
-        dev = t.device
-    return dev
+# torch.cuda.current_device / current_stream without their Python (3 us a call, 15 in a backward thread)
+_device_index = torch._C._cuda_getDevice
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _dtype_of(what, t):
-    if t.dtype not in _DTYPES:
-        raise RLPError(f"{what}: dtype {t.dtype} (float32, float16 or bfloat16)")
-    return _DTYPES[t.dtype]
+def _launch(what, tensors, fn, *args):
+    """fn(*args, stream) on the tensors' device, with its current stream."""
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise RLPError(f"{what}: not on the GPU, or on several (librlp takes tensors of one device)")
+    if dev == _device_index():
+        rc = fn(*args, _stream_of(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream_of(dev))
+    if rc != 0:
+        check(rc, what)
 
 
-def _raw(t):
-    return C.c_void_p(t.data_ptr()) if t is not None else None
+def _at(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _rows(x):
     """x with its last axis contiguous; every other axis may have any stride."""
-    return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
+    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
 def _like_order(ref, B, T, H, D):
     """An empty [B][T][H][D] tensor in ref's order of the batch and token axes (rollout buffers are
     time-major)."""
-    if ref.dim() == 4 and B > 1 and T > 1 and ref.stride(0) < ref.stride(1):
-        return torch.empty((T, B, H, D), dtype=ref.dtype, device=ref.device).transpose(0, 1)
-    return torch.empty((B, T, H, D), dtype=ref.dtype, device=ref.device)
+    if B > 1 and T > 1 and ref.stride(0) < ref.stride(1):
+        return ref.new_empty((T, B, H, D)).transpose(0, 1)
+    return ref.new_empty((B, T, H, D))
 
 
-def _la_flags(what, reset, lengths, B, T):
-    if reset is not None:
-        if reset.dtype == torch.bool:
-            reset = reset.view(torch.uint8)
-        want = (B,) if T is None else (B, T)
-        if reset.dtype != torch.uint8 or tuple(reset.shape) != want:
-            raise RLPError(f"{what}: reset {reset.dtype} {tuple(reset.shape)}, uint8 or bool {want} needed")
-    if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,)):
-        raise RLPError(f"{what}: lengths {lengths.dtype} {tuple(lengths.shape)}, int32 ({B},) needed")
-    return reset, None if lengths is None else lengths.contiguous()
+@functools.lru_cache(maxsize=1024)
+def _la_workspace_bytes(what, backward, *dims):
+    """Scratch of a call of these sizes; raises for sizes that the library refuses."""
+    cfg = _abi.LA_CFG_PACK.pack(*dims, 1.0, *(0,) * 23)
+    need = int(lib().rlp_linear_attention_workspace_bytes(cfg, backward))
+    if need < 0:
+        check(need, what)
+    return need
 
 
-def _la_cfg(what, q, k, v, log_decay, scale, state):
-    """rlp_la_cfg of q, k, v [B][T][heads][D] after the checks that need no device."""
+def _la_dims(what, q, k, v, log_decay, state):
+    """(dtype, B, T, H, Hq, Hk, Hv, Dk, Dv) of q, k, v [B][T][heads][D]."""
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise RLPError(f"{what}: {name} of {t.dim()} axes")
         if t.dtype != q.dtype:
             raise RLPError(f"{what}: {name} is {t.dtype}, q {q.dtype}")
-    B, T, Hq, Dk = q.shape
-    if k.shape[:2] != q.shape[:2] or v.shape[:2] != q.shape[:2] or k.shape[3] != Dk:
+    if q.dtype not in _DTYPES:
+        raise RLPError(f"{what}: dtype {q.dtype} (float32, float16 or bfloat16)")
+    (B, T, Hq, Dk), (Bk, Tk, Hk, Dk2), (Bv, Tv, Hv, Dv) = q.shape, k.shape, v.shape
+    if B != Bk or B != Bv or T != Tk or T != Tv or Dk != Dk2:
         raise RLPError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
-    Hk, Hv, Dv = k.shape[2], v.shape[2], v.shape[3]
     if log_decay.dim() != 1 or log_decay.dtype != torch.float32:
         raise RLPError(f"{what}: log_decay {log_decay.dtype} {tuple(log_decay.shape)}, float32 (heads,) needed")
     H = log_decay.shape[0]
-    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != (B, H, Dk, Dv)):
+    if state is not None and (state.dtype != torch.float32 or state.shape != (B, H, Dk, Dv)):
         raise RLPError(f"{what}: state {state.dtype} {tuple(state.shape)}, float32 {(B, H, Dk, Dv)} needed")
-    c = _abi.LACfg()
-    c.dtype = _dtype_of(what, q)
-    c.B, c.T, c.H, c.Hq, c.Hk, c.Hv, c.Dk, c.Dv = B, T, H, Hq, Hk, Hv, Dk, Dv
-    c.scale = float(Dk ** -0.5 if scale is None else scale)
-    need = int(lib().rlp_linear_attention_workspace_bytes(C.byref(c), 0))
-    check(need if need < 0 else 0, what)
-    return c
+    return _DTYPES[q.dtype], B, T, H, Hq, Hk, Hv, Dk, Dv
 
 
-def _set_strides(c, **tensors):
-    for name, t in tensors.items():
-        if t is not None:
-            setattr(c, name + "_stride", type(getattr(c, name + "_stride"))(*t.stride()[:3]))
-
-
-def _la_workspace(c, backward, dev):
-    need = int(lib().rlp_linear_attention_workspace_bytes(C.byref(c), int(backward)))
-    check(need if need < 0 else 0, "rlp_linear_attention_workspace_bytes")
-    return torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None, need
+def _la_flags(what, reset, lengths, want, B):
+    if reset is not None:
+        if reset.dtype == torch.bool:
+            reset = reset.view(torch.uint8)
+        if reset.dtype != torch.uint8 or reset.shape != want:
+            raise RLPError(f"{what}: reset {reset.dtype} {tuple(reset.shape)}, uint8 or bool {want} needed")
+    if lengths is not None and (lengths.dtype != torch.int32 or lengths.shape != (B,)):
+        raise RLPError(f"{what}: lengths {lengths.dtype} {tuple(lengths.shape)}, int32 ({B},) needed")
+    return reset, None if lengths is None else lengths.contiguous()
 
 
 def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=None, lengths=None,
                              return_state=False):
     """rlp_linear_attention without autograd (arguments as linear_attention): (out, state or None)."""
     what = "linear_attention"
-    c = _la_cfg(what, q, k, v, log_decay, scale, state)
-    reset, lengths = _la_flags(what, reset, lengths, c.B, c.T)
-    dev = _on_gpu(what, q=q, k=k, v=v, log_decay=log_decay, state=state, reset=reset, lengths=lengths)
-    with torch.cuda.device(dev):
-        q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-        state = state.contiguous() if state is not None else None
-        out = _like_order(q, c.B, c.T, c.H, c.Dv)
-        last = torch.empty((c.B, c.H, c.Dk, c.Dv), dtype=torch.float32, device=dev) if return_state else None
-        _set_strides(c, q=q, k=k, v=v, o=out)
-        if reset is not None:
-            c.reset_stride[:] = reset.stride()
-        ws, need = _la_workspace(c, False, dev)
-        check(lib().rlp_linear_attention(C.byref(c), _raw(q), _raw(k), _raw(v), _raw(log_decay),
-                                         _raw(reset), _raw(lengths), _raw(state), _raw(out), _raw(last),
-                                         _raw(ws), need, stream_ptr()), "rlp_linear_attention")
+    dims = _la_dims(what, q, k, v, log_decay, state)
+    need = _la_workspace_bytes(what, 0, *dims)
+    _, B, T, H, _, _, _, Dk, Dv = dims
+    reset, lengths = _la_flags(what, reset, lengths, (B, T), B)
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    state = state.contiguous() if state is not None else None
+    out = _like_order(q, B, T, H, Dv)
+    last = log_decay.new_empty((B, H, Dk, Dv)) if return_state else None
+    ws = log_decay.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale, *q.stride()[:3],
+                                *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *(0,) * 9,
+                                *(reset.stride() if reset is not None else (0, 0)))
+    _launch(what, (q, k, v, log_decay, state, reset, lengths), lib().rlp_linear_attention, cfg,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _at(reset), _at(lengths),
+            _at(state), out.data_ptr(), _at(last), _at(ws), need)
     return out, last
 
 
@@ -626,31 +620,28 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
     """rlp_linear_attention_backward: (dq, dk, dv, gradient of state or None) from the gradients of
     linear_attention's out and state (d_state None: 0)."""
     what = "linear_attention_backward"
-    c = _la_cfg(what, q, k, v, log_decay, scale, state)
-    reset, lengths = _la_flags(what, reset, lengths, c.B, c.T)
-    if tuple(d_out.shape) != (c.B, c.T, c.H, c.Dv) or d_out.dtype != q.dtype:
+    dims = _la_dims(what, q, k, v, log_decay, state)
+    need = _la_workspace_bytes(what, 1, *dims)
+    _, B, T, H, Hq, Hk, Hv, Dk, Dv = dims
+    reset, lengths = _la_flags(what, reset, lengths, (B, T), B)
+    if d_out.shape != (B, T, H, Dv) or d_out.dtype != q.dtype:
         raise RLPError(f"{what}: d_out {d_out.dtype} {tuple(d_out.shape)}")
-    if d_state is not None and (d_state.dtype != torch.float32 or
-                                tuple(d_state.shape) != (c.B, c.H, c.Dk, c.Dv)):
+    if d_state is not None and (d_state.dtype != torch.float32 or d_state.shape != (B, H, Dk, Dv)):
         raise RLPError(f"{what}: d_state {d_state.dtype} {tuple(d_state.shape)}")
-    dev = _on_gpu(what, q=q, k=k, v=v, log_decay=log_decay, state=state, reset=reset, lengths=lengths,
-                  d_out=d_out, d_state=d_state)
-    with torch.cuda.device(dev):
-        q, k, v, d_out, log_decay = _rows(q), _rows(k), _rows(v), _rows(d_out), log_decay.contiguous()
-        first = torch.empty((c.B, c.H, c.Dk, c.Dv), dtype=torch.float32, device=dev) \
-            if state is not None else None
-        state = state.contiguous() if state is not None else None
-        d_state = d_state.contiguous() if d_state is not None else None
-        dq, dk = _like_order(q, c.B, c.T, c.Hq, c.Dk), _like_order(k, c.B, c.T, c.Hk, c.Dk)
-        dv = _like_order(v, c.B, c.T, c.Hv, c.Dv)
-        _set_strides(c, q=q, k=k, v=v, o=d_out, dq=dq, dk=dk, dv=dv)
-        if reset is not None:
-            c.reset_stride[:] = reset.stride()
-        ws, need = _la_workspace(c, True, dev)
-        check(lib().rlp_linear_attention_backward(
-            C.byref(c), _raw(q), _raw(k), _raw(v), _raw(log_decay), _raw(reset), _raw(lengths),
-            _raw(state), _raw(d_out), _raw(d_state), _raw(dq), _raw(dk), _raw(dv), _raw(first), _raw(ws),
-            need, stream_ptr()), "rlp_linear_attention_backward")
+    q, k, v, d_out, log_decay = _rows(q), _rows(k), _rows(v), _rows(d_out), log_decay.contiguous()
+    first = torch.empty_like(state, memory_format=torch.contiguous_format) if state is not None else None
+    state = state.contiguous() if state is not None else None
+    d_state = d_state.contiguous() if d_state is not None else None
+    dq, dk, dv = _like_order(q, B, T, Hq, Dk), _like_order(k, B, T, Hk, Dk), _like_order(v, B, T, Hv, Dv)
+    ws = log_decay.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale, *q.stride()[:3],
+                                *k.stride()[:3], *v.stride()[:3], *d_out.stride()[:3], *dq.stride()[:3],
+                                *dk.stride()[:3], *dv.stride()[:3],
+                                *(reset.stride() if reset is not None else (0, 0)))
+    _launch(what, (q, k, v, log_decay, state, reset, lengths, d_out, d_state),
+            lib().rlp_linear_attention_backward, cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            log_decay.data_ptr(), _at(reset), _at(lengths), _at(state), d_out.data_ptr(), _at(d_state),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(first), _at(ws), need)
     return dq, dk, dv, first
 
 
@@ -666,10 +657,10 @@ class _LinearAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, d_state=None):
+        if d_out is None and d_state is None:
+            return (None,) * 9
         q, k, v, log_decay, state, reset, lengths = ctx.saved_tensors
         if d_out is None:
-            if d_state is None:
-                return (None,) * 9
             d_out = _like_order(q, q.shape[0], q.shape[1], log_decay.shape[0], v.shape[3]).zero_()
         dq, dk, dv, first = linear_attention_backward(d_out, d_state, q, k, v, log_decay, ctx.scale, state,
                                                       reset, lengths)
@@ -692,9 +683,15 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, len
 
     In a captured HIP graph, capture forward and backward together, with no graph of the same leaves
     alive from outside the capture (torch keeps one accumulation node per leaf and its stream)."""
-    if torch.is_grad_enabled() and log_decay.requires_grad:
-        raise RLPError("linear_attention: log_decay has no gradient (pass it detached)")
-    return _LinearAttention.apply(q, k, v, log_decay, scale, state, reset, lengths, bool(return_state))
+    if torch.is_grad_enabled():
+        if log_decay.requires_grad:
+            raise RLPError("linear_attention: log_decay has no gradient (pass it detached)")
+        if q.requires_grad or k.requires_grad or v.requires_grad or \
+                state is not None and state.requires_grad:
+            return _LinearAttention.apply(q, k, v, log_decay, scale, state, reset, lengths,
+                                          bool(return_state))
+    out, last = linear_attention_forward(q, k, v, log_decay, scale, state, reset, lengths, return_state)
+    return (out, last) if return_state else out
 
 
 def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, state_out=None, out=None):
@@ -702,61 +699,73 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, sta
     v [B][heads][Dv], state float32 [B][H][Dk][Dv] contiguous, updated in place or written to state_out;
     reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv]. Not differentiable."""
     what = "linear_attention_step"
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                    log_decay.requires_grad or state.requires_grad):
         raise RLPError(f"{what}: not differentiable (call it under torch.no_grad, or linear_attention)")
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 3:
             raise RLPError(f"{what}: {name} of {t.dim()} axes")
-    c = _la_cfg(what, q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), log_decay, scale, state)
-    reset, _ = _la_flags(what, reset, None, c.B, None)
-    state_out = state if state_out is None else state_out
-    shape = (c.B, c.H, c.Dv)
-    if state_out.shape != state.shape or state_out.dtype != torch.float32:
-        raise RLPError(f"{what}: state_out {state_out.dtype} {tuple(state_out.shape)}")
-    if not state.is_contiguous() or not state_out.is_contiguous():
+    dims = _la_dims(what, q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), log_decay, state)
+    _la_workspace_bytes(what, 0, *dims)
+    _, B, _, H, _, _, _, Dk, Dv = dims
+    reset, _ = _la_flags(what, reset, None, (B,), B)
+    if not state.is_contiguous():
         raise RLPError(f"{what}: state and state_out have to be contiguous")
-    lo, n = state.data_ptr(), 4 * state.numel()
-    if state_out.data_ptr() != lo and abs(state_out.data_ptr() - lo) < n:
-        raise RLPError(f"{what}: state_out overlaps state (pass state itself for an update in place)")
-    if out is not None and (tuple(out.shape) != shape or out.dtype != q.dtype or not out.is_contiguous()):
-        raise RLPError(f"{what}: out {out.dtype} {tuple(out.shape)}, contiguous {q.dtype} {shape} needed")
-    dev = _on_gpu(what, q=q, k=k, v=v, log_decay=log_decay, state=state, state_out=state_out, reset=reset,
-                  out=out)
-    with torch.cuda.device(dev):
-        q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
-        out = torch.empty(shape, dtype=q.dtype, device=dev) if out is None else out
-        for name, t in (("q", q), ("k", k), ("v", v), ("o", out)):
-            getattr(c, name + "_stride")[:] = (t.stride(0), 0, t.stride(1))
-        if reset is not None:
-            c.reset_stride[0] = reset.stride(0)
-        check(lib().rlp_linear_attention_step(C.byref(c), _raw(q), _raw(k), _raw(v), _raw(log_decay),
-                                              _raw(reset), _raw(state), _raw(state_out), _raw(out),
-                                              stream_ptr()), "rlp_linear_attention_step")
+    if state_out is None:
+        state_out = state
+    elif state_out is not state:
+        if state_out.shape != state.shape or state_out.dtype != torch.float32:
+            raise RLPError(f"{what}: state_out {state_out.dtype} {tuple(state_out.shape)}")
+        if not state_out.is_contiguous():
+            raise RLPError(f"{what}: state and state_out have to be contiguous")
+        apart = abs(state_out.data_ptr() - state.data_ptr())
+        if 0 < apart < 4 * state.numel():
+            raise RLPError(f"{what}: state_out overlaps state (pass state itself for an update in place)")
+    if out is None:
+        out = q.new_empty((B, H, Dv))
+    elif out.shape != (B, H, Dv) or out.dtype != q.dtype or not out.is_contiguous():
+        raise RLPError(f"{what}: out {out.dtype} {tuple(out.shape)}, contiguous {q.dtype} {(B, H, Dv)} needed")
+    q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
+    cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale,
+                                q.stride(0), 0, q.stride(1), k.stride(0), 0, k.stride(1),
+                                v.stride(0), 0, v.stride(1), H * Dv, 0, Dv, *(0,) * 9,
+                                reset.stride(0) if reset is not None else 0, 0)
+    _launch(what, (q, k, v, log_decay, state, state_out, reset, out), lib().rlp_linear_attention_step, cfg,
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _at(reset), state.data_ptr(),
+            state_out.data_ptr(), out.data_ptr())
     return out
 
 
-def token_logprob_forward(logits, tokens, temperature=1.0, top_k=0):
+@functools.lru_cache(maxsize=1024)
+def _lp_workspace_bytes(what, rows, vocab, top_k, dtype):
+    need = int(lib().rlp_token_logprob_workspace_bytes(rows, vocab, top_k, dtype))
+    if need < 0:
+        check(need, what)
+    return need
+
+
+def token_logprob_forward(logits, tokens, temperature=1.0, top_k=0, want_stats=True):
     """rlp_token_logprob without autograd on logits [rows][vocab], tokens [rows] int64: (logp, entropy,
     stats, top_logp, top_tokens); stats feeds token_logprob_backward, top_* are None for top_k 0."""
     what = "token_logprob"
-    if logits.dim() != 2 or tuple(tokens.shape) != (logits.shape[0],) or tokens.dtype != torch.int64:
+    if logits.dim() != 2 or tokens.dim() != 1 or tokens.shape[0] != logits.shape[0] or \
+            tokens.dtype != torch.int64:
         raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
-    dev, dt, top_k = _on_gpu(what, logits=logits, tokens=tokens), _dtype_of(what, logits), int(top_k)
+    dt = _DTYPES.get(logits.dtype)
+    if dt is None:
+        raise RLPError(f"{what}: dtype {logits.dtype} (float32, float16 or bfloat16)")
     rows, vocab = logits.shape
-    need = int(lib().rlp_token_logprob_workspace_bytes(rows, vocab, top_k, dt))
-    check(need if need < 0 else 0, what)
-    with torch.cuda.device(dev):
-        logits, tokens = _rows(logits), tokens.contiguous()
-        f32 = dict(dtype=torch.float32, device=dev)
-        logp, entropy = torch.empty(rows, **f32), torch.empty(rows, **f32)
-        stats = torch.empty((rows, 3), **f32)
-        top_logp = torch.empty((rows, top_k), **f32) if top_k else None
-        top_tokens = torch.empty((rows, top_k), dtype=torch.int64, device=dev) if top_k else None
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-        check(lib().rlp_token_logprob(_raw(logits), dt, rows, vocab, logits.stride(0), _raw(tokens),
-                                      float(temperature), top_k, _raw(logp), _raw(entropy), _raw(stats),
-                                      _raw(top_logp), _raw(top_tokens), _raw(ws), need, stream_ptr()),
-              "rlp_token_logprob")
+    need = _lp_workspace_bytes(what, rows, vocab, top_k, dt)
+    logits, tokens = _rows(logits), tokens.contiguous()
+    logp = logits.new_empty(rows, dtype=torch.float32)
+    entropy = torch.empty_like(logp)
+    stats = logp.new_empty((rows, 3)) if want_stats else None
+    top_logp = logp.new_empty((rows, top_k)) if top_k else None
+    top_tokens = tokens.new_empty((rows, top_k)) if top_k else None
+    ws = logp.new_empty(need, dtype=torch.uint8) if need > 0 else None
+    _launch(what, (logits, tokens), lib().rlp_token_logprob, logits.data_ptr(), dt, rows, vocab,
+            logits.stride(0), tokens.data_ptr(), temperature, top_k, logp.data_ptr(), entropy.data_ptr(),
+            _at(stats), _at(top_logp), _at(top_tokens), _at(ws), need)
     return logp, entropy, stats, top_logp, top_tokens
 
 
@@ -765,22 +774,21 @@ def token_logprob_backward(d_logp, d_entropy, logits, tokens, stats, temperature
     what = "token_logprob_backward"
     rows, vocab = logits.shape
     for name, t in (("d_logp", d_logp), ("d_entropy", d_entropy)):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (rows,)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (rows,)):
             raise RLPError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, float32 ({rows},) needed")
-    if tuple(stats.shape) != (rows, 3) or stats.dtype != torch.float32 or tokens.dtype != torch.int64 or \
-            tuple(tokens.shape) != (rows,):
+    if stats.shape != (rows, 3) or stats.dtype != torch.float32 or tokens.dtype != torch.int64 or \
+            tokens.shape != (rows,):
         raise RLPError(f"{what}: stats {tuple(stats.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
-    dev, dt = _on_gpu(what, logits=logits, tokens=tokens, stats=stats, d_logp=d_logp,
-                      d_entropy=d_entropy), _dtype_of(what, logits)
-    with torch.cuda.device(dev):
-        logits, tokens, stats = _rows(logits), tokens.contiguous(), stats.contiguous()
-        d_logp = d_logp.contiguous() if d_logp is not None else None
-        d_entropy = d_entropy.contiguous() if d_entropy is not None else None
-        d_logits = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
-        check(lib().rlp_token_logprob_backward(_raw(logits), dt, rows, vocab, logits.stride(0), _raw(tokens),
-                                               float(temperature), _raw(stats), _raw(d_logp),
-                                               _raw(d_entropy), _raw(d_logits), vocab, stream_ptr()),
-              "rlp_token_logprob_backward")
+    dt = _DTYPES.get(logits.dtype)
+    if dt is None:
+        raise RLPError(f"{what}: dtype {logits.dtype} (float32, float16 or bfloat16)")
+    logits, tokens, stats = _rows(logits), tokens.contiguous(), stats.contiguous()
+    d_logp = d_logp.contiguous() if d_logp is not None else None
+    d_entropy = d_entropy.contiguous() if d_entropy is not None else None
+    d_logits = logits.new_empty((rows, vocab))
+    _launch(what, (logits, tokens, stats, d_logp, d_entropy), lib().rlp_token_logprob_backward,
+            logits.data_ptr(), dt, rows, vocab, logits.stride(0), tokens.data_ptr(), temperature,
+            stats.data_ptr(), _at(d_logp), _at(d_entropy), d_logits.data_ptr(), vocab)
     return d_logits
 
 
@@ -816,13 +824,22 @@ def token_logprob(logits, tokens, temperature=1.0, top_k=0):
     probable tokens, (logp, entropy, top_logp, top_tokens [...][top_k]), ties to the lower token; those
     two carry no gradient."""
     what = "token_logprob"
-    if logits.dim() < 1 or tuple(tokens.shape) != tuple(logits.shape[:-1]):
-        raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tuple(tokens.shape)}")
-    if tokens.dtype not in (torch.int64, torch.int32):
-        raise RLPError(f"{what}: tokens {tokens.dtype} (int64 or int32)")
-    shape, vocab = tuple(tokens.shape), logits.shape[-1]
+    shape, top_k, temperature = tokens.shape, int(top_k), float(temperature)
+    if logits.dim() < 1 or shape != logits.shape[:-1]:
+        raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tuple(shape)}")
+    if tokens.dtype != torch.int64:
+        if tokens.dtype != torch.int32:
+            raise RLPError(f"{what}: tokens {tokens.dtype} (int64 or int32)")
+        tokens = tokens.long()
+    vocab = logits.shape[-1]
     if vocab < 1:
         raise RLPError(f"{what}: no logits in a row")
-    res = _TokenLogprob.apply(logits.reshape(-1, vocab), tokens.reshape(-1).long(), float(temperature),
-                              int(top_k))
-    return tuple(r.view(shape if r.dim() == 1 else shape + (int(top_k),)) for r in res)
+    flat = len(shape) == 1
+    if not flat:
+        logits, tokens = logits.reshape(-1, vocab), tokens.reshape(-1)
+    if logits.requires_grad and torch.is_grad_enabled():
+        res = _TokenLogprob.apply(logits, tokens, temperature, top_k)
+    else:
+        logp, entropy, _, top_logp, top_tokens = token_logprob_forward(logits, tokens, temperature, top_k, False)
+        res = (logp, entropy, top_logp, top_tokens) if top_k else (logp, entropy)
+    return res if flat else tuple(r.view(shape if r.dim() == 1 else shape + (top_k,)) for r in res)

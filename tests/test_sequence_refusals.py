@@ -62,7 +62,7 @@ def test_linear_attention_nulls_and_workspace():
     c.Hq = 1
     assert lib.rlp_linear_attention_workspace_bytes(C.byref(c), 1) >= need + 4 * 4096 * 4 * 16
     c = la()
-    c.B = 0
+    c.B, c.T = 0, 4096
     assert la_forward(c) == 0 and lib.rlp_linear_attention_workspace_bytes(C.byref(c), 1) == 0
 
 
