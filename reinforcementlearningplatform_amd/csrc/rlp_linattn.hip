@@ -772,8 +772,10 @@ __global__ __launch_bounds__(256) void la_share_kernel(const float *part, T *out
     }
 }
 
-// One token for every sequence: reads and writes each state once. A block owns 32 columns of one
-// (batch, head) state: 8 lanes of 4 columns x 32 rows at a time.
+// One token for every sequence: reads and writes each state once, 4 columns a lane, LC lanes a row, four
+// rows' loads in flight. A block owns 4 LC columns of one (batch, head) state. Bound by HBM: 16384 x 4
+// states of 64 x 64 from one buffer to another in 346 us, 6.2 TB/s. STREAM: loads and stores that pass
+// the caches by, for states that do not stay in them (see the launch).
 struct StepArgs {
     const void *q, *k, *v;
     void *out;
@@ -788,39 +790,72 @@ struct StepArgs {
     int H, dk, dv;
 };
 
-template <typename T>
+typedef floatx4 floatx4_any __attribute__((aligned(4)));
+
+template <typename T, int LC, bool STREAM>
 __global__ __launch_bounds__(256) void la_step_kernel(StepArgs a) {
-    __shared__ float part[32][33];
+    constexpr int R = 256 / LC, U = 4;  // rows at a time, times in flight
+    __shared__ float part[R][4 * LC + 1];
     const int64_t bh = blockIdx.x;
     const int b = (int)(bh / a.H), h = (int)(bh % a.H);
-    const int c0 = blockIdx.y * 32 + (threadIdx.x & 7) * 4, r0 = threadIdx.x >> 3;
+    const int lc = threadIdx.x % LC, r0 = threadIdx.x / LC, c0 = (blockIdx.y * LC + lc) * 4;
     const T *q = (const T *)a.q + b * a.qb + (h / a.gq) * a.qh;
     const T *k = (const T *)a.k + b * a.kb + (h / a.gk) * a.kh;
     const T *v = (const T *)a.v + b * a.vb + (h / a.gv) * a.vh;
     const bool drop = a.reset && a.reset[b * a.rb] != 0;
-    const float lam = __builtin_amdgcn_exp2f(a.log_decay[h] * kLog2e);
+    const float lam = decay_pow(log2_decay(a.log_decay[h]), 1);
+    const bool full = c0 + 4 <= a.dv;
     float vc[4], o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 4; ++e) vc[e] = c0 + e < a.dv ? to_f32(v[c0 + e]) : 0.0f;
-    const int64_t base = bh * a.dk * a.dv;
-    for (int r = r0; r < a.dk; r += 32) {
-        const float kr = to_f32(k[r]), qr = to_f32(q[r]);
+    const float *src = a.state + bh * a.dk * a.dv + c0;
+    float *dst = a.state_out + bh * a.dk * a.dv + c0;
+    for (int rb = r0; rb < a.dk; rb += R * U) {
+        floatx4 s[U];
+        float kr[U], qr[U];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (c0 + e >= a.dv) continue;
-            const int64_t at = base + (int64_t)r * a.dv + c0 + e;
-            const float s = (drop ? 0.0f : lam * a.state[at]) + kr * vc[e];
-            a.state_out[at] = s;
-            o[e] += qr * s;
+        for (int u = 0; u < U; ++u) {
+            const int r = rb + u * R;
+            s[u] = (floatx4){0.f, 0.f, 0.f, 0.f};
+            if (r >= a.dk) continue;
+            kr[u] = to_f32(k[r]), qr[u] = to_f32(q[r]);
+            if (drop) continue;
+            if (full) {
+                const floatx4_any *p = (const floatx4_any *)(src + r * a.dv);
+                s[u] = STREAM ? __builtin_nontemporal_load(p) : *p;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (c0 + e < a.dv) s[u][e] = src[r * a.dv + e];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int r = rb + u * R;
+            if (r >= a.dk) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[u][e] = lam * s[u][e] + kr[u] * vc[e];
+                o[e] += qr[u] * s[u][e];
+            }
+            if (full) {
+                if (STREAM) __builtin_nontemporal_store(s[u], (floatx4_any *)(dst + r * a.dv));
+                else *(floatx4_any *)(dst + r * a.dv) = s[u];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (c0 + e < a.dv) dst[r * a.dv + e] = s[u][e];
+            }
         }
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) part[r0][(threadIdx.x & 7) * 4 + e] = o[e];
+    for (int e = 0; e < 4; ++e) part[r0][lc * 4 + e] = o[e];
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int c = blockIdx.y * 32 + threadIdx.x;
+    if (threadIdx.x < 4 * LC) {
+        const int c = blockIdx.y * 4 * LC + threadIdx.x;
         float s = 0.0f;
-        for (int r = 0; r < 32; ++r) s += part[r][threadIdx.x];
+#pragma unroll
+        for (int r = 0; r < R; ++r) s += part[r][threadIdx.x];
         if (c < a.dv) ((T *)a.out)[b * a.ob + h * a.oh + c] = (T)(a.scale * s);
     }
 }
@@ -1092,9 +1127,22 @@ int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *
     a.gq = cfg->H / cfg->Hq, a.gk = cfg->H / cfg->Hk, a.gv = cfg->H / cfg->Hv;
     a.reset = reset, a.rb = cfg->reset_stride[0];
     a.scale = cfg->scale, a.H = cfg->H, a.dk = cfg->Dk, a.dv = cfg->Dv;
-    const dim3 grid((unsigned)((int64_t)cfg->B * cfg->H), (cfg->Dv + 31) / 32);
+    // few states: narrow blocks, more of them on the card; many: whole 256-byte rows
+    const int64_t bh = (int64_t)cfg->B * cfg->H;
+    const bool narrow = cfg->Dv <= 32 || bh < 512;
+    // states beyond the 256 MB last-level cache: past it, 512 MB in place in 167 us for 196 (within it the
+    // next step finds them: 128 MB 41 us for 44)
+    const bool stream_by = bh * cfg->Dk * cfg->Dv * (state == state_out ? 4 : 8) > (256LL << 20);
+    const dim3 grid((unsigned)bh, narrow ? (cfg->Dv + 31) / 32 : (cfg->Dv + 63) / 64);
     by_type(cfg->dtype, [&](auto *t) {
-        la_step_kernel<std::remove_pointer_t<decltype(t)>><<<grid, 256, 0, as_stream(stream)>>>(a);
+        using T = std::remove_pointer_t<decltype(t)>;
+        if (stream_by) {
+            if (narrow) la_step_kernel<T, 8, true><<<grid, 256, 0, as_stream(stream)>>>(a);
+            else la_step_kernel<T, 16, true><<<grid, 256, 0, as_stream(stream)>>>(a);
+        } else {
+            if (narrow) la_step_kernel<T, 8, false><<<grid, 256, 0, as_stream(stream)>>>(a);
+            else la_step_kernel<T, 16, false><<<grid, 256, 0, as_stream(stream)>>>(a);
+        }
     });
     RLP_CHECK_LAUNCH("rlp_linear_attention_step");
     return RLP_OK;
