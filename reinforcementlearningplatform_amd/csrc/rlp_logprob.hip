@@ -4,8 +4,10 @@
 // One pass over the logits: with m the largest so far, s = sum 2^y and w = sum 2^y y of
 // y = (l - m) log2(e) / temperature, rescaled when m grows,
 //   logp = ln 2 (y_token - log2 s),   entropy = ln 2 (log2 s - w / s).
-// y is formed from the difference l - m, not from scaled logits, so a row of the type's lowest
-// values is the uniform row it should be and large logits lose nothing. Sums are f32.
+// In the loops y is one fma, l c - rnd(m c) with c = log2(e) / temperature: a logit's product is exact
+// inside it, and what rounding m c put into every y alike (m c - rnd(m c)) is taken out of the sums at
+// the end, so large logits lose nothing. Where l c could overflow (|m| >= 1e30: a row of the type's lowest
+// values, which is the uniform row it should be) y is formed from the difference l - m. Sums are f32.
 #include "rlp_common.hpp"
 
 namespace rlp {
@@ -36,6 +38,25 @@ struct ScoreArgs {
 
 struct Sums {
     float m, s, w;  // m -inf: nothing but -inf so far
+};
+
+// max(a, b, c) of numbers; a NaN is passed over (it shows in the sums). As an instruction: fmaxf puts a
+// canonicalising copy before every operand that comes from memory.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+// y = l c - mc of the logits of a row with maximum m; off: what is in every y beside (l - m) c
+struct Shift {
+    float mc, off;
+    bool far;  // m c may overflow: (l - m) c instead
+    __device__ __forceinline__ Shift(float m, float c) {
+        far = !(fabsf(m) < 1e30f);
+        mc = m * c;
+        off = far ? 0.0f : __builtin_fmaf(m, c, -mc);
+    }
 };
 
 __device__ __forceinline__ float base_of(float m) { return m == neg_inf() ? 0.0f : m; }
@@ -172,25 +193,27 @@ struct TopList {
     __device__ int worst_i(int k) const { return __builtin_amdgcn_readlane(i, k - 1); }
 };
 
-// The k-th largest of a wave's 64 values: bit by bit on whole numbers of the same order.
-__device__ __forceinline__ float kth_largest(float x, int k) {
+// A value that k of a wave's 64 values reach: the k-th largest but for its last 16 bits, found bit by bit
+// on whole numbers of the same order.
+__device__ __forceinline__ float about_kth(float x, int k) {
     const uint32_t b = __float_as_uint(x);
     const uint32_t key = b & 0x80000000u ? ~b : b | 0x80000000u;
     uint32_t lo = 0;
-    for (int bit = 31; bit >= 0; --bit) {
+    for (int bit = 31; bit >= 16; --bit) {
         const uint32_t t = lo | 1u << bit;
         if (__popcll(__ballot(key >= t)) >= k) lo = t;
     }
     return __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
 }
 
-// Longer rows: W waves a row, one pass. A wave takes tiles of 64 lanes x U 16-byte vectors (any
-// alignment), W tiles apart, the next tile loaded ahead. Alternatives: each wave keeps its own list
+// Longer rows: W waves a row, one pass. A wave takes tiles of 64 lanes x 2 16-byte vectors (any
+// alignment), W tiles apart, the next tile loaded ahead: 5.3 TB/s of 4096 x 32768 bf16 logits (4 vectors:
+// 4.5, for the waves that a CU no longer holds). Alternatives: each wave keeps its own list
 // and a lower bound of the row's k-th value, shared between the row's waves through LDS; a tile is
 // searched only where a vector's maximum reaches the bound.
 template <typename T, int W, bool TOP>
 __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
-    constexpr int VE = 16 / sizeof(T), U = 4, TILE = 64 * VE * U;
+    constexpr int VE = 16 / sizeof(T), U = 2, TILE = 64 * VE * U;
     __shared__ float bound_s[4];
     __shared__ Sums sums_s[4];
     __shared__ float lv_s[4][kMaxTop];
@@ -226,37 +249,47 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
         }
     };
     if (!padded) {
-        T cur[U][VE], nxt[U][VE];
-        int at = v0 + w * TILE;
-        if (at < v1) load(cur, at);
-        for (; at < v1; at += W * TILE) {
-            const bool more = at + W * TILE < v1;
-            if (more) load(nxt, at + W * TILE);
+        float mc = 0.0f;  // of sum.m; the loop's sums are about it
+        auto tile = [&](const T(&cur)[U][VE], int at) {
             float x[U][VE], um[U], tm = neg_inf();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 um[u] = neg_inf();
 #pragma unroll
-                for (int e = 0; e < VE; ++e) {
-                    x[u][e] = to_f32(cur[u][e]);
-                    um[u] = fmaxf(um[u], x[u][e]);
+                for (int e = 0; e < VE; e += 2) {
+                    x[u][e] = to_f32(cur[u][e]), x[u][e + 1] = to_f32(cur[u][e + 1]);
+                    um[u] = max3(um[u], x[u][e], x[u][e + 1]);
                 }
-                tm = fmaxf(tm, um[u]);
             }
+            tm = max3(tm, um[0], um[1]);
             {
                 const float m = fmaxf(sum.m, tm), base = base_of(m);
-                const float y0 = (sum.m - base) * a.c, e0 = __builtin_amdgcn_exp2f(y0);
-                sum.w = e0 * (sum.w + fmaxf(y0, -200.0f) * sum.s);
+                const Shift sh(base, a.c);
+                // the sums so far move to the new maximum (far: mc is infinite on both sides)
+                const float y0 = sum.m == neg_inf() ? neg_inf() : sh.far ? (sum.m - base) * a.c : mc - sh.mc;
+                const float e0 = __builtin_amdgcn_exp2f(y0);
+                sum.w = e0 * __builtin_fmaf(fmaxf(y0, -200.0f), sum.s, sum.w);
                 sum.s *= e0;
-                sum.m = m;
+                sum.m = m, mc = sh.mc;
+                if (!__any(sh.far)) {
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                    for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        const float y = (x[u][e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
-                        sum.s += p;
-                        sum.w += p * fmaxf(y, -200.0f);
-                    }
+                        for (int e = 0; e < VE; ++e) {
+                            const float y = __builtin_fmaf(x[u][e], a.c, -mc), p = __builtin_amdgcn_exp2f(y);
+                            sum.s += p;
+                            sum.w = __builtin_fmaf(p, fmaxf(y, -200.0f), sum.w);
+                        }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) {
+                            const float y = __builtin_fmaf(x[u][e] - base, a.c, sh.off), p = __builtin_amdgcn_exp2f(y);
+                            sum.s += p;
+                            sum.w = __builtin_fmaf(p, fmaxf(y, -200.0f), sum.w);
+                        }
+                }
             }
             if (TOP) {
                 float lv = list.worst_v(a.k);
@@ -264,32 +297,47 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
                 float lim = fmaxf(lv, *bound);
                 const int n = __popcll(__ballot(tm >= lim));
                 if (n > 0) {
-                    // many lanes: at least k values reach the k-th largest of the lanes' maxima
-                    if (n > a.k) lim = fmaxf(lim, kth_largest(tm, a.k));
+                    // many lanes: at least k values reach what k of the lanes' maxima reach
+                    if (n > a.k) lim = fmaxf(lim, about_kth(tm, a.k));
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         if (!__any(um[u] >= lim)) continue;
 #pragma unroll
                         for (int e = 0; e < VE; ++e) {
-                            const int id = at + (u * 64 + lane) * VE + e;
-                            uint64_t pick = __ballot(x[u][e] >= lim && id < v1 && ahead(x[u][e], id, lv, li));
+                            uint64_t pick = __ballot(x[u][e] >= lim);
                             while (pick) {
                                 const int from = __builtin_ctzll(pick);
                                 pick &= pick - 1;
                                 const float nv = __uint_as_float(
                                     __builtin_amdgcn_readlane(__float_as_uint(x[u][e]), from));
-                                list.insert(nv, at + (u * 64 + from) * VE + e);
+                                const int ni = at + (u * 64 + from) * VE + e;
+                                if (ni >= v1 || !ahead(nv, ni, lv, li)) continue;
+                                list.insert(nv, ni);
+                                lv = list.worst_v(a.k), li = list.worst_i(a.k);
+                                lim = fmaxf(lim, lv);
                             }
-                            lv = list.worst_v(a.k), li = list.worst_i(a.k);
                         }
                     }
                     if (W > 1 && lane == 0 && lv > *bound) *bound = lv;
                 }
             }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int e = 0; e < VE; ++e) cur[u][e] = nxt[u][e];
+        };
+        // two tiles in turn, the other one on its way
+        T ta[U][VE], tb[U][VE];
+        int at = v0 + w * TILE;
+        if (at < v1) load(ta, at);
+        for (; at < v1; at += 2 * W * TILE) {
+            const int next = at + W * TILE;
+            if (next < v1) load(tb, next);
+            tile(ta, at);
+            if (next >= v1) break;
+            if (next + W * TILE < v1) load(ta, next + W * TILE);
+            tile(tb, next);
+        }
+        {   // out of the sums what rounding m c put into every y
+            const float off = Shift(base_of(sum.m), a.c).off, e0 = __builtin_amdgcn_exp2f(-off);
+            sum.w = e0 * __builtin_fmaf(-off, sum.s, sum.w);
+            sum.s *= e0;
         }
         sum = join_lanes<64>(sum, a.c);
     }
@@ -374,7 +422,8 @@ struct GradArgs {
     const float *stats, *d_logp, *d_entropy;
 };
 
-// d logit = (g (1[token] - p) - h p (log p + entropy)) / temperature; L lanes a row, 16 bytes each.
+// d logit = (g (1[token] - p) - h p (log p + entropy)) / temperature; L lanes a row, 16 bytes each. With
+// y = log2 p: -p (A + B y) of the row's A = g + h entropy and B = h ln 2, and g more at the token.
 template <typename T>
 __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     constexpr int VE = 16 / sizeof(T);
@@ -384,37 +433,56 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     const bool padded = tok < 0;
     const T *l = (const T *)a.logits + row * a.stride;
     T *d = (T *)a.d_logits + row * a.d_stride;
-    const float m = a.stats[3 * row], l2 = a.stats[3 * row + 1], ent = a.stats[3 * row + 2];
-    float g = a.d_logp ? a.d_logp[row] * a.inv_t : 0.0f;
-    const float h = a.d_entropy ? a.d_entropy[row] * a.inv_t : 0.0f;
-    if (l2 == __builtin_inff()) g = 0.0f;  // nothing but -inf
-    if (tok >= a.vocab) g = __builtin_nanf("");
+    // all of the block's logits on their way before the row's numbers are waited for
+    constexpr int U = 4;
     const int v0 = blockIdx.y * a.span, v1 = min(a.vocab, v0 + a.span);
-    for (int i = v0 + threadIdx.x % L * VE; i < v1; i += L * VE) {
-        const bool full = i + VE <= v1;
-        T x[VE] = {}, r[VE];
+    for (int i0 = v0 + threadIdx.x % L * VE; i0 < v1; i0 += U * L * VE) {
+        T x[U][VE] = {};
         if (!padded) {
-            if (full) {
-                __builtin_memcpy(x, l + i, 16);
-            } else {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) x[e] = i + e < v1 ? l[i + e] : (T)neg_inf();
+            for (int u = 0; u < U; ++u) {
+                const int i = i0 + u * L * VE;
+                if (i + VE <= v1) {
+                    __builtin_memcpy(x[u], l + i, 16);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) x[u][e] = i + e < v1 ? l[i + e] : (T)neg_inf();
+                }
             }
         }
+        const float m = a.stats[3 * row];
+        float g = a.d_logp ? a.d_logp[row] * a.inv_t : 0.0f;
+        const float h = a.d_entropy ? a.d_entropy[row] * a.inv_t : 0.0f;
+        const Shift sh(m, a.c);
+        const float l2 = a.stats[3 * row + 1] + sh.off;
+        if (l2 == __builtin_inff()) g = 0.0f;  // nothing but -inf
+        if (tok >= a.vocab) g = __builtin_nanf("");
+        const float A = __builtin_fmaf(h, a.stats[3 * row + 2], g), B = h * kLn2;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-            const float y = (to_f32(x[e]) - m) * a.c - l2, p = __builtin_amdgcn_exp2f(y);
-            const float lp = kLn2 * fmaxf(y, -200.0f);
-            float v = -p * (g + h * (lp + ent));
-            if (i + e == tok) v += g;
-            r[e] = (T)(padded ? 0.0f : v);
-        }
-        if (full) {
-            __builtin_memcpy(d + i, r, 16);
-        } else {
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * L * VE;
+            if (i >= v1) break;
+            float v[VE];
 #pragma unroll
-            for (int e = 0; e < VE; ++e)
-                if (i + e < v1) d[i + e] = r[e];
+            for (int e = 0; e < VE; ++e) {
+                const float xe = to_f32(x[u][e]);
+                const float y = (sh.far ? __builtin_fmaf(xe - m, a.c, sh.off) : __builtin_fmaf(xe, a.c, -sh.mc)) - l2;
+                v[e] = -__builtin_amdgcn_exp2f(y) * __builtin_fmaf(B, fmaxf(y, -200.0f), A);
+            }
+            if (tok - i >= 0 && tok - i < VE) {
+#pragma unroll
+                for (int e = 0; e < VE; ++e) v[e] += tok - i == e ? g : 0.0f;
+            }
+            T r[VE];
+#pragma unroll
+            for (int e = 0; e < VE; ++e) r[e] = (T)(padded ? 0.0f : v[e]);
+            if (i + VE <= v1) {
+                __builtin_memcpy(d + i, r, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VE; ++e)
+                    if (i + e < v1) d[i + e] = r[e];
+            }
         }
     }
 }
@@ -428,7 +496,7 @@ constexpr int kSmallVocab = 512;
 int slices_of(int64_t rows, int64_t vocab, int dtype, int *len) {
     *len = (int)vocab;
     if (rows >= 512 || vocab <= kSmallVocab) return 1;
-    const int64_t tile = 4 * (dtype == RLP_F32 ? 1024 : 2048);  // four waves' tiles
+    const int64_t tile = 4 * (dtype == RLP_F32 ? 512 : 1024);  // four waves' tiles
     int64_t want = (1024 + rows - 1) / rows;
     const int64_t most = (vocab + tile - 1) / tile;
     if (want > most) want = most;
@@ -472,7 +540,7 @@ void launch_grad(GradArgs a, hipStream_t s) {
 int check_rows(const char *who, int dtype, int64_t rows, int64_t vocab, int64_t stride, float temperature) {
     RLP_REQUIRE(dtype == RLP_F32 || dtype == RLP_F16 || dtype == RLP_BF16, "%s: dtype %d", who, dtype);
     RLP_REQUIRE(rows >= 0 && rows <= 0x7FFFFFFFLL, "%s: %lld rows", who, (long long)rows);
-    RLP_REQUIRE(vocab >= 1 && vocab < 0x7FFF0000LL, "%s: vocab %lld", who, (long long)vocab);
+    RLP_REQUIRE(vocab >= 1 && vocab <= 0x7FF00000LL, "%s: vocab %lld", who, (long long)vocab);
     RLP_REQUIRE(stride >= 0, "%s: row stride %lld", who, (long long)stride);
     RLP_REQUIRE(temperature > 0.0f && temperature <= 3.402823466e38f, "%s: temperature %g (a positive number)",
                 who, temperature);
