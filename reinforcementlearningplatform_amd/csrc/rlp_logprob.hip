@@ -13,6 +13,8 @@
 namespace rlp {
 namespace {
 
+typedef uint32_t uintx4_any __attribute__((ext_vector_type(4), aligned(2)));  // at any element's address
+
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaxTop = 32;
 constexpr int kNoIndex = 0x7FFFFFFF;
@@ -84,6 +86,18 @@ __device__ __forceinline__ Sums join_lanes(Sums v, float c) {
     return v;
 }
 
+// A value and its token as one whole number: larger for larger values, for equal ones (0 and -0 too)
+// larger for the lower token.
+__device__ __forceinline__ uint64_t rank_key(float v, int token) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+    const uint32_t k = (uint32_t)(key >> 32);
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+__device__ __forceinline__ int key_token(uint64_t key) { return (int)~(uint32_t)key; }
+
 // Row results from its sums (one lane). lt: the token's logit.
 __device__ __forceinline__ float log2_sum(const Sums &v) {
     return v.s == 0.0f ? __builtin_inff() : __builtin_amdgcn_logf(v.s);
@@ -111,10 +125,9 @@ __device__ __forceinline__ void write_padded(const ScoreArgs &a, int64_t row) {
         a.top_tokens[row * a.k + i] = -1;
     }
 }
-__device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t row, int i, const Sums &v, float val, int id) {
-    const bool none = id == kNoIndex;
-    a.top_logp[row * a.k + i] = none ? __builtin_nanf("") : logp_of(v, val, a.inv_t);
-    a.top_tokens[row * a.k + i] = none ? -1 : id;
+__device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t row, int i, const Sums &v, uint64_t key) {
+    a.top_logp[row * a.k + i] = key ? logp_of(v, key_value(key), a.inv_t) : __builtin_nanf("");
+    a.top_tokens[row * a.k + i] = key ? key_token(key) : -1;
 }
 
 __device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
@@ -170,27 +183,45 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
             if (ahead(ov, oi, bv, bi)) bv = ov, bi = oi;
         }
         if (bi != kNoIndex && bi % G == g) open &= ~(1u << (bi / G));
-        if (g == 0) write_top(a, row, i, v, bv, bi);
+        if (g == 0) write_top(a, row, i, v, bi == kNoIndex ? 0 : rank_key(bv, bi));
     }
 }
 
-// The k best (value, token) of what a wave has seen, descending over its lanes; ties to the lower
-// token. Lanes behind the last entry hold (-inf, none).
-struct TopList {
-    float v;
-    int i;
-    __device__ void clear() { v = neg_inf(), i = kNoIndex; }
-    __device__ void insert(float nv, int ni) {  // nv, ni: the same in all lanes
-        const int lane = threadIdx.x & 63;
-        const int at = __popcll(__ballot(ahead(v, i, nv, ni)));
-        // the entries behind move up one lane (DPP wave_shr:1)
-        const float uv = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x138, 0xF, 0xF, false));
-        const int ui = __builtin_amdgcn_update_dpp(0, i, 0x138, 0xF, 0xF, false);
-        v = lane < at ? v : lane == at ? nv : uv;
-        i = lane < at ? i : lane == at ? ni : ui;
+// A wave's candidates for the k best, in LDS. push takes a lane's candidate where `pick`; select keeps
+// the k best in order. Every key counts the keys above it, which places it at once: no chain from one
+// candidate to the next, as inserting them one by one has (26 us of such chains for 8 rows' 20 best).
+struct TopBuf {
+    static constexpr int kCap = 128;
+    uint64_t *key;
+    int n, k;
+    __device__ __forceinline__ void push(bool pick, uint64_t v) {
+        const uint64_t mask = __ballot(pick);
+        if (!mask) return;
+        if (n > kCap - 64) select();
+        if (pick) key[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0))] = v;
+        n += __popcll(mask);
     }
-    __device__ float worst_v(int k) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), k - 1)); }
-    __device__ int worst_i(int k) const { return __builtin_amdgcn_readlane(i, k - 1); }
+    __device__ __forceinline__ void select() {
+        const int lane = threadIdx.x & 63;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // lanes read what other lanes wrote
+        const uint64_t a = lane < n ? key[lane] : 0, b = lane + 64 < n ? key[lane + 64] : 0;
+        int ra = 0, rb = 0;
+        if (n <= 64) {
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) ra += key[i] > a;
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                const uint64_t o = key[i];
+                ra += o > a, rb += o > b;
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (lane < n && ra < k) key[ra] = a;
+        if (lane + 64 < n && rb < k) key[rb] = b;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        n = min(n, k);
+    }
 };
 
 // A value that k of a wave's 64 values reach: the k-th largest but for its last 16 bits, found bit by bit
@@ -216,8 +247,8 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
     constexpr int VE = 16 / sizeof(T), U = 2, TILE = 64 * VE * U;
     __shared__ float bound_s[4];
     __shared__ Sums sums_s[4];
-    __shared__ float lv_s[4][kMaxTop];
-    __shared__ int li_s[4][kMaxTop];
+    __shared__ int count_s[4];
+    __shared__ uint64_t top_s[TOP ? 4 : 1][TopBuf::kCap];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % W;
     const int64_t row = (int64_t)blockIdx.x * (4 / W) + wave / W;
     const int slice = blockIdx.y;
@@ -232,8 +263,9 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
     float lt = 0.0f;
     if (!padded && tok < a.vocab) lt = to_f32(l[tok]);
     Sums sum = {neg_inf(), 0.0f, 0.0f};
-    TopList list;
-    list.clear();
+    TopBuf top = {top_s[TOP ? wave : 0], 0, a.k};
+    float lv = neg_inf();  // an alternative is above (lv, li), which at least k logits of the row are not below
+    int li = v1;
     volatile float *bound = &bound_s[wave / W * W];
 
     auto load = [&](T(&t)[U][VE], int at) {
@@ -292,33 +324,31 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
                 }
             }
             if (TOP) {
-                float lv = list.worst_v(a.k);
-                int li = list.worst_i(a.k);
-                float lim = fmaxf(lv, *bound);
-                const int n = __popcll(__ballot(tm >= lim));
-                if (n > 0) {
+                const float others = *bound;
+                if (others > lv) lv = others, li = v1;
+                const int many = __popcll(__ballot(tm >= lv));
+                if (many > 0) {
                     // many lanes: at least k values reach what k of the lanes' maxima reach
-                    if (n > a.k) lim = fmaxf(lim, about_kth(tm, a.k));
+                    if (many > a.k) {
+                        const float reach = about_kth(tm, a.k);
+                        if (reach > lv) lv = reach, li = v1;
+                    }
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
-                        if (!__any(um[u] >= lim)) continue;
+                        if (!__any(um[u] >= lv)) continue;
 #pragma unroll
                         for (int e = 0; e < VE; ++e) {
-                            uint64_t pick = __ballot(x[u][e] >= lim);
-                            while (pick) {
-                                const int from = __builtin_ctzll(pick);
-                                pick &= pick - 1;
-                                const float nv = __uint_as_float(
-                                    __builtin_amdgcn_readlane(__float_as_uint(x[u][e]), from));
-                                const int ni = at + (u * 64 + from) * VE + e;
-                                if (ni >= v1 || !ahead(nv, ni, lv, li)) continue;
-                                list.insert(nv, ni);
-                                lv = list.worst_v(a.k), li = list.worst_i(a.k);
-                                lim = fmaxf(lim, lv);
-                            }
+                            if (!__any(x[u][e] >= lv)) continue;
+                            const int id = at + (u * 64 + lane) * VE + e;
+                            top.push(x[u][e] > lv || (x[u][e] == lv && id < li), rank_key(x[u][e], id));
                         }
                     }
-                    if (W > 1 && lane == 0 && lv > *bound) *bound = lv;
+                    if (top.n >= a.k + 8) {
+                        top.select();
+                        const uint64_t last = top.key[a.k - 1];
+                        lv = key_value(last), li = key_token(last);
+                        if (W > 1 && lane == 0 && lv > *bound) *bound = lv;
+                    }
                 }
             }
         };
@@ -340,32 +370,30 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
             sum.s *= e0;
         }
         sum = join_lanes<64>(sum, a.c);
+        if (TOP) top.select();
     }
     if (W > 1) {
         if (lane == 0) sums_s[wave] = sum;
-        if (TOP && lane < a.k) lv_s[wave][lane] = list.v, li_s[wave][lane] = list.i;
+        if (TOP && lane == 0) count_s[wave] = top.n;
         __syncthreads();
         if (w != 0) return;
         for (int o = 1; o < W; ++o) {
             sum = join(sum, sums_s[wave + o], a.c);
             if (!TOP) continue;
-            const float ov = lane < a.k ? lv_s[wave + o][lane] : neg_inf();
-            const int oi = lane < a.k ? li_s[wave + o][lane] : kNoIndex;
-            for (int i = 0; i < a.k; ++i) {
-                const float nv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ov), i));
-                const int ni = __builtin_amdgcn_readlane(oi, i);
-                if (!ahead(nv, ni, list.worst_v(a.k), list.worst_i(a.k))) break;
-                list.insert(nv, ni);
-            }
+            const int n = count_s[wave + o];
+            const uint64_t v = lane < n ? top_s[TOP ? wave + o : 0][lane] : 0;
+            top.push(lane < n, v);
         }
+        if (TOP) top.select();
     }
     if (row >= a.rows) return;
     if (a.slices > 1) {
         float *part = a.parts + (row * a.slices + slice) * (3 + 2 * a.k);
         if (lane == 0) part[0] = sum.m, part[1] = sum.s, part[2] = sum.w;
-        if (TOP && lane < a.k) {
-            part[3 + 2 * lane] = list.v;
-            part[4 + 2 * lane] = __int_as_float(list.i);
+        if (TOP && lane < a.k) {  // 0: no further alternative
+            const uint64_t v = lane < top.n ? top.key[lane] : 0;
+            part[3 + 2 * lane] = __uint_as_float((uint32_t)v);
+            part[4 + 2 * lane] = __uint_as_float((uint32_t)(v >> 32));
         }
         return;
     }
@@ -374,12 +402,13 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
         return;
     }
     if (lane == 0) write_row(a, row, tok, lt, sum);
-    if (TOP && lane < a.k) write_top(a, row, lane, sum, list.v, list.i);
+    if (TOP && lane < a.k) write_top(a, row, lane, sum, lane < top.n ? top.key[lane] : 0);
 }
 
 // Joins the slices (at most 64) of a row: one wave a row, one slice a lane.
 template <typename T>
 __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
+    __shared__ uint64_t top_s[4][TopBuf::kCap];
     const int lane = threadIdx.x & 63;
     const int64_t row = blockIdx.x * 4LL + (threadIdx.x >> 6);
     if (row >= a.rows) return;
@@ -395,21 +424,20 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
     sum = join_lanes<64>(sum, a.c);
     if (lane == 0) write_row(a, row, tok, lt, sum);
     if (a.k == 0) return;
-    TopList list;
-    list.clear();
+    TopBuf top = {top_s[threadIdx.x >> 6], 0, a.k};
+    uint64_t last = 0;
     for (int i = 0; i < a.k; ++i) {  // every slice's i-th entry
-        const float v = on ? part[3 + 2 * i] : neg_inf();
-        const int id = on ? __float_as_int(part[4 + 2 * i]) : kNoIndex;
-        uint64_t pick = __ballot(ahead(v, id, list.worst_v(a.k), list.worst_i(a.k)));
-        if (!pick) break;  // the slices' further entries are no better
-        while (pick) {
-            const int from = __builtin_ctzll(pick);
-            pick &= pick - 1;
-            list.insert(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), from)),
-                        __builtin_amdgcn_readlane(id, from));
+        const uint64_t v = on ? (uint64_t)__float_as_uint(part[4 + 2 * i]) << 32 | __float_as_uint(part[3 + 2 * i]) : 0;
+        const bool pick = v > last;
+        if (!__any(pick)) break;  // the slices' further entries are no better
+        top.push(pick, v);
+        if (top.n >= a.k + 8) {
+            top.select();
+            last = top.key[a.k - 1];
         }
     }
-    if (lane < a.k) write_top(a, row, lane, sum, list.v, list.i);
+    top.select();
+    if (lane < a.k) write_top(a, row, lane, sum, lane < top.n ? top.key[lane] : 0);
 }
 
 struct GradArgs {
@@ -424,7 +452,7 @@ struct GradArgs {
 
 // d logit = (g (1[token] - p) - h p (log p + entropy)) / temperature; L lanes a row, 16 bytes each. With
 // y = log2 p: -p (A + B y) of the row's A = g + h entropy and B = h ln 2, and g more at the token.
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     constexpr int VE = 16 / sizeof(T);
     const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -477,7 +505,10 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
 #pragma unroll
             for (int e = 0; e < VE; ++e) r[e] = (T)(padded ? 0.0f : v[e]);
             if (i + VE <= v1) {
-                __builtin_memcpy(d + i, r, 16);
+                uintx4_any out;
+                __builtin_memcpy(&out, r, 16);
+                if (STREAM) __builtin_nontemporal_store(out, (uintx4_any *)(d + i));
+                else *(uintx4_any *)(d + i) = out;
             } else {
 #pragma unroll
                 for (int e = 0; e < VE; ++e)
@@ -513,7 +544,10 @@ void launch_score(const ScoreArgs &a, hipStream_t s) {
     if (a.vocab <= 32) score_small_kernel<T, 4, 8><<<blocks(64), 256, 0, s>>>(a);
     else if (a.vocab <= 128) score_small_kernel<T, 16, 8><<<blocks(16), 256, 0, s>>>(a);
     else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64, 8><<<blocks(4), 256, 0, s>>>(a);
-    else if (a.slices == 1 && a.vocab <= 8192) {
+    else if (a.slices == 1 && (a.vocab <= 8192 || (a.k > 0 && a.rows >= 2048))) {
+        // a wave a row: short rows, and rows enough to fill the card where a search for alternatives begins
+        // and ends in every wave (4096 x 131071, 8 alternatives: 284 us, four waves a row 308 us; without
+        // alternatives 4096 x 32768 takes 56 us so and 50 us with four)
         if (a.k) score_rows_kernel<T, 1, true><<<blocks(4), 256, 0, s>>>(a);
         else score_rows_kernel<T, 1, false><<<blocks(4), 256, 0, s>>>(a);
     } else {
@@ -534,7 +568,11 @@ void launch_grad(GradArgs a, hipStream_t s) {
     a.span = 256 * VE * 4;
     int64_t ny = ((int64_t)a.vocab + a.span - 1) / a.span;
     while (ny > 65535) a.span *= 2, ny = ((int64_t)a.vocab + a.span - 1) / a.span;
-    score_grad_kernel<T><<<dim3((unsigned)blocks, (unsigned)ny), 256, 0, s>>>(a, L);
+    // logits and gradient beyond the 256 MB last-level cache: stores past it (4096 x 32768 bf16 102 us for
+    // 153), else the gradient stays there for what reads it next
+    const dim3 grid((unsigned)blocks, (unsigned)ny);
+    if (a.rows * a.vocab * (int64_t)sizeof(T) > (128LL << 20)) score_grad_kernel<T, true><<<grid, 256, 0, s>>>(a, L);
+    else score_grad_kernel<T, false><<<grid, 256, 0, s>>>(a, L);
 }
 
 int check_rows(const char *who, int dtype, int64_t rows, int64_t vocab, int64_t stride, float temperature) {

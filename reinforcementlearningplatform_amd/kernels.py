@@ -520,12 +520,15 @@ _device_index = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _launch(what, tensors, fn, *args):
-    """fn(*args, stream) on the tensors' device, with its current stream."""
+def _one_device(what, *tensors):
     dev = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev or dev < 0:
             raise RLPError(f"{what}: not on the GPU, or on several (librlp takes tensors of one device)")
+
+
+def _launch(what, dev, fn, *args):
+    """fn(*args, stream) on device dev, with its current stream."""
     if dev == _device_index():
         rc = fn(*args, _stream_of(dev))
     else:
@@ -601,6 +604,7 @@ def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=N
     need = _la_workspace_bytes(what, 0, *dims)
     _, B, T, H, _, _, _, Dk, Dv = dims
     reset, lengths = _la_flags(what, reset, lengths, (B, T), B)
+    _one_device(what, q, k, v, log_decay, state, reset, lengths)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     state = state.contiguous() if state is not None else None
     out = _like_order(q, B, T, H, Dv)
@@ -609,7 +613,7 @@ def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=N
     cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale, *q.stride()[:3],
                                 *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *(0,) * 9,
                                 *(reset.stride() if reset is not None else (0, 0)))
-    _launch(what, (q, k, v, log_decay, state, reset, lengths), lib().rlp_linear_attention, cfg,
+    _launch(what, q.get_device(), lib().rlp_linear_attention, cfg,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _at(reset), _at(lengths),
             _at(state), out.data_ptr(), _at(last), _at(ws), need)
     return out, last
@@ -628,6 +632,7 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
         raise RLPError(f"{what}: d_out {d_out.dtype} {tuple(d_out.shape)}")
     if d_state is not None and (d_state.dtype != torch.float32 or d_state.shape != (B, H, Dk, Dv)):
         raise RLPError(f"{what}: d_state {d_state.dtype} {tuple(d_state.shape)}")
+    _one_device(what, q, k, v, log_decay, state, reset, lengths, d_out, d_state)
     q, k, v, d_out, log_decay = _rows(q), _rows(k), _rows(v), _rows(d_out), log_decay.contiguous()
     first = torch.empty_like(state, memory_format=torch.contiguous_format) if state is not None else None
     state = state.contiguous() if state is not None else None
@@ -638,8 +643,7 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
                                 *k.stride()[:3], *v.stride()[:3], *d_out.stride()[:3], *dq.stride()[:3],
                                 *dk.stride()[:3], *dv.stride()[:3],
                                 *(reset.stride() if reset is not None else (0, 0)))
-    _launch(what, (q, k, v, log_decay, state, reset, lengths, d_out, d_state),
-            lib().rlp_linear_attention_backward, cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    _launch(what, q.get_device(), lib().rlp_linear_attention_backward, cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(),
             log_decay.data_ptr(), _at(reset), _at(lengths), _at(state), d_out.data_ptr(), _at(d_state),
             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(first), _at(ws), need)
     return dq, dk, dv, first
@@ -725,12 +729,13 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, sta
         out = q.new_empty((B, H, Dv))
     elif out.shape != (B, H, Dv) or out.dtype != q.dtype or not out.is_contiguous():
         raise RLPError(f"{what}: out {out.dtype} {tuple(out.shape)}, contiguous {q.dtype} {(B, H, Dv)} needed")
+    _one_device(what, q, k, v, log_decay, state, state_out, reset, out)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale,
                                 q.stride(0), 0, q.stride(1), k.stride(0), 0, k.stride(1),
                                 v.stride(0), 0, v.stride(1), H * Dv, 0, Dv, *(0,) * 9,
                                 reset.stride(0) if reset is not None else 0, 0)
-    _launch(what, (q, k, v, log_decay, state, state_out, reset, out), lib().rlp_linear_attention_step, cfg,
+    _launch(what, q.get_device(), lib().rlp_linear_attention_step, cfg,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _at(reset), state.data_ptr(),
             state_out.data_ptr(), out.data_ptr())
     return out
@@ -744,18 +749,10 @@ def _lp_workspace_bytes(what, rows, vocab, top_k, dtype):
     return need
 
 
-def token_logprob_forward(logits, tokens, temperature=1.0, top_k=0, want_stats=True):
-    """rlp_token_logprob without autograd on logits [rows][vocab], tokens [rows] int64: (logp, entropy,
-    stats, top_logp, top_tokens); stats feeds token_logprob_backward, top_* are None for top_k 0."""
-    what = "token_logprob"
-    if logits.dim() != 2 or tokens.dim() != 1 or tokens.shape[0] != logits.shape[0] or \
-            tokens.dtype != torch.int64:
-        raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
-    dt = _DTYPES.get(logits.dtype)
-    if dt is None:
-        raise RLPError(f"{what}: dtype {logits.dtype} (float32, float16 or bfloat16)")
+def _lp_forward(logits, tokens, temperature, top_k, want_stats):
     rows, vocab = logits.shape
-    need = _lp_workspace_bytes(what, rows, vocab, top_k, dt)
+    dt = _DTYPES[logits.dtype]
+    need = _lp_workspace_bytes("token_logprob", rows, vocab, top_k, dt)
     logits, tokens = _rows(logits), tokens.contiguous()
     logp = logits.new_empty(rows, dtype=torch.float32)
     entropy = torch.empty_like(logp)
@@ -763,39 +760,57 @@ def token_logprob_forward(logits, tokens, temperature=1.0, top_k=0, want_stats=T
     top_logp = logp.new_empty((rows, top_k)) if top_k else None
     top_tokens = tokens.new_empty((rows, top_k)) if top_k else None
     ws = logp.new_empty(need, dtype=torch.uint8) if need > 0 else None
-    _launch(what, (logits, tokens), lib().rlp_token_logprob, logits.data_ptr(), dt, rows, vocab,
+    _launch("token_logprob", logits.get_device(), lib().rlp_token_logprob, logits.data_ptr(), dt, rows, vocab,
             logits.stride(0), tokens.data_ptr(), temperature, top_k, logp.data_ptr(), entropy.data_ptr(),
             _at(stats), _at(top_logp), _at(top_tokens), _at(ws), need)
     return logp, entropy, stats, top_logp, top_tokens
 
 
+def token_logprob_forward(logits, tokens, temperature=1.0, top_k=0, want_stats=True):
+    """rlp_token_logprob without autograd on logits [rows][vocab], tokens [rows] int64: (logp, entropy,
+    stats, top_logp, top_tokens); stats feeds token_logprob_backward, top_* are None for top_k 0."""
+    what = "token_logprob"
+    if logits.dim() != 2 or tokens.dim() != 1 or tokens.shape[0] != logits.shape[0] or \
+            tokens.dtype != torch.int64:
+        raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
+    if logits.dtype not in _DTYPES:
+        raise RLPError(f"{what}: dtype {logits.dtype} (float32, float16 or bfloat16)")
+    _one_device(what, logits, tokens)
+    return _lp_forward(logits, tokens, float(temperature), int(top_k), want_stats)
+
+
+def _lp_backward(d_logp, d_entropy, logits, tokens, stats, temperature):
+    rows, vocab = logits.shape
+    logits, tokens = _rows(logits), tokens.contiguous()
+    d_logp = d_logp.contiguous() if d_logp is not None else None
+    d_entropy = d_entropy.contiguous() if d_entropy is not None else None
+    d_logits = logits.new_empty((rows, vocab))
+    _launch("token_logprob_backward", logits.get_device(), lib().rlp_token_logprob_backward,
+            logits.data_ptr(), _DTYPES[logits.dtype], rows, vocab, logits.stride(0), tokens.data_ptr(),
+            temperature, stats.data_ptr(), _at(d_logp), _at(d_entropy), d_logits.data_ptr(), vocab)
+    return d_logits
+
+
 def token_logprob_backward(d_logp, d_entropy, logits, tokens, stats, temperature=1.0):
     """rlp_token_logprob_backward: the gradient of logits from those of logp and entropy (None: 0)."""
     what = "token_logprob_backward"
-    rows, vocab = logits.shape
+    if logits.dim() != 2 or logits.dtype not in _DTYPES:
+        raise RLPError(f"{what}: logits {logits.dtype} {tuple(logits.shape)}")
+    rows = logits.shape[0]
     for name, t in (("d_logp", d_logp), ("d_entropy", d_entropy)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (rows,)):
             raise RLPError(f"{what}: {name} {t.dtype} {tuple(t.shape)}, float32 ({rows},) needed")
     if stats.shape != (rows, 3) or stats.dtype != torch.float32 or tokens.dtype != torch.int64 or \
             tokens.shape != (rows,):
         raise RLPError(f"{what}: stats {tuple(stats.shape)}, tokens {tokens.dtype} {tuple(tokens.shape)}")
-    dt = _DTYPES.get(logits.dtype)
-    if dt is None:
-        raise RLPError(f"{what}: dtype {logits.dtype} (float32, float16 or bfloat16)")
-    logits, tokens, stats = _rows(logits), tokens.contiguous(), stats.contiguous()
-    d_logp = d_logp.contiguous() if d_logp is not None else None
-    d_entropy = d_entropy.contiguous() if d_entropy is not None else None
-    d_logits = logits.new_empty((rows, vocab))
-    _launch(what, (logits, tokens, stats, d_logp, d_entropy), lib().rlp_token_logprob_backward,
-            logits.data_ptr(), dt, rows, vocab, logits.stride(0), tokens.data_ptr(), temperature,
-            stats.data_ptr(), _at(d_logp), _at(d_entropy), d_logits.data_ptr(), vocab)
-    return d_logits
+    _one_device(what, logits, tokens, stats, d_logp, d_entropy)
+    return _lp_backward(d_logp, d_entropy, logits, tokens, stats.contiguous(), float(temperature))
 
 
 class _TokenLogprob(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature, top_k):
-        logp, entropy, stats, top_logp, top_tokens = token_logprob_forward(logits, tokens, temperature, top_k)
+        logp, entropy, stats, top_logp, top_tokens = _lp_forward(logits, tokens, temperature, top_k, True)
         ctx.save_for_backward(logits, tokens, stats)
         ctx.temperature = temperature
         ctx.set_materialize_grads(False)
@@ -810,7 +825,7 @@ class _TokenLogprob(torch.autograd.Function):
         if d_logp is None and d_entropy is None:
             return None, None, None, None
         logits, tokens, stats = ctx.saved_tensors
-        return token_logprob_backward(d_logp, d_entropy, logits, tokens, stats, ctx.temperature), None, None, None
+        return _lp_backward(d_logp, d_entropy, logits, tokens, stats, ctx.temperature), None, None, None
 
 
 def token_logprob(logits, tokens, temperature=1.0, top_k=0):
@@ -834,12 +849,15 @@ def token_logprob(logits, tokens, temperature=1.0, top_k=0):
     vocab = logits.shape[-1]
     if vocab < 1:
         raise RLPError(f"{what}: no logits in a row")
+    if logits.dtype not in _DTYPES:
+        raise RLPError(f"{what}: dtype {logits.dtype} (float32, float16 or bfloat16)")
+    _one_device(what, logits, tokens)
     flat = len(shape) == 1
     if not flat:
         logits, tokens = logits.reshape(-1, vocab), tokens.reshape(-1)
     if logits.requires_grad and torch.is_grad_enabled():
         res = _TokenLogprob.apply(logits, tokens, temperature, top_k)
     else:
-        logp, entropy, _, top_logp, top_tokens = token_logprob_forward(logits, tokens, temperature, top_k, False)
+        logp, entropy, _, top_logp, top_tokens = _lp_forward(logits, tokens, temperature, top_k, False)
         res = (logp, entropy, top_logp, top_tokens) if top_k else (logp, entropy)
     return res if flat else tuple(r.view(shape if r.dim() == 1 else shape + (top_k,)) for r in res)
