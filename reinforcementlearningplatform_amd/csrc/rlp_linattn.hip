@@ -474,7 +474,8 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 // la_walk_kernel for bf16 operands on v_mfma_f32_16x16x32_bf16, 64 tokens a chunk. Products of the
 // operands are exact in f32; what is not an operand is split into bf16 pieces where it meets the
 // matrix cores: P and S for the output into two (2^-16, below the output's own rounding), the
-// weighted z of the state's sum into three (2^-24), so that the state stays an f32 state.
+// weighted z of the state's sum into PZ: three (2^-24) where the state leaves the call, so that it is
+// an f32 state, and two where it is only ever used in two pieces itself.
 //
 // A 16x16 accumulator holds rows 4 q + r (q = lane >> 4) of column lane & 15, so the accumulators of two
 // row tiles are the operand of 32 rows in the order 4 q .. 4 q + 3, 16 + 4 q .. of the quarter waves. With
@@ -483,7 +484,7 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 //
 // 16 columns a wave, not 32: with 32x32 tiles at two waves a SIMD the same work waited on LDS and on
 // its own products (9 us a chunk of 128 x 128); half the registers a wave let four waves run.
-template <int DXB, int NW>
+template <int DXB, int NW, int PZ>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
     constexpr int C = 64, DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW, PAD = 16;
     __shared__ __align__(16) unsigned short xs[C][DX + PAD];
@@ -664,13 +665,13 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                 wz[4 * m] = lo_half(zv[js][2 * m]) * f[0], wz[4 * m + 1] = hi_half(zv[js][2 * m]) * f[1];
                 wz[4 * m + 2] = lo_half(zv[js][2 * m + 1]) * f[2], wz[4 * m + 3] = hi_half(zv[js][2 * m + 1]) * f[3];
             }
-            bf16x8 Zp[3];
+            bf16x8 Zp[PZ];
             split8(wz, Zp);
 #pragma unroll
             for (int at = 0; at < 2 * DXB; ++at) {
                 const bf16x8 Y = __builtin_bit_cast(bf16x8, column32<true>(ys, 32 * js, 16 * at, lane));
 #pragma unroll
-                for (int p = 0; p < 3; ++p) S[at] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Y, Zp[p], S[at], 0, 0, 0);
+                for (int p = 0; p < PZ; ++p) S[at] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Y, Zp[p], S[at], 0, 0, 0);
             }
         }
         if (want_out) {
@@ -891,9 +892,10 @@ void launch_walk(const WalkArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.B * a.H), a.nseg);
     auto go = [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
-        if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0)
-            la_walk_bf16_kernel<DXB, NW><<<grid, 64 * NW, 0, s>>>(a);
-        else
+        if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0) {
+            if (a.fin && a.mode != 2) la_walk_bf16_kernel<DXB, NW, 3><<<grid, 64 * NW, 0, s>>>(a);
+            else la_walk_bf16_kernel<DXB, NW, 2><<<grid, 64 * NW, 0, s>>>(a);
+        } else
             la_walk_kernel<T, DXB, NW><<<grid, 64 * NW, 0, s>>>(a);
     };
     if (a.dz <= 32) go(std::integral_constant<int, 2>{});
