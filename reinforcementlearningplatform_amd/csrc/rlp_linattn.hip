@@ -413,7 +413,7 @@ struct Rows16 {
     static constexpr int VR = D / 8, N = (64 * VR + NT - 1) / NT;
     uintx4 v[N];
     // d: a multiple of 8, so a vector is wholly inside the row or behind it
-    __device__ __forceinline__ void load(const __bf16 *src, int64_t st, int n, int d, int tid) {
+    __device__ __forceinline__ void load(const __bf16 *src, int64_t st, int n, int d, unsigned tid) {
         const int row = tid / VR, c = tid % VR * 8;
         const __bf16 *p = src + row * st + c;
         if (n == 64 && d == D && 64 * VR >= NT) {
@@ -430,10 +430,11 @@ struct Rows16 {
     // PERM: of 32 columns the four-column groups in the order 0 4 1 5 2 6 3 7, in which a quarter wave's
     // eight columns are 16 bytes and match two accumulators' rows (see the kernel).
     template <bool PERM, int P>
-    __device__ __forceinline__ void store(unsigned short (*dst)[P], int tid) const {
+    __device__ __forceinline__ void store(unsigned short (*dst)[P], unsigned tid) const {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int id = k * NT + tid, row = id / VR, c = id % VR * 8;
+            const unsigned id = k * NT + tid;
+            const int row = id / VR, c = id % VR * 8;
             if (64 * VR < NT && row >= 64) break;
             if (PERM) {
                 const int at = (c & ~31) + (c & 8) * 2 + (c & 16) / 4;
@@ -493,7 +494,8 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     __shared__ __align__(16) uintx2 ps[6][2][64][2];  // (token tile, 32 tokens), piece, lane, half
     __shared__ __align__(16) float into_s[C], from_s[C];
     __shared__ int bad_s, first_s;
-    int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
+    unsigned tid = threadIdx.x;
+    int lane = tid & 63, q = lane >> 4, l15 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -524,16 +526,18 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     }
     bool seg_cut = false;
     if (tid == 0) bad_s = -1;
-    for (int id = tid; id < 6 * 2 * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
+    for (unsigned id = tid; id < 6 * 2 * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
     Rows16<DX, NT> rx, ry;
     Rows16<DZ, NT> rz;
-    auto load = [&](int pos) {
-        const int n = min(C, p1 - pos);
-        if (want_out) rx.load(x + pos * dir * a.xt, dir * a.xt, n, a.dx, tid);
-        ry.load(y + pos * dir * a.yt, dir * a.yt, n, a.dx, tid);
-        rz.load(z + pos * dir * a.zt, dir * a.zt, n, a.dz, tid);
+    const int64_t xs_t = dir * a.xt, ys_t = dir * a.yt, zs_t = dir * a.zt;
+    x += p0 * xs_t, y += p0 * ys_t, z += p0 * zs_t;  // of the chunk to load next
+    auto load = [&](int n) {
+        if (want_out) rx.load(x, xs_t, n, a.dx, tid);
+        ry.load(y, ys_t, n, a.dx, tid);
+        rz.load(z, zs_t, n, a.dz, tid);
     };
-    if (p0 < p1) load(p0);
+    auto step = [&](int n) { x += n * xs_t, y += n * ys_t, z += n * zs_t; };
+    if (p0 < p1) load(min(C, p1 - p0));
     for (int pos = p0; pos < p1;) {
         tid = anew(tid), lane = tid & 63, q = lane >> 4, l15 = lane & 15, col = c0 + l15;
         int n = min(C, p1 - pos);
@@ -541,8 +545,9 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
         // tokens of the episodes that came in and that goes out
         auto factors = [&](uint64_t cuts) {
             if (tid < C) {
-                into_s[tid] = cuts & (~0ull >> (63 - tid)) ? 0.0f : a.s2 * decay_pow(lam2, tid + a.e0);
-                from_s[tid] = tid < n && tid >= begin_of64(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - tid) : 0.0f;
+                const int i = tid;
+                into_s[i] = cuts & (~0ull >> (63 - i)) ? 0.0f : a.s2 * decay_pow(lam2, i + a.e0);
+                from_s[i] = i < n && i >= begin_of64(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - i) : 0.0f;
             }
         };
         uint64_t cuts = __ballot(lane < n && cut_at(a, b, pos + lane, len));
@@ -552,7 +557,8 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
         rz.template store<false>(zs, tid);
         factors(cuts);
         if (ry.not_finite() || rz.not_finite()) bad_s = pos;
-        if (pos + n < p1) load(pos + n);
+        step(n);
+        if (pos + n < p1) load(min(C, p1 - pos - n));
         __syncthreads();
         if (bad_s == pos) {
             // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
@@ -562,25 +568,29 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             bool head = false;
             for (int j = 0; j < n; ++j) {
                 bool bad = false;
-                for (int c = tid; c < DX; c += NT) bad |= (ys[j][c] & 0x7F80) == 0x7F80;
-                for (int c = tid; c < DZ; c += NT) bad |= (zs[j][c] & 0x7F80) == 0x7F80;
+                for (unsigned c = tid; c < DX; c += NT) bad |= (ys[j][c] & 0x7F80) == 0x7F80;
+                for (unsigned c = tid; c < DZ; c += NT) bad |= (zs[j][c] & 0x7F80) == 0x7F80;
                 if (j == 0) head = __syncthreads_or(bad);
                 else if (bad) atomicMin(&first_s, j);
             }
             __syncthreads();
+            step(-n);
             n = first_s;
             if (head && (cuts & ~1ull)) n = min(n, (int)__builtin_ctzll(cuts & ~1ull));
             cuts &= ~0ull >> (64 - n);
-            for (int id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0;
-            for (int id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0;
-            if (pos + n < p1) load(pos + n);
+            for (unsigned id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0;
+            for (unsigned id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0;
+            step(n);
+            if (pos + n < p1) load(min(C, p1 - pos - n));
             factors(cuts);
             __syncthreads();
         }
         floatx4 O[4];
         uintx4 zv[2];  // z rows 32 js .. of the wave's columns: the operand of P Z, weighted that of S
+        auto load_z = [&] {
 #pragma unroll
-        for (int js = 0; js < 2; ++js) zv[js] = column32<false>(zs, 32 * js, c0, lane);
+            for (int js = 0; js < 2; ++js) zv[js] = column32<false>(zs, 32 * js, c0, lane);
+        };
         if (want_out) {
             // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in ten 16 x 16 tiles (j, i), shared
             // out over the waves and handed to all of them as operands, two pieces each
@@ -633,6 +643,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                     for (int r = 0; r < 4; ++r) O[it][r] = f[r] != 0.0f ? O[it][r] : 0.0f;
                 }
             }
+            load_z();
             __syncthreads();  // P is there
 #pragma unroll
             for (int it = 0; it < 4; ++it)
@@ -644,6 +655,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                             *(const bf16x8 *)&ps[it + (it == 3) + js][p][lane], __builtin_bit_cast(bf16x8, zv[js]), O[it],
                             0, 0, 0);
         }
+        if (!want_out) load_z();
         // S = lam^n S + sum_j s3 lam^(n - e0 - j) y_j z_j^T
         {
             const float keep = decay_pow(lam2, n);
@@ -706,7 +718,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     // rows behind the sequence's end are 0
     if (want_out)
         for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
-            for (int c = tid; c < a.dz; c += NT) {
+            for (int c = (int)tid; c < a.dz; c += NT) {
                 const int64_t at = b * a.ob + h * a.oh + t * a.ot + c;
                 if (a.out_f32) ((float *)a.out)[at] = 0.0f;
                 else ((__bf16 *)a.out)[at] = (__bf16)0.0f;
