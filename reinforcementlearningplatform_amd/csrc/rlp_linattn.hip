@@ -58,12 +58,11 @@ struct WalkArgs {
     int out_f32;             // out is f32 (a partial of a shared head), not T
 };
 
-// Token at position p of the walk, and whether the walk's link into position p is cut: walking
-// forward by an episode that begins at p's token, backward by one that begins at the token behind.
-__device__ __forceinline__ bool cut_at(const WalkArgs &a, int b, int p, int len) {
-    if (!a.reset) return false;
-    if (!a.rev) return a.reset[b * a.rb + p * a.rt] != 0;
-    return p > 0 && a.reset[b * a.rb + (int64_t)(len - p) * a.rt] != 0;
+// Whether the walk's link into position p is cut (not 0): walking forward by an episode that begins at
+// p's token, backward by one that begins at the token behind. As it was loaded, to be waited for later.
+__device__ __forceinline__ uint32_t cut_at(const WalkArgs &a, int b, int p, int len) {
+    if (!a.reset || (a.rev && p == 0)) return 0;
+    return a.reset[b * a.rb + (int64_t)(a.rev ? len - p : p) * a.rt];
 }
 
 // log2 lam; a log_decay of -inf (no memory) becomes a finite number, so that lam^0 is 1 and lam^1 is 0
@@ -93,7 +92,7 @@ template <typename T, int D, int NT>
 struct Rows32 {
     static constexpr int VE = 16 / sizeof(T), VR = D / VE, N = (32 * VR + NT - 1) / NT;
     uintx4 v[N];
-    __device__ __forceinline__ void load(const T *src, int64_t st, int n, int d, int tid) {
+    __device__ __forceinline__ void load(const T *src, int64_t st, int n, int d, unsigned tid) {
         const int row = tid / VR, c = tid % VR * VE;
         const T *p = src + row * st + c;
         if (n == 32 && d == D && 32 * VR % NT == 0) {
@@ -120,11 +119,12 @@ struct Rows32 {
         }
     }
     // Also says whether a value is inf or NaN.
-    __device__ __forceinline__ bool store(float (*dst)[D + 4], int tid) const {
+    __device__ __forceinline__ bool store(float (*dst)[D + 4], unsigned tid) const {
         uint32_t most = 0;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            const int id = k * NT + tid, row = id / VR, c = id % VR * VE;
+            const unsigned id = k * NT + tid;
+            const int row = id / VR, c = id % VR * VE;
             if (32 * VR % NT != 0 && row >= 32) break;
             float f[VE];
             if constexpr (sizeof(T) == 4) {
@@ -166,7 +166,8 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     __shared__ __align__(16) floatx4 ps[3][64];
     __shared__ __align__(16) float into_s[C], from_s[C];
     __shared__ int bad_s, first_s;
-    int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, l15 = lane & 15;
+    unsigned tid = threadIdx.x;
+    int lane = tid & 63, q = lane >> 4, l15 = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, g = blockIdx.y;
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -199,13 +200,18 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     if (tid == 0) bad_s = -1;
     Rows32<T, DX, NT> rx, ry;
     Rows32<T, DZ, NT> rz;
-    auto load = [&](int pos) {
-        const int n = min(C, p1 - pos);
-        if (want_out) rx.load(x + pos * dir * a.xt, dir * a.xt, n, a.dx, tid);
-        ry.load(y + pos * dir * a.yt, dir * a.yt, n, a.dx, tid);
-        rz.load(z + pos * dir * a.zt, dir * a.zt, n, a.dz, tid);
+    const int64_t xs_t = dir * a.xt, ys_t = dir * a.yt, zs_t = dir * a.zt;
+    x += p0 * xs_t, y += p0 * ys_t, z += p0 * zs_t;  // of the chunk to load next, at position `ahead`
+    int ahead = p0;
+    uint32_t cut = 0;
+    auto load = [&](int n) {
+        cut = lane < n ? cut_at(a, b, ahead + lane, len) : 0;
+        if (want_out) rx.load(x, xs_t, n, a.dx, tid);
+        ry.load(y, ys_t, n, a.dx, tid);
+        rz.load(z, zs_t, n, a.dz, tid);
     };
-    if (p0 < p1) load(p0);
+    auto step = [&](int n) { x += n * xs_t, y += n * ys_t, z += n * zs_t, ahead += n; };
+    if (p0 < p1) load(min(C, p1 - p0));
     for (int pos = p0; pos < p1;) {
         tid = anew(tid), lane = tid & 63, q = lane >> 4, l15 = lane & 15, col = c0 + l15;
         int n = min(C, p1 - pos);
@@ -213,18 +219,20 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
         // tokens of the episodes that came in and that goes out
         auto factors = [&](uint32_t cuts) {
             if (tid < C) {
-                into_s[tid] = cuts & (~0u >> (31 - tid)) ? 0.0f : a.s2 * decay_pow(lam2, tid + a.e0);
-                from_s[tid] = tid < n && tid >= begin_of(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - tid) : 0.0f;
+                const int i = tid;
+                into_s[i] = cuts & (~0u >> (31 - i)) ? 0.0f : a.s2 * decay_pow(lam2, i + a.e0);
+                from_s[i] = i < n && i >= begin_of(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - i) : 0.0f;
             }
         };
-        uint32_t cuts = (uint32_t)__ballot(lane < n && cut_at(a, b, pos + lane, len));
+        uint32_t cuts = (uint32_t)__ballot(cut != 0);
         __syncthreads();  // the chunk before is done with the tiles
         if (want_out) rx.store(xs, tid);
         bool bad = ry.store(ys, tid);
         bad |= rz.store(zs, tid);
         if (bad) bad_s = pos;
         factors(cuts);
-        if (pos + n < p1) load(pos + n);
+        step(n);
+        if (ahead < p1) load(min(C, p1 - ahead));
         __syncthreads();
         if (bad_s == pos) {
             // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
@@ -234,18 +242,20 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             bool head = false;
             for (int j = 0; j < n; ++j) {
                 bool here = false;
-                for (int c = tid; c < DX; c += NT) here |= (__float_as_uint(ys[j][c]) & 0x7F800000u) == 0x7F800000u;
-                for (int c = tid; c < DZ; c += NT) here |= (__float_as_uint(zs[j][c]) & 0x7F800000u) == 0x7F800000u;
+                for (unsigned c = tid; c < DX; c += NT) here |= (__float_as_uint(ys[j][c]) & 0x7F800000u) == 0x7F800000u;
+                for (unsigned c = tid; c < DZ; c += NT) here |= (__float_as_uint(zs[j][c]) & 0x7F800000u) == 0x7F800000u;
                 if (j == 0) head = __syncthreads_or(here);
                 else if (here) atomicMin(&first_s, j);
             }
             __syncthreads();
+            step(-n);
             n = first_s;
             if (head && (cuts & ~1u)) n = min(n, (int)__builtin_ctz(cuts & ~1u));
             cuts &= ~0u >> (32 - n);
-            for (int id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0.0f;
-            for (int id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0.0f;
-            if (pos + n < p1) load(pos + n);
+            for (unsigned id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0.0f;
+            for (unsigned id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0.0f;
+            step(n);
+            if (ahead < p1) load(min(C, p1 - ahead));
             factors(cuts);
             __syncthreads();
         }
@@ -347,7 +357,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     // rows behind the sequence's end are 0
     if (want_out)
         for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
-            for (int c = tid; c < a.dz; c += NT) {
+            for (int c = (int)tid; c < a.dz; c += NT) {
                 const int64_t at = b * a.ob + h * a.oh + t * a.ot + c;
                 if (a.out_f32) ((float *)a.out)[at] = 0.0f;
                 else ((T *)a.out)[at] = (T)0.0f;
@@ -530,13 +540,16 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     Rows16<DX, NT> rx, ry;
     Rows16<DZ, NT> rz;
     const int64_t xs_t = dir * a.xt, ys_t = dir * a.yt, zs_t = dir * a.zt;
-    x += p0 * xs_t, y += p0 * ys_t, z += p0 * zs_t;  // of the chunk to load next
+    x += p0 * xs_t, y += p0 * ys_t, z += p0 * zs_t;  // of the chunk to load next, at position `ahead`
+    int ahead = p0;
+    uint32_t cut = 0;
     auto load = [&](int n) {
+        cut = lane < n ? cut_at(a, b, ahead + lane, len) : 0;
         if (want_out) rx.load(x, xs_t, n, a.dx, tid);
         ry.load(y, ys_t, n, a.dx, tid);
         rz.load(z, zs_t, n, a.dz, tid);
     };
-    auto step = [&](int n) { x += n * xs_t, y += n * ys_t, z += n * zs_t; };
+    auto step = [&](int n) { x += n * xs_t, y += n * ys_t, z += n * zs_t, ahead += n; };
     if (p0 < p1) load(min(C, p1 - p0));
     for (int pos = p0; pos < p1;) {
         tid = anew(tid), lane = tid & 63, q = lane >> 4, l15 = lane & 15, col = c0 + l15;
@@ -550,7 +563,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                 from_s[i] = i < n && i >= begin_of64(cuts, n - 1) ? a.s3 * decay_pow(lam2, n - a.e0 - i) : 0.0f;
             }
         };
-        uint64_t cuts = __ballot(lane < n && cut_at(a, b, pos + lane, len));
+        uint64_t cuts = __ballot(cut != 0);
         __syncthreads();  // the chunk before is done with the tiles
         if (want_out) rx.template store<true>(xs, tid);
         ry.template store<true>(ys, tid);
@@ -558,7 +571,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
         factors(cuts);
         if (ry.not_finite() || rz.not_finite()) bad_s = pos;
         step(n);
-        if (pos + n < p1) load(min(C, p1 - pos - n));
+        if (ahead < p1) load(min(C, p1 - ahead));
         __syncthreads();
         if (bad_s == pos) {
             // An inf or NaN would reach rows it has no part in, through 0 * x in the products: the
@@ -581,7 +594,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             for (unsigned id = tid; id < (C - n) * DX; id += NT) ys[n + id / DX][id % DX] = 0;
             for (unsigned id = tid; id < (C - n) * DZ; id += NT) zs[n + id / DZ][id % DZ] = 0;
             step(n);
-            if (pos + n < p1) load(min(C, p1 - pos - n));
+            if (ahead < p1) load(min(C, p1 - ahead));
             factors(cuts);
             __syncthreads();
         }
