@@ -667,19 +667,22 @@ typedef struct rlp_la_cfg {
     int64_t dq_stride[3], dk_stride[3], dv_stride[3];            /* backward only */
     int64_t reset_stride[2];
 } rlp_la_cfg;
-/* Scratch of one call (0: none); it holds nothing between calls. */
+/* Scratch of one call (0: none). What the forward leaves in it, the states before each part of a split
+ * sequence, its backward can take (forward_workspace: the same sizes and inputs); else it is free. */
 int64_t rlp_linear_attention_workspace_bytes(const rlp_la_cfg *cfg, int backward);
 int rlp_linear_attention(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
                          const float *log_decay, const uint8_t *reset, const int32_t *lengths,
                          const float *state, void *out, float *state_out, void *workspace,
                          int64_t workspace_bytes, rlp_stream_t stream);
 /* Gradients of q, k, v (required; of shared heads the sum over their states) and of state
- * (nullable) from d_out and d_state_out (nullable: 0). State is recomputed from the inputs. */
+ * (nullable) from d_out and d_state_out (nullable: 0). States are recomputed from the inputs, but for
+ * those in forward_workspace (nullable). */
 int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
                                   const float *log_decay, const uint8_t *reset, const int32_t *lengths,
                                   const float *state, const void *d_out, const float *d_state_out,
-                                  void *dq, void *dk, void *dv, float *d_state, void *workspace,
-                                  int64_t workspace_bytes, rlp_stream_t stream);
+                                  const void *forward_workspace, void *dq, void *dk, void *dv,
+                                  float *d_state, void *workspace, int64_t workspace_bytes,
+                                  rlp_stream_t stream);
 /* One token for every sequence (T = 1): state_out = reset ? 0 : lam state, + k v^T; state_out may be
  * state. reset [B], stride reset_stride[0]. */
 int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,

@@ -80,7 +80,7 @@ def _declare(lib):
         "rlp_sac_update": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
         "rlp_linear_attention_workspace_bytes": (i64, [vp, i32]),
         "rlp_linear_attention": (i32, [vp] * 11 + [i64, vp]),
-        "rlp_linear_attention_backward": (i32, [vp] * 15 + [i64, vp]),
+        "rlp_linear_attention_backward": (i32, [vp] * 16 + [i64, vp]),
         "rlp_linear_attention_step": (i32, [vp] * 10),
         "rlp_token_logprob_workspace_bytes": (i64, [i64, i64, i32, i32]),
         "rlp_token_logprob": (i32, [vp, i32, i64, i64, i64, vp, C.c_float, i32, vp, vp, vp, vp, vp, vp,

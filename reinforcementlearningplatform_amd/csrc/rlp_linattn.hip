@@ -66,7 +66,10 @@ __device__ __forceinline__ uint32_t cut_at(const WalkArgs &a, int b, int p, int 
 }
 
 // log2 lam; a log_decay of -inf (no memory) becomes a finite number, so that lam^0 is 1 and lam^1 is 0
-__device__ __forceinline__ float log2_decay(float log_decay) { return fmaxf(log_decay * kLog2e, -1e6f); }
+__device__ __forceinline__ float log2_decay(float log_decay) {
+    const float l = log_decay * kLog2e;
+    return l < -1e6f ? -1e6f : l;  // a NaN stays one
+}
 __device__ __forceinline__ float decay_pow(float lam2, int n) {
     return __builtin_amdgcn_exp2f(lam2 * (float)n);
 }
@@ -356,8 +359,8 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     }
     // rows behind the sequence's end are 0
     if (want_out)
-        for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
-            for (int c = (int)tid; c < a.dz; c += NT) {
+        for (int t = max(p0, len) + (int)tid / DZ; t < min(a.T, p0 + a.seglen); t += NT / DZ)
+            if (const int c = tid % DZ; c < a.dz) {
                 const int64_t at = b * a.ob + h * a.oh + t * a.ot + c;
                 if (a.out_f32) ((float *)a.out)[at] = 0.0f;
                 else ((T *)a.out)[at] = (T)0.0f;
@@ -730,8 +733,8 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     }
     // rows behind the sequence's end are 0
     if (want_out)
-        for (int t = max(p0, len); t < min(a.T, p0 + a.seglen); ++t)
-            for (int c = (int)tid; c < a.dz; c += NT) {
+        for (int t = max(p0, len) + (int)tid / DZ; t < min(a.T, p0 + a.seglen); t += NT / DZ)
+            if (const int c = tid % DZ; c < a.dz) {
                 const int64_t at = b * a.ob + h * a.oh + t * a.ot + c;
                 if (a.out_f32) ((float *)a.out)[at] = 0.0f;
                 else ((__bf16 *)a.out)[at] = (__bf16)0.0f;
@@ -935,7 +938,8 @@ void launch_walk(const WalkArgs &a, hipStream_t s) {
     else launch_walk<T, 4>(a, s);
 }
 
-// have_states: ws holds the segments' states of the walk before, which were this one's transposed.
+// have_states: ws holds the segments' states of another walk, which were this one's transposed; they are
+// read only.
 template <typename T>
 void walk(WalkArgs a, float *ws, hipStream_t s, bool have_states = false) {
     const int64_t bh = (int64_t)a.B * a.H;
@@ -995,7 +999,8 @@ void share(const rlp_la_cfg &c, const float *part, void *out, const int64_t *st,
 template <typename T>
 void backward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, const float *log_decay,
               const uint8_t *reset, const int32_t *lengths, const float *init, const void *d_out,
-              const float *d_fin, void *dq, void *dk, void *dv, float *d_init, float *ws, hipStream_t s) {
+              const float *d_fin, void *dq, void *dk, void *dv, float *d_init, const float *forward_ws, float *ws,
+              hipStream_t s) {
     const int64_t bh = (int64_t)c.B * c.H;
     float *part = ws + segment_floats(bh, c.T, c.Dk, c.Dv);
     // a gradient of unshared heads goes straight out, of shared heads through f32 partials
@@ -1017,7 +1022,7 @@ void backward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, 
         a.init = init, a.ia = 1, a.in = c.Dv;  // S transposed
         a.e0 = 1, a.s1 = a.s2 = c.scale, a.s3 = 1.0f;
         target(a, dq, c.dq_stride, c.Hq, c.Dk);
-        walk<T>(a, ws, s);
+        walk<T>(a, forward_ws ? const_cast<float *>(forward_ws) : ws, s, forward_ws != nullptr);
         if (c.Hq != c.H) share<T>(c, part, dq, c.dq_stride, c.Hq, c.Dk, s);
     }
     if (dv || d_init) {
@@ -1058,7 +1063,7 @@ int check_cfg(const rlp_la_cfg *c, const char *who) {
                 c->Hq, c->Hk, c->Hv);
     RLP_REQUIRE(c->Dk >= 1 && c->Dk <= kMaxD && c->Dv >= 1 && c->Dv <= kMaxD,
                 "%s: Dk %d, Dv %d (1 to %d)", who, c->Dk, c->Dv, kMaxD);
-    RLP_REQUIRE((int64_t)c->B * c->H <= 0x7FFFFFFFLL, "%s: B x H too large", who);
+    RLP_REQUIRE((int64_t)c->B * c->H < (1 << 23) && c->T <= (1 << 30), "%s: B x H or T too large", who);
     return RLP_OK;
 }
 
@@ -1117,8 +1122,9 @@ int rlp_linear_attention(const rlp_la_cfg *cfg, const void *q, const void *k, co
 int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
                                   const float *log_decay, const uint8_t *reset, const int32_t *lengths,
                                   const float *state, const void *d_out, const float *d_state_out,
-                                  void *dq, void *dk, void *dv, float *d_state, void *workspace,
-                                  int64_t workspace_bytes_, rlp_stream_t stream) {
+                                  const void *forward_workspace, void *dq, void *dk, void *dv,
+                                  float *d_state, void *workspace, int64_t workspace_bytes_,
+                                  rlp_stream_t stream) {
     take_pending();
     const int rc = check_cfg(cfg, "rlp_linear_attention_backward");
     if (rc != RLP_OK) return rc;
@@ -1131,7 +1137,8 @@ int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const vo
                 (long long)workspace_bytes_, (long long)need);
     by_type(cfg->dtype, [&](auto *t) {
         backward<std::remove_pointer_t<decltype(t)>>(*cfg, q, k, v, log_decay, reset, lengths, state, d_out,
-                                                     d_state_out, dq, dk, dv, d_state, (float *)workspace,
+                                                     d_state_out, dq, dk, dv, d_state,
+                                                     (const float *)forward_workspace, (float *)workspace,
                                                      as_stream(stream));
     });
     RLP_CHECK_LAUNCH("rlp_linear_attention_backward");

@@ -580,8 +580,8 @@ int check_rows(const char *who, int dtype, int64_t rows, int64_t vocab, int64_t 
     RLP_REQUIRE(rows >= 0 && rows <= 0x7FFFFFFFLL, "%s: %lld rows", who, (long long)rows);
     RLP_REQUIRE(vocab >= 1 && vocab <= 0x7FF00000LL, "%s: vocab %lld", who, (long long)vocab);
     RLP_REQUIRE(stride >= 0, "%s: row stride %lld", who, (long long)stride);
-    RLP_REQUIRE(temperature > 0.0f && temperature <= 3.402823466e38f, "%s: temperature %g (a positive number)",
-                who, temperature);
+    RLP_REQUIRE(temperature >= 1e-30f && temperature <= 1e30f, "%s: temperature %g (1e-30 to 1e30)", who,
+                temperature);
     return RLP_OK;
 }
 

@@ -598,7 +598,8 @@ def _la_flags(what, reset, lengths, want, B):
 
 def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=None, lengths=None,
                              return_state=False):
-    """rlp_linear_attention without autograd (arguments as linear_attention): (out, state or None)."""
+    """rlp_linear_attention without autograd (arguments as linear_attention): (out, state or None,
+    workspace or None); the workspace can go into linear_attention_backward."""
     what = "linear_attention"
     dims = _la_dims(what, q, k, v, log_decay, state)
     need = _la_workspace_bytes(what, 0, *dims)
@@ -616,13 +617,14 @@ def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=N
     _launch(what, q.get_device(), lib().rlp_linear_attention, cfg,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _at(reset), _at(lengths),
             _at(state), out.data_ptr(), _at(last), _at(ws), need)
-    return out, last
+    return out, last, ws
 
 
 def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, state=None, reset=None,
-                              lengths=None):
+                              lengths=None, forward_workspace=None):
     """rlp_linear_attention_backward: (dq, dk, dv, gradient of state or None) from the gradients of
-    linear_attention's out and state (d_state None: 0)."""
+    linear_attention's out and state (d_state None: 0); forward_workspace: linear_attention_forward's of the
+    same arguments, which spares a pass over k and v where sequences are split."""
     what = "linear_attention_backward"
     dims = _la_dims(what, q, k, v, log_decay, state)
     need = _la_workspace_bytes(what, 1, *dims)
@@ -632,7 +634,9 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
         raise RLPError(f"{what}: d_out {d_out.dtype} {tuple(d_out.shape)}")
     if d_state is not None and (d_state.dtype != torch.float32 or d_state.shape != (B, H, Dk, Dv)):
         raise RLPError(f"{what}: d_state {d_state.dtype} {tuple(d_state.shape)}")
-    _one_device(what, q, k, v, log_decay, state, reset, lengths, d_out, d_state)
+    if forward_workspace is not None and forward_workspace.numel() != _la_workspace_bytes(what, 0, *dims):
+        raise RLPError(f"{what}: forward_workspace of {forward_workspace.numel()} bytes is of another forward")
+    _one_device(what, q, k, v, log_decay, state, reset, lengths, d_out, d_state, forward_workspace)
     q, k, v, d_out, log_decay = _rows(q), _rows(k), _rows(v), _rows(d_out), log_decay.contiguous()
     first = torch.empty_like(state, memory_format=torch.contiguous_format) if state is not None else None
     state = state.contiguous() if state is not None else None
@@ -645,6 +649,7 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
                                 *(reset.stride() if reset is not None else (0, 0)))
     _launch(what, q.get_device(), lib().rlp_linear_attention_backward, cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(),
             log_decay.data_ptr(), _at(reset), _at(lengths), _at(state), d_out.data_ptr(), _at(d_state),
+            _at(forward_workspace),
             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(first), _at(ws), need)
     return dq, dk, dv, first
 
@@ -652,8 +657,8 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, scale, state, reset, lengths, return_state):
-        out, last = linear_attention_forward(q, k, v, log_decay, scale, state, reset, lengths, return_state)
-        ctx.save_for_backward(q, k, v, log_decay, state, reset, lengths)
+        out, last, ws = linear_attention_forward(q, k, v, log_decay, scale, state, reset, lengths, return_state)
+        ctx.save_for_backward(q, k, v, log_decay, state, reset, lengths, ws)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return (out, last) if return_state else out
@@ -663,11 +668,11 @@ class _LinearAttention(torch.autograd.Function):
     def backward(ctx, d_out, d_state=None):
         if d_out is None and d_state is None:
             return (None,) * 9
-        q, k, v, log_decay, state, reset, lengths = ctx.saved_tensors
+        q, k, v, log_decay, state, reset, lengths, ws = ctx.saved_tensors
         if d_out is None:
             d_out = _like_order(q, q.shape[0], q.shape[1], log_decay.shape[0], v.shape[3]).zero_()
         dq, dk, dv, first = linear_attention_backward(d_out, d_state, q, k, v, log_decay, ctx.scale, state,
-                                                      reset, lengths)
+                                                      reset, lengths, ws)
         return dq, dk, dv, None, None, first, None, None, None
 
 
@@ -694,7 +699,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, len
                 state is not None and state.requires_grad:
             return _LinearAttention.apply(q, k, v, log_decay, scale, state, reset, lengths,
                                           bool(return_state))
-    out, last = linear_attention_forward(q, k, v, log_decay, scale, state, reset, lengths, return_state)
+    out, last, _ = linear_attention_forward(q, k, v, log_decay, scale, state, reset, lengths, return_state)
     return (out, last) if return_state else out
 
 

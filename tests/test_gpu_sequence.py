@@ -731,3 +731,29 @@ def test_policy_acts_and_learns(K):
                                list(p64.values()))
     for m, a, b in zip(par, got, want):
         assert torch.allclose(a.cpu().double(), b, rtol=1e-3, atol=1e-4 * float(b.abs().max())), m
+
+
+def test_la_backward_with_and_without_the_forwards_states(K):
+    """The raw wrappers: the gradients are the same whether the states of the parts of a split sequence
+    come from the forward or are formed anew; another forward's workspace is refused."""
+    from reinforcementlearningplatform_amd._native import RLPError
+    s = la_inputs(1, 1500, 2, (1, 2, 2), 64, 48, F32, seed=41, reset=0.003)
+    args = [s[n].cuda() for n in "qkv"] + [s["ld"].cuda()]
+    kw = dict(state=s["state"].cuda(), reset=s["reset"].cuda())
+    out, last, ws = K.linear_attention_forward(*args, return_state=True, **kw)
+    assert ws is not None
+    a = K.linear_attention_backward(s["d_out"].cuda(), s["d_state"].cuda(), *args, forward_workspace=ws, **kw)
+    b = K.linear_attention_backward(s["d_out"].cuda(), s["d_state"].cuda(), *args, **kw)
+    # the states are the same sums, read in another order of the pieces they are held in
+    for x, y in zip(a, b):
+        assert torch.allclose(x, y, rtol=1e-5, atol=1e-5 * float(y.abs().max()))
+    with pytest.raises(RLPError, match="another forward"):
+        K.linear_attention_backward(s["d_out"].cuda(), None, *args, forward_workspace=ws[:-4], **kw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_la_nan_decay_shows(K, dtype):
+    s = la_inputs(1, 70, 2, (2, 2, 2), 16, 16, dtype, seed=2)
+    s["ld"][1] = float("nan")
+    out = K.linear_attention(*[s[n].cuda() for n in "qkv"], s["ld"].cuda())
+    assert torch.isnan(out[0, 1:, 1]).all() and torch.isfinite(out[:, :, 0]).all()

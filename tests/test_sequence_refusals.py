@@ -36,7 +36,7 @@ def test_linear_attention_cfg_is_checked(over, word):
     lib = _native.lib()
     assert la_forward(c) == _abi.RLP_EINVAL and word in lib.rlp_last_error_string()
     assert lib.rlp_linear_attention_workspace_bytes(C.byref(c), 1) == _abi.RLP_EINVAL
-    assert lib.rlp_linear_attention_backward(C.byref(c), *[DEV] * 14, 1 << 40, None) == _abi.RLP_EINVAL
+    assert lib.rlp_linear_attention_backward(C.byref(c), *[DEV] * 15, 1 << 40, None) == _abi.RLP_EINVAL
     c.T = 1 if c.T == 8 else c.T
     assert lib.rlp_linear_attention_step(C.byref(c), *[DEV] * 8, None) == _abi.RLP_EINVAL
 
