@@ -420,16 +420,16 @@ __device__ __forceinline__ int begin_of64(uint64_t m, int i) {
     return below ? 63 - __builtin_clzll(below) : -1;
 }
 
-// 64 rows of D bf16 columns on their way from global memory to LDS: 16 bytes a thread and step.
-template <int D, int NT>
+// C rows of D bf16 columns on their way from global memory to LDS: 16 bytes a thread and step at any
+// alignment; rows >= n and columns >= d become 0.
+template <int C, int D, int NT>
 struct Rows16 {
-    static constexpr int VR = D / 8, N = (64 * VR + NT - 1) / NT;
+    static constexpr int VR = D / 8, N = (C * VR + NT - 1) / NT;
     uintx4 v[N];
-    // d: a multiple of 8, so a vector is wholly inside the row or behind it
     __device__ __forceinline__ void load(const __bf16 *src, int64_t st, int n, int d, unsigned tid) {
         const int row = tid / VR, c = tid % VR * 8;
         const __bf16 *p = src + row * st + c;
-        if (n == 64 && d == D && 64 * VR >= NT) {
+        if (n == C && d == D && C * VR >= NT) {
 #pragma unroll
             for (int k = 0; k < N; ++k) v[k] = *(const uintx4_any *)(p + k * (NT / VR) * st);
             return;
@@ -437,7 +437,15 @@ struct Rows16 {
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             v[k] = (uintx4){0, 0, 0, 0};
-            if (c < d && row + k * (NT / VR) < n) v[k] = *(const uintx4_any *)(p + k * (NT / VR) * st);
+            if (row + k * (NT / VR) >= n) continue;
+            const __bf16 *pk = p + k * (NT / VR) * st;
+            if (c + 8 <= d) {
+                v[k] = *(const uintx4_any *)pk;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 7; ++e)
+                    if (c + e < d) v[k][e / 2] |= (uint32_t)__builtin_bit_cast(unsigned short, pk[e]) << (16 * (e & 1));
+            }
         }
     }
     // PERM: of 32 columns the four-column groups in the order 0 4 1 5 2 6 3 7, in which a quarter wave's
@@ -448,7 +456,7 @@ struct Rows16 {
         for (int k = 0; k < N; ++k) {
             const unsigned id = k * NT + tid;
             const int row = id / VR, c = id % VR * 8;
-            if (64 * VR < NT && row >= 64) break;
+            if (C * VR < NT && row >= C) break;
             if (PERM) {
                 const int at = (c & ~31) + (c & 8) * 2 + (c & 16) / 4;
                 *(uintx2 *)&dst[row][at] = (uintx2){v[k][0], v[k][1]};
@@ -485,7 +493,7 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
     return (uintx4){a[0], a[1], b[0], b[1]};
 }
 
-// la_walk_kernel for bf16 operands on v_mfma_f32_16x16x32_bf16, 64 tokens a chunk. Products of the
+// la_walk_kernel for bf16 operands on v_mfma_f32_16x16x32_bf16, C tokens a chunk. Products of the
 // operands are exact in f32; what is not an operand is split into bf16 pieces where it meets the
 // matrix cores: P and S for the output into two (2^-16, below the output's own rounding), the
 // weighted z of the state's sum into PZ: three (2^-24) where the state leaves the call, so that it is
@@ -498,13 +506,14 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 //
 // 16 columns a wave, not 32: with 32x32 tiles at two waves a SIMD the same work waited on LDS and on
 // its own products (9 us a chunk of 128 x 128); half the registers a wave let four waves run.
-template <int DXB, int NW, int PZ>
+template <int DXB, int NW, int PZ, int C>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
-    constexpr int C = 64, DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW, PAD = 16;
+    constexpr int CT = C / 16, NP = CT * (CT + 1) / 2, SLOTS = C == 64 ? 6 : 2;  // token tiles, P's, their operands
+    constexpr int DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW, PAD = 16;
     __shared__ __align__(16) unsigned short xs[C][DX + PAD];
     __shared__ __align__(16) unsigned short ys[C][DX + PAD];
     __shared__ __align__(16) unsigned short zs[C][DZ + PAD];
-    __shared__ __align__(16) uintx2 ps[6][2][64][2];  // (token tile, 32 tokens), piece, lane, half
+    __shared__ __align__(16) uintx2 ps[SLOTS][2][64][2];  // (token tile, 32 tokens), piece, lane, half
     __shared__ __align__(16) float into_s[C], from_s[C];
     __shared__ int bad_s, first_s;
     unsigned tid = threadIdx.x;
@@ -539,9 +548,9 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     }
     bool seg_cut = false;
     if (tid == 0) bad_s = -1;
-    for (unsigned id = tid; id < 6 * 2 * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
-    Rows16<DX, NT> rx, ry;
-    Rows16<DZ, NT> rz;
+    for (unsigned id = tid; id < SLOTS * 2 * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
+    Rows16<C, DX, NT> rx, ry;
+    Rows16<C, DZ, NT> rz;
     const int64_t xs_t = dir * a.xt, ys_t = dir * a.yt, zs_t = dir * a.zt;
     x += p0 * xs_t, y += p0 * ys_t, z += p0 * zs_t;  // of the chunk to load next, at position `ahead`
     int ahead = p0;
@@ -601,16 +610,16 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             factors(cuts);
             __syncthreads();
         }
-        floatx4 O[4];
-        uintx4 zv[2];  // z rows 32 js .. of the wave's columns: the operand of P Z, weighted that of S
+        floatx4 O[CT];
+        uintx4 zv[CT / 2];  // z rows 32 js .. of the wave's columns: the operand of P Z, weighted that of S
         auto load_z = [&] {
 #pragma unroll
-            for (int js = 0; js < 2; ++js) zv[js] = column32<false>(zs, 32 * js, c0, lane);
+            for (int js = 0; js < CT / 2; ++js) zv[js] = column32<false>(zs, 32 * js, c0, lane);
         };
         if (want_out) {
-            // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in ten 16 x 16 tiles (j, i), shared
+            // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in 16 x 16 tiles (j, i), shared
             // out over the waves and handed to all of them as operands, two pieces each
-            for (int t = w; t < 10; t += NW) {
+            for (int t = w; t < NP; t += NW) {
                 const int it = (t > 0) + (t > 2) + (t > 5), jt = t - it * (it + 1) / 2;
                 floatx4 P = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -634,7 +643,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             }
             // x S, decayed to each row
 #pragma unroll
-            for (int it = 0; it < 4; ++it) O[it] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int it = 0; it < CT; ++it) O[it] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < DXB; ++s) {
                 bf16x8 Sp[2];
@@ -643,14 +652,14 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                 for (int e = 0; e < 8; ++e) sv[e] = S[2 * s + (e >> 2)][e & 3];
                 split8(sv, Sp);
 #pragma unroll
-                for (int it = 0; it < 4; ++it) {
+                for (int it = 0; it < CT; ++it) {
                     const bf16x8 X = *(const bf16x8 *)&xs[16 * it + l15][32 * s + 8 * q];
                     O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[0], O[it], 0, 0, 0);
                     O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[1], O[it], 0, 0, 0);
                 }
             }
 #pragma unroll
-            for (int it = 0; it < 4; ++it) {
+            for (int it = 0; it < CT; ++it) {
                 const floatx4 f = *(const floatx4 *)&into_s[16 * it + 4 * q];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) O[it][r] *= f[r];
@@ -662,7 +671,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             load_z();
             __syncthreads();  // P is there
 #pragma unroll
-            for (int it = 0; it < 4; ++it)
+            for (int it = 0; it < CT; ++it)
 #pragma unroll
                 for (int js = 0; js < (it >> 1) + 1; ++js)
 #pragma unroll
@@ -685,7 +694,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             for (int at = 0; at < 2 * DXB; ++at) S[at] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
         }
 #pragma unroll
-        for (int js = 0; js < 2; ++js) {
+        for (int js = 0; js < CT / 2; ++js) {
             float wz[8];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
@@ -706,7 +715,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
             // out through the wave's own columns of the z tile, which it is done with: 16-byte stores
             if (!a.out_f32) {
 #pragma unroll
-                for (int it = 0; it < 4; ++it)
+                for (int it = 0; it < CT; ++it)
 #pragma unroll
                     for (int r = 0; r < 4; r += 2) {
                         const uint32_t o = pack2(O[it][r], O[it][r + 1]);
@@ -716,13 +725,20 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                 const int row = lane >> 1, c = c0 + (lane & 1) * 8;
                 __bf16 *o = (__bf16 *)a.out + out0 + (pos + row) * dir * a.ot + c;
 #pragma unroll
-                for (int k = 0; k < 2; ++k)
-                    if (c < a.dz && row + 32 * k < n) *(uintx4_any *)(o + 32 * k * dir * a.ot) = *(uintx4 *)&zs[row + 32 * k][c];
+                for (int k = 0; k < CT / 2; ++k) {
+                    if (row + 32 * k >= n) continue;
+                    __bf16 *ok = o + 32 * k * dir * a.ot;
+                    if (c + 8 <= a.dz) {
+                        *(uintx4_any *)ok = *(uintx4 *)&zs[row + 32 * k][c];
+                    } else {
+                        for (int e = 0; c + e < a.dz; ++e) ok[e] = __builtin_bit_cast(__bf16, zs[row + 32 * k][c + e]);
+                    }
+                }
             } else {
                 float *o = (float *)a.out + out0 + (pos + 4 * q) * dir * a.ot + col;
                 if (col < a.dz)
 #pragma unroll
-                    for (int it = 0; it < 4; ++it)
+                    for (int it = 0; it < CT; ++it)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (16 * it + 4 * q + r < n) o[(16 * it + r) * dir * a.ot] = O[it][r];
@@ -920,11 +936,21 @@ void launch_walk(const WalkArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.B * a.H), a.nseg);
     auto go = [&](auto nw) {
         constexpr int NW = decltype(nw)::value;
-        if (std::is_same_v<T, __bf16> && a.dx % 8 == 0 && a.dz % 8 == 0) {
-            if (a.fin && a.mode != 2) la_walk_bf16_kernel<DXB, NW, 3><<<grid, 64 * NW, 0, s>>>(a);
-            else la_walk_bf16_kernel<DXB, NW, 2><<<grid, 64 * NW, 0, s>>>(a);
-        } else
+        if constexpr (std::is_same_v<T, __bf16>) {
+            // 64 tokens a chunk: half the barriers and state steps. Up to 64 columns 32 tokens leave LDS for twice
+            // the blocks, which pays where there are blocks enough: 16384 of 128 tokens, 64 x 64, in 278 us for
+            // 302, but 512 of 2048 tokens in 182 for 149
+            auto chunk = [&](auto c) {
+                constexpr int C = decltype(c)::value;
+                if (a.fin && a.mode != 2) la_walk_bf16_kernel<DXB, NW, 3, C><<<grid, 64 * NW, 0, s>>>(a);
+                else la_walk_bf16_kernel<DXB, NW, 2, C><<<grid, 64 * NW, 0, s>>>(a);
+            };
+            if constexpr (NW <= 4)
+                if ((int64_t)grid.x * a.nseg >= 2048) return chunk(std::integral_constant<int, 32>{});
+            chunk(std::integral_constant<int, 64>{});
+        } else {
             la_walk_kernel<T, DXB, NW><<<grid, 64 * NW, 0, s>>>(a);
+        }
     };
     if (a.dz <= 32) go(std::integral_constant<int, 2>{});
     else if (a.dz <= 64) go(std::integral_constant<int, 4>{});
