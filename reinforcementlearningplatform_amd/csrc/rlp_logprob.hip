@@ -76,12 +76,19 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
     return r;
 }
 
-template <int G>
-__device__ __forceinline__ Sums join_lanes(Sums v, float c) {
+// Of all lanes: first the maximum, then the sums about it.
+__device__ __forceinline__ Sums join_wave(Sums v, float c) {
+    float m = v.m;
 #pragma unroll
-    for (int d = G / 2; d > 0; d >>= 1) {
-        Sums o = {__shfl_xor(v.m, d), __shfl_xor(v.s, d), __shfl_xor(v.w, d)};
-        v = join(v, o, c);
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float y = (v.m - base_of(m)) * c, e = __builtin_amdgcn_exp2f(y);
+    v.w = e * __builtin_fmaf(fmaxf(y, -200.0f), v.s, v.w);
+    v.s *= e;
+    v.m = m;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        v.s += __shfl_xor(v.s, d);
+        v.w += __shfl_xor(v.w, d);
     }
     return v;
 }
@@ -132,61 +139,6 @@ __device__ __forceinline__ void write_top(const ScoreArgs &a, int64_t row, int i
 
 __device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
-// Rows of up to G * E logits, G lanes a row, all of it in registers: lane g holds tokens g + G e.
-template <typename T, int G, int E>
-__global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
-    const int g = threadIdx.x % G;
-    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
-    if (row >= a.rows) return;
-    const int64_t tok = a.tokens[row];
-    if (tok < 0) {
-        if (g == 0) write_padded(a, row);
-        return;
-    }
-    const T *l = (const T *)a.logits + row * a.stride;
-    float x[E];
-    Sums v = {neg_inf(), 0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        x[e] = g + G * e < a.vocab ? to_f32(l[g + G * e]) : neg_inf();
-        v.m = fmaxf(v.m, x[e]);
-    }
-    const float lt = tok < a.vocab ? to_f32(l[tok]) : 0.0f;
-#pragma unroll
-    for (int d = G / 2; d > 0; d >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, d));
-    const float base = base_of(v.m);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float y = (x[e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
-        v.s += p;
-        v.w += p * fmaxf(y, -200.0f);
-    }
-#pragma unroll
-    for (int d = G / 2; d > 0; d >>= 1) {
-        v.s += __shfl_xor(v.s, d);
-        v.w += __shfl_xor(v.w, d);
-    }
-    if (g == 0) write_row(a, row, tok, lt, v);
-    uint32_t open = 0;  // own tokens that are still to choose from
-#pragma unroll
-    for (int e = 0; e < E; ++e) open |= (g + G * e < a.vocab && x[e] == x[e] ? 1u : 0u) << e;
-    for (int i = 0; i < a.k; ++i) {
-        float bv = neg_inf();
-        int bi = kNoIndex;
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if ((open >> e & 1) && ahead(x[e], g + G * e, bv, bi)) bv = x[e], bi = g + G * e;
-#pragma unroll
-        for (int d = G / 2; d > 0; d >>= 1) {
-            const float ov = __shfl_xor(bv, d);
-            const int oi = __shfl_xor(bi, d);
-            if (ahead(ov, oi, bv, bi)) bv = ov, bi = oi;
-        }
-        if (bi != kNoIndex && bi % G == g) open &= ~(1u << (bi / G));
-        if (g == 0) write_top(a, row, i, v, bi == kNoIndex ? 0 : rank_key(bv, bi));
-    }
-}
-
 // A wave's candidates for the k best, in LDS. push takes a lane's candidate where `pick`; select keeps
 // the k best in order. Every key counts the keys above it, which places it at once: no chain from one
 // candidate to the next, as inserting them one by one has (26 us of such chains for 8 rows' 20 best).
@@ -234,7 +186,98 @@ __device__ __forceinline__ float about_kth(float x, int k) {
         const uint32_t t = lo | 1u << bit;
         if (__popcll(__ballot(key >= t)) >= k) lo = t;
     }
+    if (lo < 0x007FFFFFu) return neg_inf();  // below the number of -inf stand NaNs
     return __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
+}
+
+// Rows of up to 8 G logits, G lanes a row, all of it in registers: every lane a 16-byte vector (f32: two,
+// G vectors apart) at any alignment.
+template <typename T, int G>
+__global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
+    constexpr int E = 8, VE = 16 / sizeof(T);
+    const int g = threadIdx.x % G;
+    auto token = [&](int i) { return ((i / VE) * G + g) * VE + i % VE; };  // of the lane's i-th logit
+    const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (row >= a.rows) return;
+    const int64_t tok = a.tokens[row];
+    if (tok < 0) {
+        if (g == 0) write_padded(a, row);
+        return;
+    }
+    const T *l = (const T *)a.logits + row * a.stride;
+    float x[E];
+    Sums v = {neg_inf(), 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < E; c += VE) {
+        T raw[VE];
+        const int t0 = token(c);
+        if (t0 + VE <= a.vocab) {
+            __builtin_memcpy(raw, l + t0, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) raw[e] = t0 + e < a.vocab ? l[t0 + e] : (T)neg_inf();
+        }
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+            x[c + e] = to_f32(raw[e]);
+            v.m = fmaxf(v.m, x[c + e]);
+        }
+    }
+    const float lt = tok < a.vocab ? to_f32(l[tok]) : 0.0f;
+#pragma unroll
+    for (int d = G / 2; d > 0; d >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, d));
+    const float base = base_of(v.m);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float y = (x[e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
+        v.s += p;
+        v.w += p * fmaxf(y, -200.0f);
+    }
+#pragma unroll
+    for (int d = G / 2; d > 0; d >>= 1) {
+        v.s += __shfl_xor(v.s, d);
+        v.w += __shfl_xor(v.w, d);
+    }
+    if (g == 0) write_row(a, row, tok, lt, v);
+    if constexpr (G == 64) {
+        if (a.k > 2) {
+            // a wave a row: what reaches a value that k of the lanes' largest reach, ranked in LDS (2^20 rows of 300
+            // logits, 20 alternatives: 3.5 ms one after the other)
+            __shared__ uint64_t top_s[4][TopBuf::kCap];
+            TopBuf top = {top_s[threadIdx.x >> 6], 0, a.k};
+            float most = neg_inf();
+#pragma unroll
+            for (int e = 0; e < E; ++e) most = fmaxf(most, x[e]);
+            const float lim = about_kth(most, a.k);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (!__any(x[e] >= lim)) continue;
+                const int id = token(e);
+                top.push(x[e] >= lim && id < a.vocab, rank_key(x[e], id));
+            }
+            top.select();
+            if (g < a.k) write_top(a, row, g, v, g < top.n ? top.key[g] : 0);
+            return;
+        }
+    }
+    uint32_t open = 0;  // own tokens that are still to choose from
+#pragma unroll
+    for (int e = 0; e < E; ++e) open |= (token(e) < a.vocab && x[e] == x[e] ? 1u : 0u) << e;
+    for (int i = 0; i < a.k; ++i) {
+        float bv = neg_inf();
+        int bi = kNoIndex;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if ((open >> e & 1) && ahead(x[e], token(e), bv, bi)) bv = x[e], bi = token(e);
+#pragma unroll
+        for (int d = G / 2; d > 0; d >>= 1) {
+            const float ov = __shfl_xor(bv, d);
+            const int oi = __shfl_xor(bi, d);
+            if (ahead(ov, oi, bv, bi)) bv = ov, bi = oi;
+        }
+        if (bi != kNoIndex && bi / VE % G == g) open &= ~(1u << (bi / (VE * G) * VE + bi % VE));
+        if (g == 0) write_top(a, row, i, v, bi == kNoIndex ? 0 : rank_key(bv, bi));
+    }
 }
 
 // Longer rows: W waves a row, one pass. A wave takes tiles of 64 lanes x 2 16-byte vectors (any
@@ -369,7 +412,7 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
             sum.w = e0 * __builtin_fmaf(-off, sum.s, sum.w);
             sum.s *= e0;
         }
-        sum = join_lanes<64>(sum, a.c);
+        sum = join_wave(sum, a.c);
         if (TOP) top.select();
     }
     if (W > 1) {
@@ -421,7 +464,7 @@ __global__ __launch_bounds__(256) void score_join_kernel(ScoreArgs a) {
     const float *part = a.parts + (row * a.slices + min(lane, a.slices - 1)) * (3 + 2 * a.k);
     const bool on = lane < a.slices;
     Sums sum = {on ? part[0] : neg_inf(), on ? part[1] : 0.0f, on ? part[2] : 0.0f};
-    sum = join_lanes<64>(sum, a.c);
+    sum = join_wave(sum, a.c);
     if (lane == 0) write_row(a, row, tok, lt, sum);
     if (a.k == 0) return;
     TopBuf top = {top_s[threadIdx.x >> 6], 0, a.k};
@@ -452,7 +495,7 @@ struct GradArgs {
 
 // d logit = (g (1[token] - p) - h p (log p + entropy)) / temperature; L lanes a row, 16 bytes each. With
 // y = log2 p: -p (A + B y) of the row's A = g + h entropy and B = h ln 2, and g more at the token.
-template <typename T, bool STREAM>
+template <typename T, bool STREAM, int U>
 __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     constexpr int VE = 16 / sizeof(T);
     const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -461,8 +504,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     const bool padded = tok < 0;
     const T *l = (const T *)a.logits + row * a.stride;
     T *d = (T *)a.d_logits + row * a.d_stride;
-    // all of the block's logits on their way before the row's numbers are waited for
-    constexpr int U = 4;
+    // U vectors on their way before the row's numbers are waited for
     const int v0 = blockIdx.y * a.span, v1 = min(a.vocab, v0 + a.span);
     for (int i0 = v0 + threadIdx.x % L * VE; i0 < v1; i0 += U * L * VE) {
         T x[U][VE] = {};
@@ -541,9 +583,9 @@ int slices_of(int64_t rows, int64_t vocab, int dtype, int *len) {
 template <typename T>
 void launch_score(const ScoreArgs &a, hipStream_t s) {
     auto blocks = [&](int per) { return (unsigned)((a.rows + per - 1) / per); };
-    if (a.vocab <= 32) score_small_kernel<T, 4, 8><<<blocks(64), 256, 0, s>>>(a);
-    else if (a.vocab <= 128) score_small_kernel<T, 16, 8><<<blocks(16), 256, 0, s>>>(a);
-    else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64, 8><<<blocks(4), 256, 0, s>>>(a);
+    if (a.vocab <= 32) score_small_kernel<T, 4><<<blocks(64), 256, 0, s>>>(a);
+    else if (a.vocab <= 128) score_small_kernel<T, 16><<<blocks(16), 256, 0, s>>>(a);
+    else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64><<<blocks(4), 256, 0, s>>>(a);
     else if (a.slices == 1 && (a.vocab <= 8192 || (a.k > 0 && a.rows >= 2048))) {
         // a wave a row: short rows, and rows enough to fill the card where a search for alternatives begins
         // and ends in every wave (4096 x 131071, 8 alternatives: 284 us, four waves a row 308 us; without
@@ -571,8 +613,14 @@ void launch_grad(GradArgs a, hipStream_t s) {
     // logits and gradient beyond the 256 MB last-level cache: stores past it (4096 x 32768 bf16 102 us for
     // 153), else the gradient stays there for what reads it next
     const dim3 grid((unsigned)blocks, (unsigned)ny);
-    if (a.rows * a.vocab * (int64_t)sizeof(T) > (128LL << 20)) score_grad_kernel<T, true><<<grid, 256, 0, s>>>(a, L);
-    else score_grad_kernel<T, false><<<grid, 256, 0, s>>>(a, L);
+    const bool past = a.rows * a.vocab * (int64_t)sizeof(T) > (128LL << 20);
+    if (L * VE >= a.vocab) {
+        if (past) score_grad_kernel<T, true, 1><<<grid, 256, 0, s>>>(a, L);
+        else score_grad_kernel<T, false, 1><<<grid, 256, 0, s>>>(a, L);
+    } else {
+        if (past) score_grad_kernel<T, true, 4><<<grid, 256, 0, s>>>(a, L);
+        else score_grad_kernel<T, false, 4><<<grid, 256, 0, s>>>(a, L);
+    }
 }
 
 int check_rows(const char *who, int dtype, int64_t rows, int64_t vocab, int64_t stride, float temperature) {
