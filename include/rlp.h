@@ -657,8 +657,7 @@ int rlp_sac_update(const rlp_sac_nets *nets, const rlp_sac_cfg *cfg, const float
  * lengths [B] i32 device (nullable): tokens of each sequence, clamped to [0, T]; rows behind them
  * are not read, their outputs and gradients are 0.
  * state / state_out [B][H][Dk][Dv] f32 contiguous (nullable): the state before the first token (0)
- * and behind the last one. State and sums are f32 whatever dtype is. No atomics: run-to-run
- * identical. */
+ * and behind the last one. State and sums are f32 whatever dtype is; run-to-run identical. */
 typedef struct rlp_la_cfg {
     int32_t dtype;             /* of q, k, v, out and their gradients */
     int32_t B, T, H, Hq, Hk, Hv, Dk, Dv;

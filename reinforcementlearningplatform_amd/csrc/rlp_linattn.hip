@@ -722,6 +722,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                         zs[16 * it + 4 * q + r][col] = (unsigned short)o;
                         zs[16 * it + 4 * q + r + 1][col] = (unsigned short)(o >> 16);
                     }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // lanes read what other lanes wrote
                 const int row = lane >> 1, c = c0 + (lane & 1) * 8;
                 __bf16 *o = (__bf16 *)a.out + out0 + (pos + row) * dir * a.ot + c;
 #pragma unroll

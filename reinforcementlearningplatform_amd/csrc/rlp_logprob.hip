@@ -6,8 +6,9 @@
 //   logp = ln 2 (y_token - log2 s),   entropy = ln 2 (log2 s - w / s).
 // In the loops y is one fma, l c - rnd(m c) with c = log2(e) / temperature: a logit's product is exact
 // inside it, and what rounding m c put into every y alike (m c - rnd(m c)) is taken out of the sums at
-// the end, so large logits lose nothing. Where l c could overflow (|m| >= 1e30: a row of the type's lowest
-// values, which is the uniform row it should be) y is formed from the difference l - m. Sums are f32.
+// the end, so large logits lose nothing. Where m c is beyond 1e6 (a row of the type's lowest values, which
+// is the uniform row it should be; a temperature near 0) y is formed from the difference l - m. Sums are
+// f32.
 #include "rlp_common.hpp"
 
 namespace rlp {
@@ -53,10 +54,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // y = l c - mc of the logits of a row with maximum m; off: what is in every y beside (l - m) c
 struct Shift {
     float mc, off;
-    bool far;  // m c may overflow: (l - m) c instead
+    bool far;  // m c is large, its rounding too, or overflows: (l - m) c instead
     __device__ __forceinline__ Shift(float m, float c) {
-        far = !(fabsf(m) < 1e30f);
         mc = m * c;
+        far = !(fabsf(m) < 1e30f && fabsf(mc) < 1e6f);
         off = far ? 0.0f : __builtin_fmaf(m, c, -mc);
     }
 };
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
             {
                 const float m = fmaxf(sum.m, tm), base = base_of(m);
                 const Shift sh(base, a.c);
-                // the sums so far move to the new maximum (far: mc is infinite on both sides)
+                // the sums so far move to the new maximum (far: mc may be infinite)
                 const float y0 = sum.m == neg_inf() ? neg_inf() : sh.far ? (sum.m - base) * a.c : mc - sh.mc;
                 const float e0 = __builtin_amdgcn_exp2f(y0);
                 sum.w = e0 * __builtin_fmaf(fmaxf(y0, -200.0f), sum.s, sum.w);

@@ -757,3 +757,45 @@ def test_la_nan_decay_shows(K, dtype):
     s["ld"][1] = float("nan")
     out = K.linear_attention(*[s[n].cuda() for n in "qkv"], s["ld"].cuda())
     assert torch.isnan(out[0, 1:, 1]).all() and torch.isfinite(out[:, :, 0]).all()
+
+
+@pytest.mark.parametrize("V", [18, 300, 5000, 40000])
+@pytest.mark.parametrize("shift, temperature", [(1e4, 0.7), (-1e4, 1.0), (0.0, 1e-3), (0.0, 1e3), (1e6, 1e-20)])
+def test_lp_large_logits_and_temperatures(K, V, shift, temperature):
+    """Logits far from 0 lose nothing but their own rounding; cold and hot distributions."""
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn(5, V, generator=g) * 3 + shift
+    tokens = logits.argmax(-1) if temperature < 1e-10 else torch.randint(0, V, (5,), generator=g)
+    if temperature < 1e-10:   # all but the largest at no probability: logp 0, entropy 0
+        first = logits == logits.amax(-1, keepdim=True)
+        logits = torch.where(first.cumsum(-1) * first == 1, logits, logits - 1.0)
+        res = K.token_logprob(logits.cuda(), tokens.cuda(), temperature=temperature, top_k=1)
+        assert (res[0] == 0).all() and (res[1] == 0).all() and torch.equal(res[3].cpu()[:, 0], tokens)
+    else:
+        lp_check(K, logits, tokens, temperature=temperature, k=min(V, 6))
+
+
+def test_sequence_operators_in_two_threads(K):
+    """Calls from two threads at once, on streams of their own."""
+    import threading
+    s = la_inputs(1, 700, 2, (2, 2, 2), 32, 32, BF16, seed=51)
+    ins, ld = [s[n].cuda() for n in "qkv"], s["ld"].cuda()
+    x = torch.randn(5, 30000, device="cuda")
+    t = torch.arange(5, device="cuda")
+    want = K.linear_attention(*ins, ld), K.token_logprob(x, t, top_k=5)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                o, r = K.linear_attention(*ins, ld), K.token_logprob(x, t, top_k=5)
+                torch.cuda.current_stream().synchronize()
+                if not (torch.equal(o, want[0]) and all(torch.equal(a, b) for a, b in zip(r, want[1]))):
+                    bad.append(1)
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not bad
