@@ -160,6 +160,10 @@ __device__ __forceinline__ floatx4 mfma_f32(float a, float b, floatx4 c) {
 // operand one value of row q of four. With the order of a contraction free, register r of an
 // accumulator is the operand of rows q -> 4 q + r as it stands: S goes from accumulator to operand
 // without leaving its wave, and so does P, computed transposed as Y X^T and shared out over the waves.
+//
+// Bound by HBM where the state is small (4096 x 4 sequences of 64 tokens, 64 x 64: 1.6 GB in 343 us,
+// 4.7 TB/s), by the f32 matrix rate at 128 x 128 (16 x 16 of 4096: 858 us for 2.15 GB). 32 columns a wave
+// with 32x32 products, at one wave a SIMD, took 1210 us for the former.
 template <typename T, int DXB, int NW>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_kernel(WalkArgs a) {
     constexpr int C = 32, DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW;
@@ -506,6 +510,10 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 //
 // 16 columns a wave, not 32: with 32x32 tiles at two waves a SIMD the same work waited on LDS and on
 // its own products (9 us a chunk of 128 x 128); half the registers a wave let four waves run.
+//
+// Bound by issue: of the cycles of 16 sequences of 65536 tokens, 128 x 128 (outputs in 278 us for 1.07 GB),
+// vector instructions take 44 % and matrix instructions 28 %, and they seldom run at once. The check for
+// infs and NaNs is 2 % of it, the second piece of S 5 %.
 template <int DXB, int NW, int PZ, int C>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
     constexpr int CT = C / 16, NP = CT * (CT + 1) / 2, SLOTS = C == 64 ? 6 : 2;  // token tiles, P's, their operands
@@ -913,8 +921,9 @@ constexpr int kMaxD = 128;
 
 // A sequence is split where batch x heads leave most CUs idle, into as many segments as fill the card
 // with the two blocks a CU holds at D = 128. A segment has 256 tokens at least, so that its state's way
-// through memory stays below the walk. The split walk reads y and z twice: with 384 sequences of up to
-// 2047 tokens it took 425 us, the whole walk 290 us (128 x 128 bf16).
+// through memory stays below the walk. The split walk reads y and z twice: 384 sequences of up to 2047
+// tokens took 322 us in two parts each, 236 us whole (128 x 128 bf16); 16 of 65536 tokens 504 us in 512
+// blocks, 571 in 256 and 535 in 768.
 int segments(int64_t bh, int T, int *seglen) {
     *seglen = T > 0 ? T : 1;
     if (bh < 1 || bh > 128 || T < 512) return 1;
