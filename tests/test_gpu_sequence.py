@@ -184,6 +184,16 @@ def la_check_values(K, s):
                                                   [s["d_out"].cuda(), s["d_state"].cuda()]))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B, H", [(2, 257), (3, 100), (5, 100), (25, 12), (42, 12), (64, 5), (64, 30), (65, 8)])
+def test_la_ragged_batches(K, dtype, B, H):
+    """Orders of the blocks by length: each sequence is walked once, also of equal, empty and odd lengths."""
+    g = torch.Generator().manual_seed(B * H)
+    for lengths in (torch.randint(0, 41, (B,), generator=g), torch.randint(0, 2, (B,), generator=g) * 33,
+                    torch.full((B,), 40)):
+        la_check(K, la_inputs(B, 40, H, (H, H, H), 7, 9, dtype, seed=B, lengths=lengths.tolist(), reset=0.02))
+
+
 def test_la_lengths_are_clamped(K):
     s = la_inputs(2, 40, 1, (1, 1, 1), 8, 8, F32, seed=2, lengths=[-3, 1000])
     out, last = K.linear_attention(*[s[n].cuda() for n in "qkv"], s["ld"].cuda(), state=s["state"].cuda(),
