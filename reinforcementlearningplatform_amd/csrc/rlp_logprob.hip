@@ -566,6 +566,16 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
 // ------------------------------------------------------------------------------------------
 constexpr int kSmallVocab = 512;
 
+// Rows a block takes: 256 threads over the lanes of a row. A launch has at most 2^24 - 1 such blocks (2^32 - 1
+// threads along x).
+bool rows_fit(int64_t rows, int lanes) { return rows * lanes <= 256LL * ((1 << 24) - 1); }
+int score_lanes(int64_t vocab) { return vocab <= 32 ? 4 : vocab <= 128 ? 16 : vocab <= 8192 ? 64 : 256; }
+int grad_lanes(int64_t vocab, int dtype) {
+    int L = 1;
+    while (L < 256 && L * (dtype == RLP_F32 ? 4 : 8) < vocab) L *= 2;
+    return L;
+}
+
 // Few long rows: each over several blocks of at least one tile per wave.
 int slices_of(int64_t rows, int64_t vocab, int dtype, int *len) {
     *len = (int)vocab;
@@ -604,8 +614,7 @@ void launch_score(const ScoreArgs &a, hipStream_t s) {
 template <typename T>
 void launch_grad(GradArgs a, hipStream_t s) {
     constexpr int VE = 16 / sizeof(T);
-    int L = 1;
-    while (L < 256 && L * VE < a.vocab) L *= 2;
+    const int L = grad_lanes(a.vocab, VE == 4 ? RLP_F32 : RLP_BF16);
     const int64_t blocks = (a.rows + 256 / L - 1) / (256 / L);
     // a block takes 4 vectors a lane of a long row; at most 65535 blocks in y
     a.span = 256 * VE * 4;
@@ -663,6 +672,8 @@ int rlp_token_logprob(const void *logits, int dtype, int64_t rows, int64_t vocab
     if (rows == 0) return RLP_OK;
     RLP_REQUIRE(logits && tokens && logp && entropy && (top_k == 0 || (top_logp && top_tokens)),
                 "rlp_token_logprob: null argument");
+    RLP_REQUIRE(rows_fit(rows, score_lanes(vocab)), "rlp_token_logprob: %lld rows of %lld logits are too many for one launch",
+                (long long)rows, (long long)vocab);
     const int64_t need = rlp_token_logprob_workspace_bytes(rows, vocab, top_k, dtype);
     RLP_REQUIRE(need == 0 || (workspace && workspace_bytes >= need),
                 "rlp_token_logprob: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
@@ -691,6 +702,9 @@ int rlp_token_logprob_backward(const void *logits, int dtype, int64_t rows, int6
     RLP_REQUIRE(rows <= 1 || d_row_stride >= vocab, "rlp_token_logprob_backward: rows of d_logits overlap");
     if (rows == 0) return RLP_OK;
     RLP_REQUIRE(logits && tokens && stats && d_logits, "rlp_token_logprob_backward: null argument");
+    RLP_REQUIRE(rows_fit(rows, grad_lanes(vocab, dtype)),
+                "rlp_token_logprob_backward: %lld rows of %lld logits are too many for one launch", (long long)rows,
+                (long long)vocab);
     GradArgs a = {};
     a.logits = logits, a.d_logits = d_logits, a.rows = rows, a.stride = row_stride, a.d_stride = d_row_stride;
     a.vocab = (int)vocab, a.tokens = tokens;

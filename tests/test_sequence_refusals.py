@@ -152,3 +152,15 @@ def test_token_logprob_wrapper_refusals():
             ((l.double(), t), {}, "GPU|dtype")]:
         with pytest.raises(RLPError, match=word):
             K.token_logprob(*args, **kw)
+
+
+@pytest.mark.parametrize("vocab, rows", [(18, 1 << 30), (100, 1 << 28), (600, 1 << 26), (40000, 1 << 24)])
+def test_token_logprob_rows_of_one_launch(vocab, rows):
+    """A launch has fewer than 2^32 threads along an axis; more rows are refused."""
+    lib = _native.lib()
+    assert lib.rlp_token_logprob(DEV, _abi.RLP_F32, rows, vocab, vocab, DEV, 1.0, 0, DEV, DEV, None, None, None,
+                                 None, 0, None) == _abi.RLP_EINVAL
+    assert b"rows" in lib.rlp_last_error_string() and b"launch" in lib.rlp_last_error_string()
+    assert lib.rlp_token_logprob_backward(DEV, _abi.RLP_F32, rows, vocab, vocab, DEV, 1.0, DEV, DEV, DEV, DEV,
+                                          vocab, None) == _abi.RLP_EINVAL
+    assert b"launch" in lib.rlp_last_error_string()
