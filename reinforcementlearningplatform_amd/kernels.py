@@ -515,9 +515,12 @@ def sac_update(nets, cfg, s, a, r, s_next, dw, noise, work, losses):
 _DTYPES = {torch.float32: _abi.RLP_F32, torch.float16: _abi.RLP_F16, torch.bfloat16: _abi.RLP_BF16}
 
 
-# torch.cuda.current_device / current_stream without their Python (3 us a call, 15 in a backward thread)
+# torch.cuda.current_device / current_stream without their Python (3 us a call, 15 in a backward thread),
+# and two more of torch's own short ways
 _device_index = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream
+_increment_version = torch._C._increment_version
+_same_storage = torch._C._is_alias_of
 
 
 def _one_device(what, *tensors):
@@ -547,6 +550,15 @@ def _rows(x):
     return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
 
 
+def _overlaps(a, b):
+    """Whether the memory that a and b span has bytes in common."""
+    if not _same_storage(a, b):
+        return False
+    ends = [t.data_ptr() + t.element_size() * (1 + sum((n - 1) * d for n, d in zip(t.shape, t.stride())))
+            for t in (a, b)]
+    return a.numel() > 0 and b.numel() > 0 and a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
 def _like_order(ref, B, T, H, D):
     """An empty [B][T][H][D] tensor in ref's order of the batch and token axes (rollout buffers are
     time-major)."""
@@ -565,16 +577,20 @@ def _la_workspace_bytes(what, backward, *dims):
     return need
 
 
-def _la_dims(what, q, k, v, log_decay, state):
-    """(dtype, B, T, H, Hq, Hk, Hv, Dk, Dv) of q, k, v [B][T][heads][D]."""
+def _la_dims(what, q, k, v, log_decay, state, axes=4):
+    """(dtype, B, T, H, Hq, Hk, Hv, Dk, Dv) of q, k, v [B][T][heads][D], of three axes [B][heads][D]."""
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
+        if t.dim() != axes:
             raise RLPError(f"{what}: {name} of {t.dim()} axes")
         if t.dtype != q.dtype:
             raise RLPError(f"{what}: {name} is {t.dtype}, q {q.dtype}")
     if q.dtype not in _DTYPES:
         raise RLPError(f"{what}: dtype {q.dtype} (float32, float16 or bfloat16)")
-    (B, T, Hq, Dk), (Bk, Tk, Hk, Dk2), (Bv, Tv, Hv, Dv) = q.shape, k.shape, v.shape
+    if axes == 4:
+        (B, T, Hq, Dk), (Bk, Tk, Hk, Dk2), (Bv, Tv, Hv, Dv) = q.shape, k.shape, v.shape
+    else:
+        (B, Hq, Dk), (Bk, Hk, Dk2), (Bv, Hv, Dv) = q.shape, k.shape, v.shape
+        T = Tk = Tv = 1
     if B != Bk or B != Bv or T != Tk or T != Tv or Dk != Dk2:
         raise RLPError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if log_decay.dim() != 1 or log_decay.dtype != torch.float32:
@@ -706,20 +722,19 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, len
 def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, state_out=None, out=None):
     """linear_attention for one token of every sequence, for acting: q, k [B][heads][Dk],
     v [B][heads][Dv], state float32 [B][H][Dk][Dv] contiguous, updated in place or written to state_out;
-    reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv]. Not differentiable."""
+    reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv] (in `out`, apart from the other
+    arguments, where given). Not differentiable."""
     what = "linear_attention_step"
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     log_decay.requires_grad or state.requires_grad):
         raise RLPError(f"{what}: not differentiable (call it under torch.no_grad, or linear_attention)")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 3:
-            raise RLPError(f"{what}: {name} of {t.dim()} axes")
-    dims = _la_dims(what, q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), log_decay, state)
+    dims = _la_dims(what, q, k, v, log_decay, state, 3)
     _la_workspace_bytes(what, 0, *dims)
     _, B, _, H, _, _, _, Dk, Dv = dims
     reset, _ = _la_flags(what, reset, None, (B,), B)
     if not state.is_contiguous():
         raise RLPError(f"{what}: state and state_out have to be contiguous")
+    written = []
     if state_out is None:
         state_out = state
     elif state_out is not state:
@@ -727,13 +742,21 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, sta
             raise RLPError(f"{what}: state_out {state_out.dtype} {tuple(state_out.shape)}")
         if not state_out.is_contiguous():
             raise RLPError(f"{what}: state and state_out have to be contiguous")
-        apart = abs(state_out.data_ptr() - state.data_ptr())
-        if 0 < apart < 4 * state.numel():
+        if state_out.data_ptr() != state.data_ptr() and _overlaps(state_out, state):
             raise RLPError(f"{what}: state_out overlaps state (pass state itself for an update in place)")
+        written.append(("state_out", state_out))
     if out is None:
         out = q.new_empty((B, H, Dv))
-    elif out.shape != (B, H, Dv) or out.dtype != q.dtype or not out.is_contiguous():
-        raise RLPError(f"{what}: out {out.dtype} {tuple(out.shape)}, contiguous {q.dtype} {(B, H, Dv)} needed")
+    else:
+        if out.shape != (B, H, Dv) or out.dtype != q.dtype or not out.is_contiguous():
+            raise RLPError(f"{what}: out {out.dtype} {tuple(out.shape)}, contiguous {q.dtype} {(B, H, Dv)} needed")
+        written.append(("out", out))
+    for name, t in written:  # blocks of other columns and heads read the inputs while these are written
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RLPError(f"{what}: {name} wants a gradient (call it under torch.no_grad)")
+        for other in (q, k, v, log_decay, reset) + ((state, state_out) if t is out else ()):
+            if other is not None and _overlaps(t, other):
+                raise RLPError(f"{what}: {name} overlaps another argument")
     _one_device(what, q, k, v, log_decay, state, state_out, reset, out)
     q, k, v, log_decay = _rows(q), _rows(k), _rows(v), log_decay.contiguous()
     cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale,
@@ -743,6 +766,8 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, sta
     _launch(what, q.get_device(), lib().rlp_linear_attention_step, cfg,
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _at(reset), state.data_ptr(),
             state_out.data_ptr(), out.data_ptr())
+    # autograd's saved tensors: a backward that was to read the old state raises instead of using the new one
+    _increment_version((state_out, out))
     return out
 
 

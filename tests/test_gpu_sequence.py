@@ -427,6 +427,16 @@ def test_la_step_drops_nan_and_takes_slices(K):
     assert K.linear_attention_step(q[:0], k[:0], v[:0], s["ld"].cuda(), st[:0]).shape == (0, 2, 16)
 
 
+def test_la_step_invalidates_saved_states(K):
+    """A backward that saved a state which a step then updated in place raises."""
+    s = la_inputs(2, 5, 2, (2, 2, 2), 8, 8, F32, seed=11)
+    q, k, v, st = (s[n].cuda() for n in ("q", "k", "v", "state"))
+    out = K.linear_attention(q.requires_grad_(), k, v, s["ld"].cuda(), state=st)
+    K.linear_attention_step(q.detach()[:, 0], k[:, 0], v[:, 0], s["ld"].cuda(), st)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
 def test_la_step_graph(K):
     s = la_inputs(2, 1, 2, (2, 2, 2), 64, 64, BF16, seed=13)
     q, k, v = (s[n][:, 0].cuda() for n in "qkv")

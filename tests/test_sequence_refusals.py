@@ -164,3 +164,23 @@ def test_token_logprob_rows_of_one_launch(vocab, rows):
     assert lib.rlp_token_logprob_backward(DEV, _abi.RLP_F32, rows, vocab, vocab, DEV, 1.0, DEV, DEV, DEV, DEV,
                                           vocab, None) == _abi.RLP_EINVAL
     assert b"launch" in lib.rlp_last_error_string()
+
+
+def test_step_refuses_outputs_over_its_inputs():
+    q, k, v = (torch.zeros(3, 2, 8) for _ in range(3))
+    ld, mem, reset = torch.zeros(2), torch.zeros(3, 2, 8, 8), torch.zeros(3, dtype=torch.uint8)
+    big = torch.zeros(2 * mem.numel())
+    for over in (dict(out=q), dict(out=k), dict(out=v), dict(out=mem[0, 0].view(-1)[:48].view(3, 2, 8)),
+                 dict(state_out=q.new_zeros(0).set_(q.untyped_storage()).resize_(3, 2, 8, 8))):
+        with pytest.raises(RLPError, match="overlaps"):
+            K.linear_attention_step(q, k, v, ld, mem, reset, **over)
+    one = big[:mem.numel()].view_as(mem)
+    with pytest.raises(RLPError, match="overlaps state"):
+        K.linear_attention_step(q, k, v, ld, one, state_out=big[4:4 + mem.numel()].view_as(mem))
+    for name in ("out", "state_out"):
+        t = torch.zeros(3, 2, 8) if name == "out" else torch.zeros_like(mem)
+        with pytest.raises(RLPError, match="gradient"):
+            K.linear_attention_step(q, k, v, ld, mem, **{name: t.requires_grad_()})
+    # apart: on to the next check, of the device
+    with pytest.raises(RLPError, match="GPU"):
+        K.linear_attention_step(q, k, v, ld, one, state_out=big[mem.numel():].view_as(mem), out=torch.zeros(3, 2, 8))
