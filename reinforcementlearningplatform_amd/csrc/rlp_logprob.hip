@@ -26,6 +26,15 @@ __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
+// 16 bytes in one load at any element's address. Not as a memcpy, which might alias the stores: the gradient
+// of 4096 x 32769 bf16 logits took 110 us with it, 97 so.
+template <bool STREAM = false, typename T>
+__device__ __forceinline__ void take16(T *to, const T *from) {
+    const uintx4_any *p = (const uintx4_any *)from;
+    const uintx4_any v = STREAM ? __builtin_nontemporal_load(p) : *p;
+    __builtin_memcpy(to, &v, 16);
+}
+
 struct ScoreArgs {
     const void *logits;
     int64_t rows, stride;
@@ -213,7 +222,7 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
         T raw[VE];
         const int t0 = token(c);
         if (t0 + VE <= a.vocab) {
-            __builtin_memcpy(raw, l + t0, 16);
+            take16(raw, l + t0);
         } else {
 #pragma unroll
             for (int e = 0; e < VE; ++e) raw[e] = t0 + e < a.vocab ? l[t0 + e] : (T)neg_inf();
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
 // 4.5, for the waves that a CU no longer holds). Alternatives: each wave keeps its own list
 // and a lower bound of the row's k-th value, shared between the row's waves through LDS; a tile is
 // searched only where a vector's maximum reaches the bound.
-template <typename T, int W, bool TOP>
+template <typename T, int W, bool TOP, bool STREAM>
 __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
     constexpr int VE = 16 / sizeof(T), U = 2, TILE = 64 * VE * U;
     __shared__ float bound_s[4];
@@ -303,7 +312,9 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
     const int64_t tok = row < a.rows ? a.tokens[row] : -1;
     const bool padded = tok < 0;  // the same for all W waves of the row
     const T *l = (const T *)a.logits + row * a.stride;
-    const int v0 = slice * a.slice_len, v1 = min(a.vocab, v0 + a.slice_len);
+    // STREAM: vectors begin at multiples of 16 bytes, so the first may begin before the row
+    const int before = STREAM ? (uintptr_t)l / sizeof(T) % VE : 0, v0 = slice * a.slice_len - before;
+    const int v1 = slice == a.slices - 1 ? a.vocab : v0 + a.slice_len;
     float lt = 0.0f;
     if (!padded && tok < a.vocab) lt = to_f32(l[tok]);
     Sums sum = {neg_inf(), 0.0f, 0.0f};
@@ -316,11 +327,11 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = at + (u * 64 + lane) * VE;
-            if (i + VE <= v1) {
-                __builtin_memcpy(t[u], l + i, 16);
+            if ((!STREAM || i >= 0) && i + VE <= v1) {
+                take16<STREAM>(t[u], l + i);
             } else {
 #pragma unroll
-                for (int e = 0; e < VE; ++e) t[u][e] = i + e < v1 ? l[i + e] : (T)neg_inf();
+                for (int e = 0; e < VE; ++e) t[u][e] = (!STREAM || i + e >= 0) && i + e < v1 ? l[i + e] : (T)neg_inf();
             }
         }
     };
@@ -384,7 +395,7 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
                         for (int e = 0; e < VE; ++e) {
                             if (!__any(x[u][e] >= lv)) continue;
                             const int id = at + (u * 64 + lane) * VE + e;
-                            top.push(x[u][e] > lv || (x[u][e] == lv && id < li), rank_key(x[u][e], id));
+                            top.push(x[u][e] > lv || (x[u][e] == lv && (unsigned)id < (unsigned)li), rank_key(x[u][e], id));
                         }
                     }
                     if (top.n >= a.k + 8) {
@@ -496,7 +507,7 @@ struct GradArgs {
 
 // d logit = (g (1[token] - p) - h p (log p + entropy)) / temperature; L lanes a row, 16 bytes each. With
 // y = log2 p: -p (A + B y) of the row's A = g + h entropy and B = h ln 2, and g more at the token.
-template <typename T, bool STREAM, int U>
+template <typename T, bool STREAM, bool ALIGNED, int U>
 __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     constexpr int VE = 16 / sizeof(T);
     const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
@@ -506,18 +517,20 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
     const T *l = (const T *)a.logits + row * a.stride;
     T *d = (T *)a.d_logits + row * a.d_stride;
     // U vectors on their way before the row's numbers are waited for
-    const int v0 = blockIdx.y * a.span, v1 = min(a.vocab, v0 + a.span);
+    // ALIGNED: vectors begin at multiples of 16 bytes of d, so the first may begin before the row
+    const int before = ALIGNED ? (int)((uintptr_t)d / sizeof(T) % VE) : 0;
+    const int v0 = (int)blockIdx.y * a.span - before, v1 = min(a.vocab, v0 + a.span);
     for (int i0 = v0 + threadIdx.x % L * VE; i0 < v1; i0 += U * L * VE) {
         T x[U][VE] = {};
         if (!padded) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = i0 + u * L * VE;
-                if (i + VE <= v1) {
-                    __builtin_memcpy(x[u], l + i, 16);
+                if ((!ALIGNED || i >= 0) && i + VE <= v1) {
+                    take16(x[u], l + i);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) x[u][e] = i + e < v1 ? l[i + e] : (T)neg_inf();
+                    for (int e = 0; e < VE; ++e) x[u][e] = (!ALIGNED || i + e >= 0) && i + e < v1 ? l[i + e] : (T)neg_inf();
                 }
             }
         }
@@ -547,7 +560,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
             T r[VE];
 #pragma unroll
             for (int e = 0; e < VE; ++e) r[e] = (T)(padded ? 0.0f : v[e]);
-            if (i + VE <= v1) {
+            if ((!ALIGNED || i >= 0) && i + VE <= v1) {
                 uintx4_any out;
                 __builtin_memcpy(&out, r, 16);
                 if (STREAM) __builtin_nontemporal_store(out, (uintx4_any *)(d + i));
@@ -555,7 +568,7 @@ __global__ __launch_bounds__(256) void score_grad_kernel(GradArgs a, int L) {
             } else {
 #pragma unroll
                 for (int e = 0; e < VE; ++e)
-                    if (i + e < v1) d[i + e] = r[e];
+                    if ((!ALIGNED || i + e >= 0) && i + e < v1) d[i + e] = r[e];
             }
         }
     }
@@ -594,6 +607,12 @@ int slices_of(int64_t rows, int64_t vocab, int dtype, int *len) {
 template <typename T>
 void launch_score(const ScoreArgs &a, hipStream_t s) {
     auto blocks = [&](int per) { return (unsigned)((a.rows + per - 1) / per); };
+    // logits of twice the 256 MB last-level cache and more: loads past it and aligned, as vectors over two cache
+    // lines cost time then (bf16, 4096 x 131071 254 -> 205 us, with 8 alternatives 268 -> 213; 16384 x 32769
+    // 226 -> 177). Fewer stay in the cache for the gradient, and are summed in an order that does not
+    // depend on a row's address.
+    const bool past = a.rows * a.vocab * (int64_t)sizeof(T) > (512LL << 20);
+    auto rows = [&](auto kept, auto stream, dim3 grid) { (past ? stream : kept)<<<grid, 256, 0, s>>>(a); };
     if (a.vocab <= 32) score_small_kernel<T, 4><<<blocks(64), 256, 0, s>>>(a);
     else if (a.vocab <= 128) score_small_kernel<T, 16><<<blocks(16), 256, 0, s>>>(a);
     else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64><<<blocks(4), 256, 0, s>>>(a);
@@ -601,12 +620,12 @@ void launch_score(const ScoreArgs &a, hipStream_t s) {
         // a wave a row: short rows, and rows enough to fill the card where a search for alternatives begins
         // and ends in every wave (4096 x 131071, 8 alternatives: 284 us, four waves a row 308 us; without
         // alternatives 4096 x 32768 takes 56 us so and 50 us with four)
-        if (a.k) score_rows_kernel<T, 1, true><<<blocks(4), 256, 0, s>>>(a);
-        else score_rows_kernel<T, 1, false><<<blocks(4), 256, 0, s>>>(a);
+        if (a.k) rows(score_rows_kernel<T, 1, true, false>, score_rows_kernel<T, 1, true, true>, blocks(4));
+        else rows(score_rows_kernel<T, 1, false, false>, score_rows_kernel<T, 1, false, true>, blocks(4));
     } else {
         const dim3 grid((unsigned)a.rows, a.slices);
-        if (a.k) score_rows_kernel<T, 4, true><<<grid, 256, 0, s>>>(a);
-        else score_rows_kernel<T, 4, false><<<grid, 256, 0, s>>>(a);
+        if (a.k) rows(score_rows_kernel<T, 4, true, false>, score_rows_kernel<T, 4, true, true>, grid);
+        else rows(score_rows_kernel<T, 4, false, false>, score_rows_kernel<T, 4, false, true>, grid);
         if (a.slices > 1) score_join_kernel<T><<<blocks(4), 256, 0, s>>>(a);
     }
 }
@@ -618,18 +637,22 @@ void launch_grad(GradArgs a, hipStream_t s) {
     const int64_t blocks = (a.rows + 256 / L - 1) / (256 / L);
     // a block takes 4 vectors a lane of a long row; at most 65535 blocks in y
     a.span = 256 * VE * 4;
-    int64_t ny = ((int64_t)a.vocab + a.span - 1) / a.span;
-    while (ny > 65535) a.span *= 2, ny = ((int64_t)a.vocab + a.span - 1) / a.span;
+    const int64_t most = (int64_t)a.vocab + VE - 1;  // with what lies before the row
+    int64_t ny = (most + a.span - 1) / a.span;
+    while (ny > 65535) a.span *= 2, ny = (most + a.span - 1) / a.span;
     // logits and gradient beyond the 256 MB last-level cache: stores past it (4096 x 32768 bf16 102 us for
-    // 153), else the gradient stays there for what reads it next
+    // 153), else the gradient stays there for what reads it next. Twice that and more also aligned, where a row's
+    // ends cost less than vectors over two cache lines (16384 x 32769 bf16 450 us for 483; 4096 x 32769 97 for 96)
     const dim3 grid((unsigned)blocks, (unsigned)ny);
-    const bool past = a.rows * a.vocab * (int64_t)sizeof(T) > (128LL << 20);
+    const int64_t bytes = a.rows * a.vocab * (int64_t)sizeof(T);
+    const bool past = bytes > (128LL << 20);
     if (L * VE >= a.vocab) {
-        if (past) score_grad_kernel<T, true, 1><<<grid, 256, 0, s>>>(a, L);
-        else score_grad_kernel<T, false, 1><<<grid, 256, 0, s>>>(a, L);
+        if (past) score_grad_kernel<T, true, false, 1><<<grid, 256, 0, s>>>(a, L);
+        else score_grad_kernel<T, false, false, 1><<<grid, 256, 0, s>>>(a, L);
     } else {
-        if (past) score_grad_kernel<T, true, 4><<<grid, 256, 0, s>>>(a, L);
-        else score_grad_kernel<T, false, 4><<<grid, 256, 0, s>>>(a, L);
+        if (bytes > (512LL << 20)) score_grad_kernel<T, true, true, 4><<<grid, 256, 0, s>>>(a, L);
+        else if (past) score_grad_kernel<T, true, false, 4><<<grid, 256, 0, s>>>(a, L);
+        else score_grad_kernel<T, false, false, 4><<<grid, 256, 0, s>>>(a, L);
     }
 }
 

@@ -544,6 +544,48 @@ def test_lp_many_rows(K, N, V):
     lp_check(K, logits, torch.randint(0, V, (N,), generator=g), k=8)
 
 
+@pytest.mark.parametrize("dtype, N, V", [(BF16, 8203, 32801), (F32, 4100, 32801), (F16, 530, 520003), (F32, 300000, 601)])
+@pytest.mark.parametrize("k", [0, 5])
+def test_lp_past_the_caches(K, dtype, N, V, k):
+    """More than 512 MB of logits, with rows at every alignment: some rows of one call against float64."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    flat = torch.empty(N * V + 1, dtype=dtype, device="cuda").normal_(0.0, 3.0, generator=g)
+    x = flat[1:].view(N, V)
+    x[N // 2] = float("-inf")
+    x[N // 2, 1] = 0.5
+    x[N // 3, :V // 2] = float("-inf")
+    pick = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, N // 3, N // 2, N - 2, N - 1])
+    tokens = torch.randint(0, V, (N,), device="cuda", generator=g)
+    tokens[5], tokens[N // 2] = -1, 1
+    x.requires_grad_()
+    res = K.token_logprob(x, tokens, top_k=k)
+    gl, ge = (torch.randn(N, device="cuda", generator=g) for _ in range(2))
+    d, = torch.autograd.grad(res[:2], [x], [gl, ge])
+    got = [r[pick.cuda()] for r in res] + [d[pick.cuda()]]
+    # the same rows by themselves: the small call is held against float64, the large one against it
+    rows = x.detach()[pick.cuda()].cpu()
+    own = lp_check(K, rows, tokens[pick.cuda()].cpu(), k=k, grads=False)
+    r = lp_plain(rows, tokens[pick.cuda()].cpu(), 1.0, k)
+    base = 2 * (V / 64 + 48 + 6 * torch.nan_to_num(r["spread"])) * U   # both calls' sums
+    fin = lambda t: torch.where(torch.isfinite(t), t.abs(), torch.zeros_like(t)).cpu().double()
+    same = lambda a, b, tol: (((a.detach().cpu().double() - b.detach().cpu().double()).abs() <= tol) | (a.cpu() == b.cpu())).all()
+    assert same(got[0], own[0], base + 12 * U * fin(own[0].detach()))
+    assert same(got[1], own[1], base * (2 + 2 * r["spread"]))
+    if k:
+        assert torch.equal(got[3], own[3])
+        assert same(got[2], own[2], base[:, None] + 12 * U * fin(own[2].detach()))
+    s = K.token_logprob_forward(x.detach()[pick.cuda()], tokens[pick.cuda()])[2]
+    d_own = K.token_logprob_backward(gl[pick.cuda()], ge[pick.cuda()], x.detach()[pick.cuda()], tokens[pick.cuda()], s)
+    p, z = r["p"], torch.where(r["p"] > 0, r["z"].abs(), torch.zeros_like(r["z"]))
+    hot = torch.zeros_like(p).scatter_(1, r["at"][:, None], 1.0)
+    a, b = (t[pick.cuda()].cpu().double().abs()[:, None] for t in (gl, ge))
+    terms = a * (hot + p) + b * p * (z + r["entropy"][:, None] + 1)
+    tol = torch.finfo(dtype).eps * d_own.cpu().double().abs() + \
+        2 * (base[:, None] + 6 * U * (z + 2)) * terms + (2.0 ** -24 if dtype == F16 else 2.0 ** -126)
+    assert same(got[-1], d_own, tol)
+    assert (got[-1][5] == 0).all() and int((d[6] != 0).sum()) > 0
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [7, 100, 400, 3000, 30000])
 def test_lp_masks(K, dtype, V):
