@@ -200,11 +200,12 @@ __device__ __forceinline__ float about_kth(float x, int k) {
     return __uint_as_float(lo & 0x80000000u ? lo ^ 0x80000000u : ~lo);
 }
 
-// Rows of up to 8 G logits, G lanes a row, all of it in registers: every lane a 16-byte vector (f32: two,
-// G vectors apart) at any alignment.
-template <typename T, int G>
+// Rows of up to E G logits, G lanes a row, all of it in registers: 16-byte vectors at any alignment, a lane's
+// G vectors apart. Bound by instructions from 129 logits on, most of them the lanes' sums and the results,
+// which a few rows a wave share: 2^20 rows of 300 bf16 logits in 219 us with 16 lanes a row, 412 with 64.
+template <typename T, int G, int E = 8>
 __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
-    constexpr int E = 8, VE = 16 / sizeof(T);
+    constexpr int VE = 16 / sizeof(T);
     const int g = threadIdx.x % G;
     auto token = [&](int i) { return ((i / VE) * G + g) * VE + i % VE; };  // of the lane's i-th logit
     const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
@@ -221,7 +222,10 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
     for (int c = 0; c < E; c += VE) {
         T raw[VE];
         const int t0 = token(c);
-        if (t0 + VE <= a.vocab) {
+        if (E > 8 && c * G >= a.vocab) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) raw[e] = (T)neg_inf();
+        } else if (t0 + VE <= a.vocab) {
             take16(raw, l + t0);
         } else {
 #pragma unroll
@@ -238,10 +242,14 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
     for (int d = G / 2; d > 0; d >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, d));
     const float base = base_of(v.m);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const float y = (x[e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
-        v.s += p;
-        v.w += p * fmaxf(y, -200.0f);
+    for (int c = 0; c < E; c += VE) {
+        if (E > 8 && c * G >= a.vocab) break;
+#pragma unroll
+        for (int e = c; e < c + VE; ++e) {
+            const float y = (x[e] - base) * a.c, p = __builtin_amdgcn_exp2f(y);
+            v.s += p;
+            v.w += p * fmaxf(y, -200.0f);
+        }
     }
 #pragma unroll
     for (int d = G / 2; d > 0; d >>= 1) {
@@ -582,7 +590,7 @@ constexpr int kSmallVocab = 512;
 // Rows a block takes: 256 threads over the lanes of a row. A launch has at most 2^24 - 1 such blocks (2^32 - 1
 // threads along x).
 bool rows_fit(int64_t rows, int lanes) { return rows * lanes <= 256LL * ((1 << 24) - 1); }
-int score_lanes(int64_t vocab) { return vocab <= 32 ? 4 : vocab <= 128 ? 16 : vocab <= 8192 ? 64 : 256; }
+int score_lanes(int64_t vocab) { return vocab <= 8192 ? 64 : 256; }
 int grad_lanes(int64_t vocab, int dtype) {
     int L = 1;
     while (L < 256 && L * (dtype == RLP_F32 ? 4 : 8) < vocab) L *= 2;
@@ -613,8 +621,10 @@ void launch_score(const ScoreArgs &a, hipStream_t s) {
     // depend on a row's address.
     const bool past = a.rows * a.vocab * (int64_t)sizeof(T) > (512LL << 20);
     auto rows = [&](auto kept, auto stream, dim3 grid) { (past ? stream : kept)<<<grid, 256, 0, s>>>(a); };
-    if (a.vocab <= 32) score_small_kernel<T, 4><<<blocks(64), 256, 0, s>>>(a);
-    else if (a.vocab <= 128) score_small_kernel<T, 16><<<blocks(16), 256, 0, s>>>(a);
+    if (a.vocab <= 32) score_small_kernel<T, 2, 16><<<blocks(128), 256, 0, s>>>(a);
+    else if (a.vocab <= 128) score_small_kernel<T, 4, 32><<<blocks(64), 256, 0, s>>>(a);
+    else if (a.vocab <= 256 && a.k <= 2) score_small_kernel<T, 8, 32><<<blocks(32), 256, 0, s>>>(a);
+    else if (a.vocab <= kSmallVocab && a.k <= 2) score_small_kernel<T, 16, 32><<<blocks(16), 256, 0, s>>>(a);
     else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64><<<blocks(4), 256, 0, s>>>(a);
     else if (a.slices == 1 && (a.vocab <= 8192 || (a.k > 0 && a.rows >= 2048))) {
         // a wave a row: short rows, and rows enough to fill the card where a search for alternatives begins

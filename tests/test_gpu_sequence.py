@@ -650,6 +650,22 @@ def test_lp_ties(K, dtype, V, k):
     lp_check(K, logits, torch.randint(0, V, (6,), generator=g), k=k)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("V", [33, 64, 65, 128, 129, 256, 257, 300, 385, 511, 512])
+@pytest.mark.parametrize("k", [1, 2, 3])
+def test_lp_few_alternatives(K, dtype, V, k):
+    g = torch.Generator().manual_seed(V + k)
+    logits = torch.randint(-3, 3, (70, V), generator=g).to(dtype)
+    logits[1, -1] = 5.0
+    logits[2] = float("-inf")
+    logits[3, 1:] = float("-inf")
+    logits[4:40] += torch.randn(36, V, generator=g).to(dtype)
+    tokens = torch.randint(0, V, (70,), generator=g)
+    tokens[7] = -1
+    tokens[3] = 0
+    lp_check(K, logits, tokens, k=k, grads=False)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [18, 1001, 33001])
 def test_lp_strides_and_shapes(K, dtype, V):
