@@ -591,10 +591,14 @@ constexpr int kSmallVocab = 512;
 // threads along x).
 bool rows_fit(int64_t rows, int lanes) { return rows * lanes <= 256LL * ((1 << 24) - 1); }
 int score_lanes(int64_t vocab) { return vocab <= 8192 ? 64 : 256; }
+// Lanes of a row's gradient, up to four vectors a lane (300 bf16 logits: 167 us of 2^19 rows, 268 with one), two
+// up to 64 logits (2^20 rows of 64 f32: 98 us for 121). At least 256 bytes of a row at a time beyond that, as
+// stores past the caches of less fill no line (2^20 rows of 100 bf16: 122 us for 220), and 256 lanes, not 128
+// (65536 rows of 2000 f32: 175 us for 204).
 int grad_lanes(int64_t vocab, int dtype) {
-    int L = 1;
-    while (L < 256 && L * (dtype == RLP_F32 ? 4 : 8) < vocab) L *= 2;
-    return L;
+    int L = vocab <= 64 ? 1 : 16;
+    while (L < 256 && L * (dtype == RLP_F32 ? 4 : 8) * (vocab <= 64 ? 2 : 4) < vocab) L *= 2;
+    return L == 128 ? 256 : L;
 }
 
 // Few long rows: each over several blocks of at least one tile per wave.
@@ -660,7 +664,7 @@ void launch_grad(GradArgs a, hipStream_t s) {
         if (past) score_grad_kernel<T, true, false, 1><<<grid, 256, 0, s>>>(a, L);
         else score_grad_kernel<T, false, false, 1><<<grid, 256, 0, s>>>(a, L);
     } else {
-        if (bytes > (512LL << 20)) score_grad_kernel<T, true, true, 4><<<grid, 256, 0, s>>>(a, L);
+        if (L == 256 && bytes > (512LL << 20)) score_grad_kernel<T, true, true, 4><<<grid, 256, 0, s>>>(a, L);
         else if (past) score_grad_kernel<T, true, false, 4><<<grid, 256, 0, s>>>(a, L);
         else score_grad_kernel<T, false, false, 4><<<grid, 256, 0, s>>>(a, L);
     }

@@ -667,6 +667,17 @@ def test_lp_few_alternatives(K, dtype, V, k):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [3, 4, 9, 16, 17, 40, 63, 66, 101, 200, 257, 300, 513, 700, 1023, 1025, 1999, 2049, 4097])
+def test_lp_gradient_sizes(K, dtype, V):
+    """Each number of lanes and vectors a row, with rows at any alignment and tokens at both ends."""
+    g = torch.Generator().manual_seed(V)
+    logits = torch.randn(19, V, generator=g).to(dtype)
+    tokens = torch.randint(0, V, (19,), generator=g)
+    tokens[0], tokens[1], tokens[2] = 0, V - 1, -1
+    lp_check(K, logits, tokens, temperature=1.5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [18, 1001, 33001])
 def test_lp_strides_and_shapes(K, dtype, V):
     g = torch.Generator().manual_seed(V)
