@@ -210,9 +210,10 @@ __device__ __forceinline__ floatx4 mfma_f32(float a, float b, floatx4 c) {
 // accumulator is the operand of rows q -> 4 q + r as it stands: S goes from accumulator to operand
 // without leaving its wave, and so does P, computed transposed as Y X^T and shared out over the waves.
 //
-// Bound by HBM where the state is small (4096 x 4 sequences of 64 tokens, 64 x 64: 1.6 GB in 343 us,
-// 4.7 TB/s), by the f32 matrix rate at 128 x 128 (16 x 16 of 4096: 858 us for 2.15 GB). 32 columns a wave
-// with 32x32 products, at one wave a SIMD, took 1210 us for the former.
+// Bound by HBM and matrix instructions together up to 64 x 64 (4096 x 4 sequences of 64 tokens: 1.6 GB in
+// 343 us, 4.7 TB/s, with 50 % of the cycles in f32 products), by the latter at 128 x 128 (16 x 16 of 4096:
+// 858 us for 2.15 GB, 100 TF/s). 32 columns a wave with 32x32 products, at one wave a SIMD, took three
+// times as long (that training segment 4.86 ms for 1.68).
 template <typename T, int DXB, int NW>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_kernel(WalkArgs a) {
     constexpr int C = 32, DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW;
@@ -556,8 +557,8 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 // its own products (9 us a chunk of 128 x 128); half the registers a wave let four waves run.
 //
 // Bound by issue: of the cycles of 16 sequences of 65536 tokens, 128 x 128 (outputs in 278 us for 1.07 GB),
-// vector instructions take 44 % and matrix instructions 28 %, and they seldom run at once. The check for
-// infs and NaNs is 2 % of it, the second piece of S 5 %.
+// vector instructions take 44 % and matrix instructions 28 %, and they seldom run at once. Without
+// the check for infs and NaNs it takes 1 to 2 % less, without the second piece of S 3 to 6 %.
 template <int DXB, int NW, int PZ, int C>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
     constexpr int CT = C / 16, NP = CT * (CT + 1) / 2, SLOTS = C == 64 ? 6 : 2;  // token tiles, P's, their operands

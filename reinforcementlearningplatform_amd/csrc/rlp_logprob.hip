@@ -202,7 +202,7 @@ __device__ __forceinline__ float about_kth(float x, int k) {
 
 // Rows of up to E G logits, G lanes a row, all of it in registers: 16-byte vectors at any alignment, a lane's
 // G vectors apart. Bound by instructions from 129 logits on, most of them the lanes' sums and the results,
-// which a few rows a wave share: 2^20 rows of 300 bf16 logits in 219 us with 16 lanes a row, 412 with 64.
+// which a few rows a wave share: 2^20 rows of 300 bf16 logits in 199 us with 16 lanes a row, 412 with 64.
 template <typename T, int G, int E = 8>
 __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
     constexpr int VE = 16 / sizeof(T);
@@ -299,10 +299,10 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
 }
 
 // Longer rows: W waves a row, one pass. A wave takes tiles of 64 lanes x 2 16-byte vectors (any
-// alignment), W tiles apart, the next tile loaded ahead: 5.3 TB/s of 4096 x 32768 bf16 logits (4 vectors:
-// 4.5, for the waves that a CU no longer holds). Alternatives: each wave keeps its own list
-// and a lower bound of the row's k-th value, shared between the row's waves through LDS; a tile is
-// searched only where a vector's maximum reaches the bound.
+// alignment), W tiles apart, the next tile loaded ahead: 6.0 TB/s of 4096 x 32768 bf16 logits, 5.3 of
+// 4096 x 131071 (4 vectors: 6.3 and 5.5, but 65536 x 8193 takes 346 us for 245). Alternatives: each wave
+// keeps its own list and a lower bound of the row's k-th value, shared between the row's waves through
+// LDS; a tile is searched only where a vector's maximum reaches the bound.
 template <typename T, int W, bool TOP, bool STREAM>
 __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
     constexpr int VE = 16 / sizeof(T), U = 2, TILE = 64 * VE * U;
@@ -630,10 +630,10 @@ void launch_score(const ScoreArgs &a, hipStream_t s) {
     else if (a.vocab <= 256 && a.k <= 2) score_small_kernel<T, 8, 32><<<blocks(32), 256, 0, s>>>(a);
     else if (a.vocab <= kSmallVocab && a.k <= 2) score_small_kernel<T, 16, 32><<<blocks(16), 256, 0, s>>>(a);
     else if (a.vocab <= kSmallVocab) score_small_kernel<T, 64><<<blocks(4), 256, 0, s>>>(a);
-    else if (a.slices == 1 && (a.vocab <= 8192 || (a.k > 0 && a.rows >= 2048))) {
+    else if (a.slices == 1 && (a.vocab <= 8192 || (a.rows >= 2048 && (a.k > 0 || a.vocab <= 16384)))) {
         // a wave a row: short rows, and rows enough to fill the card where a search for alternatives begins
-        // and ends in every wave (4096 x 131071, 8 alternatives: 284 us, four waves a row 308 us; without
-        // alternatives 4096 x 32768 takes 56 us so and 50 us with four)
+        // and ends in every wave (bf16, 16384 x 32769, 8 alternatives: 226 us, four waves a row 296; without,
+        // 65536 x 8193 takes 189 us so and 245 with four, 4096 x 32768 49 and 45)
         if (a.k) rows(score_rows_kernel<T, 1, true, false>, score_rows_kernel<T, 1, true, true>, blocks(4));
         else rows(score_rows_kernel<T, 1, false, false>, score_rows_kernel<T, 1, false, true>, blocks(4));
     } else {

@@ -35,7 +35,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float2v __attribute__((ext_vector_type(2)));
 
-// tanh(x) for two values on the packed FP32 pipe (v_pk_mul/add/fma_f32 around the two
+// tanh(x) for two values (the build has no packed FP32: two scalar instructions each around the two
 // transcendentals), k = 2 / ln 2 times any exact scale of x
 __device__ __forceinline__ float2v tanh2(float2v x, float k) {
     const float2v t = x * k;
@@ -222,8 +222,8 @@ __device__ __forceinline__ void mlp_x3_forward(const float *__restrict__ P0, con
         }
     }
 
-    // ---- layer 3: out[a][env] = sum_n W3[a][n] tanh(H2^T[n][env]) + b3[a] (pairs of neurons on
-    // the packed FP32 pipe: two partial sums per output)
+    // ---- layer 3: out[a][env] = sum_n W3[a][n] tanh(H2^T[n][env]) + b3[a] (pairs of
+    // neurons: two partial sums per output)
     float2v part[SUB][NOUT];
 #pragma unroll
     for (int sb = 0; sb < SUB; ++sb)

@@ -162,11 +162,10 @@ __device__ __forceinline__ void x3_gemm16(const gptr<float> Xw, float *ring, flo
     }
 }
 
-// packed FP32 (v_pk_mul / v_pk_add / v_pk_fma_f32: two IEEE f32 results per instruction, each
-// rounded exactly as the scalar op) for the FD kernel's elementwise work (layer-1 tanh, h2 tanh and
-// z3, dW3 products, g2, the backward operand scale, the g1 recompute, dW1): 2745 -> 2226 VALU per
-// 16-row wave tile in the ISA, FD -0.5 to -1.2 % (profiles/r6/r6b_fd_pk_lidar_ab.txt): the kernel is
-// not VALU-issue bound
+// Two f32 results per expression, each rounded as the scalar operation, for the FD kernel's elementwise work
+// (layer-1 tanh, h2 tanh and z3, dW3 products, g2, the backward operand scale, the g1 recompute, dW1).
+// The build has no packed FP32 instructions, so they are two scalar ones; as packed ones the FD kernel
+// took 0.5 to 1.2 % less (profiles/r6/r6b_fd_pk_lidar_ab.txt): it is not VALU-issue bound.
 __device__ __forceinline__ float2v pk(float a, float b) { return (float2v){a, b}; }
 __device__ __forceinline__ float2v pk_fma(float2v a, float2v b, float2v c) {
     return __builtin_elementwise_fma(a, b, c);
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(64 * kFdWaves, 1) ppo2_fd_kernel(Ppo2Args g) {
             for (int tt = 0; tt < 8; ++tt) {
                 const floatx4 gt = dh1[8 * h + tt];
 #pragma unroll
-                for (int f = 0; f < 4 * KS; f += 2) {  // two features per packed op
+                for (int f = 0; f < 4 * KS; f += 2) {  // two features at a time
                     float2v x = pk(gt[0], gt[0]) * pk(sv[0][f], sv[0][f + 1]);
 #pragma unroll
                     for (int q = 1; q < 4; ++q) x = pk_fma(pk(gt[q], gt[q]), pk(sv[q][f], sv[q][f + 1]), x);
