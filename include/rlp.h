@@ -683,7 +683,8 @@ int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const vo
                                   float *d_state, void *workspace, int64_t workspace_bytes,
                                   rlp_stream_t stream);
 /* One token for every sequence (T = 1): state_out = reset ? 0 : lam state, + k v^T; state_out may be
- * state. reset [B], stride reset_stride[0]. */
+ * state, and must not overlap it otherwise; out is apart from the inputs. reset [B], stride
+ * reset_stride[0]. */
 int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
                               const float *log_decay, const uint8_t *reset, const float *state,
                               float *state_out, void *out, rlp_stream_t stream);
@@ -697,7 +698,8 @@ int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *
  * gradient 0. A row with NaN or +inf: NaN (NaN is no alternative; where fewer than top_k logits are
  * numbers, the rest of top_tokens is -1 and of top_logp NaN). token < 0 marks a padded row, whose
  * logits are not read: logp, entropy and top_logp 0, top_tokens -1, gradient 0. token >= vocab: logp
- * and gradient NaN. top_k: 0 (no alternatives, top_* unused) to min(vocab, 32). vocab < 2^31.
+ * and gradient NaN. top_k: 0 (no alternatives, top_* unused) to min(vocab, 32). vocab < 2^31;
+ * 2^24 rows and more only as far as one launch has threads for them (else refused).
  * stats [rows][3] f32 (nullable): what the backward needs of the row sums. */
 int64_t rlp_token_logprob_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype);
 int rlp_token_logprob(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,

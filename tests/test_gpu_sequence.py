@@ -194,6 +194,15 @@ def test_la_ragged_batches(K, dtype, B, H):
         la_check(K, la_inputs(B, 40, H, (H, H, H), 7, 9, dtype, seed=B, lengths=lengths.tolist(), reset=0.02))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T", [1, 6, 17, 31, 32])
+@pytest.mark.parametrize("Dk, Dv", [(128, 128), (64, 128), (20, 97), (128, 66)])
+def test_la_short_and_wide(K, dtype, T, Dk, Dv):
+    """Sequences within one chunk, with states, episodes and lengths."""
+    s = la_inputs(5, T, 4, (2, 4, 4), Dk, Dv, dtype, seed=T + Dk, reset=0.1, lengths=[T, 0, 1, T // 2, T])
+    la_check(K, s)
+
+
 def test_la_lengths_are_clamped(K):
     s = la_inputs(2, 40, 1, (1, 1, 1), 8, 8, F32, seed=2, lengths=[-3, 1000])
     out, last = K.linear_attention(*[s[n].cuda() for n in "qkv"], s["ld"].cuda(), state=s["state"].cuda(),
