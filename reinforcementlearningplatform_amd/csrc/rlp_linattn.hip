@@ -442,23 +442,22 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {  // two roundings 
 __device__ __forceinline__ float lo_half(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_half(uint32_t v) { return __uint_as_float(v & 0xFFFF0000u); }
 
-// Eight f32 values as the sum of N bf16 operands: each piece takes what the pieces before left over,
-// so two pieces hold a value to 2^-16 and three to 2^-24 of itself.
-template <int N>
-__device__ __forceinline__ void split8(const float *v, bf16x8 (&out)[N]) {
+// An f32 value as the sum of three bf16 operands: each piece takes what the pieces before left over, at most
+// 2^-9 of it, so the three hold a value to less than 2^-24 of itself, as f32 does.
+constexpr int kPieces = 3;
+
+__device__ __forceinline__ void split8(const float *v, bf16x8 (&out)[kPieces]) {
     float rest[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) rest[e] = v[e];
 #pragma unroll
-    for (int p = 0; p < N; ++p) {
+    for (int p = 0; p < kPieces; ++p) {
         uintx4 w;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             w[e] = pack2(rest[2 * e], rest[2 * e + 1]);
-            if (p + 1 < N) {
-                rest[2 * e] -= lo_half(w[e]);
-                rest[2 * e + 1] -= hi_half(w[e]);
-            }
+            rest[2 * e] -= lo_half(w[e]);
+            rest[2 * e + 1] -= hi_half(w[e]);
         }
         out[p] = __builtin_bit_cast(bf16x8, w);
     }
@@ -543,10 +542,10 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 }
 
 // la_walk_kernel for bf16 operands on v_mfma_f32_16x16x32_bf16, C tokens a chunk. Products of the
-// operands are exact in f32; what is not an operand is split into bf16 pieces where it meets the
-// matrix cores: P and S for the output into two (2^-16, below the output's own rounding), the
-// weighted z of the state's sum into PZ: three (2^-24) where the state leaves the call, so that it is
-// an f32 state, and two where it is only ever used in two pieces itself.
+// operands are exact in f32; what is not an operand (P and S for the output, the weighted z of the state's
+// sum) is split into three bf16 pieces where it meets the matrix cores, so that outputs, gradients and states
+// are those of f32 sums. With two pieces (2^-17 of each term) an output that is small beside its terms had
+// wrong digits, for 7 to 14 % less time (65536 tokens 433 us for 487, the ragged prompts 179 for 197).
 //
 // A 16x16 accumulator holds rows 4 q + r (q = lane >> 4) of column lane & 15, so the accumulators of two
 // row tiles are the operand of 32 rows in the order 4 q .. 4 q + 3, 16 + 4 q .. of the quarter waves. With
@@ -559,14 +558,14 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 // Bound by issue: of the cycles of 16 sequences of 65536 tokens, 128 x 128 (outputs in 278 us for 1.07 GB),
 // vector instructions take 44 % and matrix instructions 28 %, and they seldom run at once. Without
 // the check for infs and NaNs it takes 1 to 2 % less, without the second piece of S 3 to 6 %.
-template <int DXB, int NW, int PZ, int C>
+template <int DXB, int NW, int C>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
     constexpr int CT = C / 16, NP = CT * (CT + 1) / 2, SLOTS = C == 64 ? 6 : 2;  // token tiles, P's, their operands
     constexpr int DX = 32 * DXB, DZ = 16 * NW, NT = 64 * NW, PAD = 16;
     __shared__ __align__(16) unsigned short xs[C][DX + PAD];
     __shared__ __align__(16) unsigned short ys[C][DX + PAD];
     __shared__ __align__(16) unsigned short zs[C][DZ + PAD];
-    __shared__ __align__(16) uintx2 ps[SLOTS][2][64][2];  // (token tile, 32 tokens), piece, lane, half
+    __shared__ __align__(16) uintx2 ps[SLOTS][kPieces][64][2];  // (token tile, 32 tokens), piece, lane, half
     __shared__ __align__(16) float into_s[C], from_s[C];
     __shared__ int bad_s, first_s;
     unsigned tid = threadIdx.x;
@@ -596,7 +595,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     }
     bool seg_cut = false;
     if (tid == 0) bad_s = -1;
-    for (unsigned id = tid; id < SLOTS * 2 * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
+    for (unsigned id = tid; id < SLOTS * kPieces * 64 * 2; id += NT) (&ps[0][0][0][0])[id] = (uintx2){0, 0};  // stays above the diagonal
     Rows16<C, DX, NT> rx, ry;
     Rows16<C, DZ, NT> rz;
     const int64_t xs_t = dir * a.xt, ys_t = dir * a.yt, zs_t = dir * a.zt;
@@ -666,7 +665,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
         };
         if (want_out) {
             // P^T = s1 lam^(i-j) Y X^T of the pairs j <= i of one episode in 16 x 16 tiles (j, i), shared
-            // out over the waves and handed to all of them as operands, two pieces each
+            // out over the waves and handed to all of them as operands, in pieces
             for (int t = w; t < NP; t += NW) {
                 const int it = (t > 0) + (t > 2) + (t > 5), jt = t - it * (it + 1) / 2;
                 floatx4 P = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -683,18 +682,20 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                     pv[r] = P[r] * (a.s1 * decay_pow(lam2, d0 - r));
                     pv[r] = r <= d0 && r >= j0 ? pv[r] : 0.0f;  // 0 whatever stood there
                 }
-                const uintx2 hi = {pack2(pv[0], pv[1]), pack2(pv[2], pv[3])};
                 const int slot = it + (it == 3) + (jt >> 1);
-                ps[slot][0][lane][jt & 1] = hi;
-                ps[slot][1][lane][jt & 1] = (uintx2){pack2(pv[0] - lo_half(hi[0]), pv[1] - hi_half(hi[0])),
-                                                     pack2(pv[2] - lo_half(hi[1]), pv[3] - hi_half(hi[1]))};
+#pragma unroll
+                for (int p = 0; p < kPieces; ++p) {
+                    const uintx2 o = {pack2(pv[0], pv[1]), pack2(pv[2], pv[3])};
+                    ps[slot][p][lane][jt & 1] = o;
+                    pv[0] -= lo_half(o[0]), pv[1] -= hi_half(o[0]), pv[2] -= lo_half(o[1]), pv[3] -= hi_half(o[1]);
+                }
             }
             // x S, decayed to each row
 #pragma unroll
             for (int it = 0; it < CT; ++it) O[it] = (floatx4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < DXB; ++s) {
-                bf16x8 Sp[2];
+                bf16x8 Sp[kPieces];
                 float sv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sv[e] = S[2 * s + (e >> 2)][e & 3];
@@ -702,8 +703,8 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
 #pragma unroll
                 for (int it = 0; it < CT; ++it) {
                     const bf16x8 X = *(const bf16x8 *)&xs[16 * it + l15][32 * s + 8 * q];
-                    O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[0], O[it], 0, 0, 0);
-                    O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[1], O[it], 0, 0, 0);
+#pragma unroll
+                    for (int p = 0; p < kPieces; ++p) O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(X, Sp[p], O[it], 0, 0, 0);
                 }
             }
 #pragma unroll
@@ -723,7 +724,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
 #pragma unroll
                 for (int js = 0; js < (it >> 1) + 1; ++js)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
+                    for (int p = 0; p < kPieces; ++p)
                         O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                             *(const bf16x8 *)&ps[it + (it == 3) + js][p][lane], __builtin_bit_cast(bf16x8, zv[js]), O[it],
                             0, 0, 0);
@@ -750,13 +751,13 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
                 wz[4 * m] = lo_half(zv[js][2 * m]) * f[0], wz[4 * m + 1] = hi_half(zv[js][2 * m]) * f[1];
                 wz[4 * m + 2] = lo_half(zv[js][2 * m + 1]) * f[2], wz[4 * m + 3] = hi_half(zv[js][2 * m + 1]) * f[3];
             }
-            bf16x8 Zp[PZ];
+            bf16x8 Zp[kPieces];
             split8(wz, Zp);
 #pragma unroll
             for (int at = 0; at < 2 * DXB; ++at) {
                 const bf16x8 Y = __builtin_bit_cast(bf16x8, column32<true>(ys, 32 * js, 16 * at, lane));
 #pragma unroll
-                for (int p = 0; p < PZ; ++p) S[at] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Y, Zp[p], S[at], 0, 0, 0);
+                for (int p = 0; p < kPieces; ++p) S[at] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(Y, Zp[p], S[at], 0, 0, 0);
             }
         }
         if (want_out) {
@@ -991,8 +992,7 @@ void launch_walk(const WalkArgs &a, hipStream_t s) {
             // 128 x 128, 107 us for 147; 800 of 24 tokens 17 for 22)
             auto chunk = [&](auto c) {
                 constexpr int C = decltype(c)::value;
-                if (a.fin && a.mode != 2) la_walk_bf16_kernel<DXB, NW, 3, C><<<grid, 64 * NW, 0, s>>>(a);
-                else la_walk_bf16_kernel<DXB, NW, 2, C><<<grid, 64 * NW, 0, s>>>(a);
+                la_walk_bf16_kernel<DXB, NW, C><<<grid, 64 * NW, 0, s>>>(a);
             };
             if ((NW <= 4 && (int64_t)grid.x * a.nseg >= 2048) || a.T <= 32) return chunk(std::integral_constant<int, 32>{});
             chunk(std::integral_constant<int, 64>{});
