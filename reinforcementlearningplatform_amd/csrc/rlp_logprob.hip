@@ -604,7 +604,7 @@ int grad_lanes(int64_t vocab, int dtype) {
 // Few long rows: each over several blocks of at least one tile per wave.
 int slices_of(int64_t rows, int64_t vocab, int dtype, int *len) {
     *len = (int)vocab;
-    if (rows >= 512 || vocab <= kSmallVocab) return 1;
+    if (rows < 1 || rows >= 512 || vocab <= kSmallVocab) return 1;
     const int64_t tile = 4 * (dtype == RLP_F32 ? 512 : 1024);  // four waves' tiles
     int64_t want = (1024 + rows - 1) / rows;
     const int64_t most = (vocab + tile - 1) / tile;

@@ -70,3 +70,17 @@ def test_la_weighted_values_cancel(K, dtype, D):
     want = FINE * (a + b)
     tol = torch.finfo(dtype).eps / 2 * want.abs() + 8 * U * FINE * (a.abs() + b.abs())
     assert ((dv - want).abs() <= tol).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# empty batches
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("V", [7, 512, 513, 40000])
+def test_lp_no_rows(K, V):
+    x = torch.zeros(0, V, device="cuda", requires_grad=True)
+    t = torch.zeros(0, dtype=torch.int64, device="cuda")
+    logp, ent, tl, tt = K.token_logprob(x, t, top_k=2)
+    assert logp.shape == ent.shape == (0,) and tl.shape == tt.shape == (0, 2)
+    assert torch.autograd.grad(logp.sum() + ent.sum(), [x])[0].shape == (0, V)
+    logp, ent = K.token_logprob(x.detach().view(3, 0, V), t.view(3, 0))
+    assert logp.shape == ent.shape == (3, 0)
