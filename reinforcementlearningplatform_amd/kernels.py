@@ -6,6 +6,7 @@ import ctypes as C
 import functools
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _abi
 from ._native import RLPError, check, lib, ptr, stream_ptr
@@ -530,6 +531,14 @@ def _one_device(what, *tensors):
             raise RLPError(f"{what}: not on the GPU, or on several (librlp takes tensors of one device)")
 
 
+def _no_tangents(what, *tensors):
+    """Refuses forward-mode derivatives, which the kernels would drop: a tangent shows in no requires_grad."""
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise RLPError(f"{what}: has no forward-mode derivative, and an argument is a dual tensor")
+
+
 def _launch(what, dev, fn, *args):
     """fn(*args, stream) on device dev, with its current stream."""
     if dev == _device_index():
@@ -696,7 +705,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, len
                      return_state=False):
     """Linear attention with one decay per head, a policy's memory over a rollout segment or a prompt:
     S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T, out_t = scale * q_t S_t (include/rlp.h
-    rlp_linear_attention). Differentiable in q, k, v and state.
+    rlp_linear_attention). Differentiable in q, k, v and state, once and in reverse mode.
 
     q, k [B][T][heads][Dk], v [B][T][heads][Dv] (float32, float16 or bfloat16; 1 to 128 wide; each may
     have fewer heads than log_decay [H], which its heads divide; any strides, so a time-major buffer
@@ -708,6 +717,7 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, len
 
     In a captured HIP graph, capture forward and backward together, with no graph of the same leaves
     alive from outside the capture (torch keeps one accumulation node per leaf and its stream)."""
+    _no_tangents("linear_attention", q, k, v, log_decay, state)
     if torch.is_grad_enabled():
         if log_decay.requires_grad:
             raise RLPError("linear_attention: log_decay has no gradient (pass it detached)")
@@ -725,6 +735,7 @@ def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, sta
     reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv] (in `out`, apart from the other
     arguments, where given). Not differentiable."""
     what = "linear_attention_step"
+    _no_tangents(what, q, k, v, log_decay, state, state_out, out)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
                                     log_decay.requires_grad or state.requires_grad):
         raise RLPError(f"{what}: not differentiable (call it under torch.no_grad, or linear_attention)")
@@ -861,7 +872,7 @@ class _TokenLogprob(torch.autograd.Function):
 def token_logprob(logits, tokens, temperature=1.0, top_k=0):
     """Log-probability of the given tokens (discrete actions) and the entropy of their distributions
     softmax(logits / temperature): the two terms of a PPO2 actor loss over tokens (include/rlp.h
-    rlp_token_logprob). Differentiable in logits.
+    rlp_token_logprob). Differentiable in logits, once and in reverse mode.
 
     logits [...][vocab] float32, float16 or bfloat16; tokens [...] int64 or int32, negative: a padded
     row (0 everywhere, no gradient). -inf logits are actions that are not allowed.
@@ -869,6 +880,7 @@ def token_logprob(logits, tokens, temperature=1.0, top_k=0):
     probable tokens, (logp, entropy, top_logp, top_tokens [...][top_k]), ties to the lower token; those
     two carry no gradient."""
     what = "token_logprob"
+    _no_tangents(what, logits)
     shape, top_k, temperature = tokens.shape, int(top_k), float(temperature)
     if logits.dim() < 1 or shape != logits.shape[:-1]:
         raise RLPError(f"{what}: logits {tuple(logits.shape)}, tokens {tuple(shape)}")

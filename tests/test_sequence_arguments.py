@@ -23,3 +23,33 @@ def test_token_logprob_without_rows(vocab, top_k):
                                      None) == 0
         assert lib.rlp_token_logprob_backward(DEV, dtype, 0, vocab, vocab, DEV, 1.0, DEV, DEV, DEV, DEV, vocab,
                                               None) == 0
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(grad):
+    """A tangent does not show in requires_grad; the operators raise instead of returning none."""
+    import torch.autograd.forward_ad as fwd
+    q, k, v = (torch.ones(2, 3, 2, 4) for _ in range(3))
+    ld, state = -torch.ones(2), torch.ones(2, 2, 4, 4)
+    logits, tokens = torch.ones(3, 5), torch.zeros(3, dtype=torch.int64)
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        def dual(x):
+            return fwd.make_dual(x, torch.ones_like(x))
+        args = dict(q=q, k=k, v=v, log_decay=ld, state=state)
+        for name in args:
+            with pytest.raises(RLPError, match="forward-mode"):
+                K.linear_attention(**{**args, name: dual(args[name])})
+        step = dict(q=q[:, 0], k=k[:, 0], v=v[:, 0], log_decay=ld, state=state, state_out=state.clone(),
+                    out=torch.ones(2, 2, 4))
+        for name in step:
+            with pytest.raises(RLPError, match="forward-mode"):
+                K.linear_attention_step(**{**step, name: dual(step[name])})
+        with pytest.raises(RLPError, match="forward-mode"):
+            K.token_logprob(dual(logits), tokens)
+        # no tangent: on to the next check, of the device
+        for call in (lambda: K.linear_attention(**args), lambda: K.linear_attention_step(**step),
+                     lambda: K.token_logprob(logits, tokens)):
+            with pytest.raises(RLPError, match="GPU"):
+                call()
+    with pytest.raises(RLPError, match="forward-mode"):
+        torch.func.jvp(lambda x: K.token_logprob(x, tokens)[0], (logits,), (logits,))
