@@ -344,7 +344,7 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
         }
     };
     if (!padded) {
-        float mc = 0.0f;  // of sum.m; the loop's sums are about it
+        float off = 0.0f;  // what is in every y of the sums beside (l - sum.m) c
         auto tile = [&](const T(&cur)[U][VE], int at) {
             float x[U][VE], um[U], tm = neg_inf();
 #pragma unroll
@@ -360,18 +360,18 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
             {
                 const float m = fmaxf(sum.m, tm), base = base_of(m);
                 const Shift sh(base, a.c);
-                // the sums so far move to the new maximum (far: mc may be infinite)
-                const float y0 = sum.m == neg_inf() ? neg_inf() : sh.far ? (sum.m - base) * a.c : mc - sh.mc;
+                // the sums so far move to the new maximum and its off, near or far (none so far: -inf)
+                const float y0 = __builtin_fmaf(sum.m - base, a.c, sh.off - off);
                 const float e0 = __builtin_amdgcn_exp2f(y0);
                 sum.w = e0 * __builtin_fmaf(fmaxf(y0, -200.0f), sum.s, sum.w);
                 sum.s *= e0;
-                sum.m = m, mc = sh.mc;
+                sum.m = m, off = sh.off;
                 if (!__any(sh.far)) {
 #pragma unroll
                     for (int u = 0; u < U; ++u)
 #pragma unroll
                         for (int e = 0; e < VE; ++e) {
-                            const float y = __builtin_fmaf(x[u][e], a.c, -mc), p = __builtin_amdgcn_exp2f(y);
+                            const float y = __builtin_fmaf(x[u][e], a.c, -sh.mc), p = __builtin_amdgcn_exp2f(y);
                             sum.s += p;
                             sum.w = __builtin_fmaf(p, fmaxf(y, -200.0f), sum.w);
                         }
@@ -428,7 +428,7 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
             tile(tb, next);
         }
         {   // out of the sums what rounding m c put into every y
-            const float off = Shift(base_of(sum.m), a.c).off, e0 = __builtin_amdgcn_exp2f(-off);
+            const float e0 = __builtin_amdgcn_exp2f(-off);
             sum.w = e0 * __builtin_fmaf(-off, sum.s, sum.w);
             sum.s *= e0;
         }

@@ -84,3 +84,26 @@ def test_lp_no_rows(K, V):
     assert torch.autograd.grad(logp.sum() + ent.sum(), [x])[0].shape == (0, V)
     logp, ent = K.token_logprob(x.detach().view(3, 0, V), t.view(3, 0))
     assert logp.shape == ent.shape == (3, 0)
+
+
+# ---------------------------------------------------------------------------------------------
+# token log-probabilities: maxima that rise through |m log2(e) / temperature| = 1e6, where the exponents'
+# form changes
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("temperature", [1.0, 1e-3, 0.37])
+@pytest.mark.parametrize("V", [513, 3000, 20000])
+def test_lp_rising_through_the_border(K, V, temperature, sign):
+    """Values of neighbouring logits on either side, the larger ones behind, so that each lane's sums move
+    from one form to the other; a few steps apart, so that the sums before count in the result."""
+    g = torch.Generator().manual_seed(V)
+    border = 1e6 / 1.4426950408889634 * temperature
+    step = max(math.ulp(border) * 2.0 ** 29, 0.25 * temperature)   # a float32 step, or a quarter of the temperature
+    N = 520                              # rows enough that none is split, so a wave takes tile after tile
+    at = torch.linspace(-6.0, 6.0, V).expand(N, V) + 0.3 * torch.randn(N, V, generator=g)
+    at[1::8] = -at[1::8]                              # falling
+    at[2::8, :-1], at[2::8, -1] = -2.0, 2.0           # one step at the end
+    at[3::8] = at[3::8].abs() - 1.0
+    at[4::8] = torch.where(torch.arange(V) % 1024 < 512, -2.0, 2.0)
+    logits = (sign * border + at.double() * step).float()
+    lp_check(K, logits, torch.randint(0, V, (N,), generator=g), temperature=temperature, k=5)
