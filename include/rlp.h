@@ -673,9 +673,9 @@ int rlp_linear_attention(const rlp_la_cfg *cfg, const void *q, const void *k, co
                          const float *log_decay, const uint8_t *reset, const int32_t *lengths,
                          const float *state, void *out, float *state_out, void *workspace,
                          int64_t workspace_bytes, rlp_stream_t stream);
-/* Gradients of q, k, v (required; of shared heads the sum over their states) and of state
- * (nullable) from d_out and d_state_out (nullable: 0). States are recomputed from the inputs, but for
- * those in forward_workspace (nullable). */
+/* Gradients of q, k, v (of shared heads the sum over their states) and of state from d_out and
+ * d_state_out (nullable: 0); each nullable: not wanted, and not computed. States are recomputed from the
+ * inputs, but for those in forward_workspace (nullable). */
 int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
                                   const float *log_decay, const uint8_t *reset, const int32_t *lengths,
                                   const float *state, const void *d_out, const float *d_state_out,

@@ -36,7 +36,7 @@ __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
 // One walk over the sequences: operand strides in elements (batch, token, head), D contiguous.
 struct WalkArgs {
     const void *x, *y, *z;
-    void *out;
+    void *out;               // nullable: only the state is wanted
     int64_t xb, xt, xh, yb, yt, yh, zb, zt, zh, ob, ot, oh;
     int gx, gy, gz;          // states per x / y / z head (shared heads)
     const float *log_decay;  // [H]
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     const T *y = (const T *)a.y + b * a.yb + (h / a.gy) * a.yh + tok0 * a.yt;
     const T *z = (const T *)a.z + b * a.zb + (h / a.gz) * a.zh + tok0 * a.zt;
     const int64_t out0 = b * a.ob + h * a.oh + tok0 * a.ot;
-    const bool want_out = a.mode != 1;
+    const bool want_out = a.mode != 1 && a.out;
     const int c0 = 16 * w;
     int col = c0 + l15;
 
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_
     const __bf16 *y = (const __bf16 *)a.y + b * a.yb + (h / a.gy) * a.yh + tok0 * a.yt;
     const __bf16 *z = (const __bf16 *)a.z + b * a.zb + (h / a.gz) * a.zh + tok0 * a.zt;
     const int64_t out0 = b * a.ob + h * a.oh + tok0 * a.ot;
-    const bool want_out = a.mode != 1;
+    const bool want_out = a.mode != 1 && a.out;
     const int c0 = 16 * w;
     int col = c0 + l15;
 
@@ -1030,7 +1030,7 @@ void walk(WalkArgs a, float *ws, hipStream_t s, bool have_states = false) {
         la_join_kernel<<<dim3((unsigned)bh, (a.dx * a.dz + 255) / 256), 256, 0, s>>>(a);
         a.mode = 2;
     }
-    launch_walk<T>(a, s);
+    if (a.mode == 0 || a.out) launch_walk<T>(a, s);
 }
 
 WalkArgs base_args(const rlp_la_cfg &c, const float *log_decay, const uint8_t *reset, const int32_t *lengths) {
@@ -1079,7 +1079,7 @@ void backward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, 
     float *part = ws + segment_floats(bh, c.T, c.Dk, c.Dv);
     // a gradient of unshared heads goes straight out, of shared heads through f32 partials
     auto target = [&](WalkArgs &a, void *out, const int64_t *st, int Hs, int D) {
-        if (Hs == c.H) {
+        if (!out || Hs == c.H) {
             a.out = out, a.ob = st[0], a.ot = st[1], a.oh = st[2];
         } else {
             a.out = part, a.out_f32 = 1;
@@ -1110,7 +1110,7 @@ void backward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, 
         a.rev = 1, a.e0 = 0, a.s1 = c.scale, a.s2 = 1.0f, a.s3 = c.scale;
         target(a, dv, c.dv_stride, c.Hv, c.Dv);
         walk<T>(a, ws, s);
-        if (c.Hv != c.H) share<T>(c, part, dv, c.dv_stride, c.Hv, c.Dv, s);
+        if (dv && c.Hv != c.H) share<T>(c, part, dv, c.dv_stride, c.Hv, c.Dv, s);
     }
     if (dk) {
         WalkArgs a = base_args(c, log_decay, reset, lengths);
@@ -1122,7 +1122,7 @@ void backward(const rlp_la_cfg &c, const void *q, const void *k, const void *v, 
         a.init = d_fin, a.ia = 1, a.in = c.Dv;  // R transposed
         a.rev = 1, a.e0 = 0, a.s1 = c.scale, a.s2 = 1.0f, a.s3 = c.scale;
         target(a, dk, c.dk_stride, c.Hk, c.Dk);
-        walk<T>(a, ws, s, dv != nullptr);
+        walk<T>(a, ws, s, dv || d_init);
         if (c.Hk != c.H) share<T>(c, part, dk, c.dk_stride, c.Hk, c.Dk, s);
     }
 }
@@ -1203,7 +1203,8 @@ int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const vo
     const int rc = check_cfg(cfg, "rlp_linear_attention_backward");
     if (rc != RLP_OK) return rc;
     if (cfg->B == 0 || (cfg->T == 0 && !d_state)) return RLP_OK;
-    RLP_REQUIRE(log_decay && (cfg->T == 0 || (q && k && v && d_out && dq && dk && dv)),
+    if (!dq && !dk && !dv && !d_state) return RLP_OK;
+    RLP_REQUIRE(log_decay && (cfg->T == 0 || (q && k && v && d_out)),
                 "rlp_linear_attention_backward: null argument");
     const int64_t need = workspace_bytes(*cfg, true);
     RLP_REQUIRE(need == 0 || (workspace && workspace_bytes_ >= need),

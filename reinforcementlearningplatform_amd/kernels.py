@@ -646,10 +646,11 @@ def linear_attention_forward(q, k, v, log_decay, scale=None, state=None, reset=N
 
 
 def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, state=None, reset=None,
-                              lengths=None, forward_workspace=None):
-    """rlp_linear_attention_backward: (dq, dk, dv, gradient of state or None) from the gradients of
-    linear_attention's out and state (d_state None: 0); forward_workspace: linear_attention_forward's of the
-    same arguments, which spares a pass over k and v where sequences are split."""
+                              lengths=None, forward_workspace=None, want=(True, True, True, True)):
+    """rlp_linear_attention_backward: (dq, dk, dv, gradient of state) from the gradients of linear_attention's
+    out and state (d_state None: 0); those not in `want`, and the last one without a state, are None and not
+    computed. forward_workspace: linear_attention_forward's of the same arguments, which spares a pass over k
+    and v where sequences are split."""
     what = "linear_attention_backward"
     dims = _la_dims(what, q, k, v, log_decay, state)
     need = _la_workspace_bytes(what, 1, *dims)
@@ -663,19 +664,20 @@ def linear_attention_backward(d_out, d_state, q, k, v, log_decay, scale=None, st
         raise RLPError(f"{what}: forward_workspace of {forward_workspace.numel()} bytes is of another forward")
     _one_device(what, q, k, v, log_decay, state, reset, lengths, d_out, d_state, forward_workspace)
     q, k, v, d_out, log_decay = _rows(q), _rows(k), _rows(v), _rows(d_out), log_decay.contiguous()
-    first = torch.empty_like(state, memory_format=torch.contiguous_format) if state is not None else None
+    first = torch.empty_like(state, memory_format=torch.contiguous_format) if state is not None and want[3] else None
     state = state.contiguous() if state is not None else None
     d_state = d_state.contiguous() if d_state is not None else None
-    dq, dk, dv = _like_order(q, B, T, Hq, Dk), _like_order(k, B, T, Hk, Dk), _like_order(v, B, T, Hv, Dv)
+    dq, dk, dv = (_like_order(x, B, T, heads, D) if wanted else None
+                  for x, heads, D, wanted in ((q, Hq, Dk, want[0]), (k, Hk, Dk, want[1]), (v, Hv, Dv, want[2])))
     ws = log_decay.new_empty(need, dtype=torch.uint8) if need > 0 else None
     cfg = _abi.LA_CFG_PACK.pack(*dims, Dk ** -0.5 if scale is None else scale, *q.stride()[:3],
-                                *k.stride()[:3], *v.stride()[:3], *d_out.stride()[:3], *dq.stride()[:3],
-                                *dk.stride()[:3], *dv.stride()[:3],
+                                *k.stride()[:3], *v.stride()[:3], *d_out.stride()[:3],
+                                *(n for g in (dq, dk, dv) for n in (g.stride()[:3] if g is not None else (0, 0, 0))),
                                 *(reset.stride() if reset is not None else (0, 0)))
     _launch(what, q.get_device(), lib().rlp_linear_attention_backward, cfg, q.data_ptr(), k.data_ptr(), v.data_ptr(),
             log_decay.data_ptr(), _at(reset), _at(lengths), _at(state), d_out.data_ptr(), _at(d_state),
             _at(forward_workspace),
-            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(first), _at(ws), need)
+            _at(dq), _at(dk), _at(dv), _at(first), _at(ws), need)
     return dq, dk, dv, first
 
 
@@ -697,7 +699,8 @@ class _LinearAttention(torch.autograd.Function):
         if d_out is None:
             d_out = _like_order(q, q.shape[0], q.shape[1], log_decay.shape[0], v.shape[3]).zero_()
         dq, dk, dv, first = linear_attention_backward(d_out, d_state, q, k, v, log_decay, ctx.scale, state,
-                                                      reset, lengths, ws)
+                                                      reset, lengths, ws, ctx.needs_input_grad[:3] +
+                                                      ctx.needs_input_grad[5:6])
         return dq, dk, dv, None, None, first, None, None, None
 
 

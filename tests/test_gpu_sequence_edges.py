@@ -107,3 +107,60 @@ def test_lp_rising_through_the_border(K, V, temperature, sign):
     at[4::8] = torch.where(torch.arange(V) % 1024 < 512, -2.0, 2.0)
     logits = (sign * border + at.double() * step).float()
     lp_check(K, logits, torch.randint(0, V, (N,), generator=g), temperature=temperature, k=5)
+
+
+# ---------------------------------------------------------------------------------------------
+# linear attention against float64, value by value
+# ---------------------------------------------------------------------------------------------
+def la_exact(s, scale=None):
+    """{name: (value, the same sum with every term's magnitude)} of out, state, dq, dk, dv, d_state."""
+    sc = s["q"].shape[3] ** -0.5 if scale is None else scale
+
+    def run(f, sc):
+        ls = [f(s[n].double()).requires_grad_() for n in ("q", "k", "v", "state") if s[n] is not None]
+        out, last = la_plain(*ls[:3], s["ld"].double(), sc, ls[3] if len(ls) > 3 else None, s["reset"], s["lengths"])
+        gr = torch.autograd.grad([out, last], ls, [f(s["d_out"].double()), f(s["d_state"].double())], allow_unused=True)
+        return [out.detach(), last.detach()] + [torch.zeros_like(x) if g is None else g for g, x in zip(gr, ls)]
+    return dict(zip(("out", "state", "dq", "dk", "dv", "d_state"), zip(run(lambda x: x, sc), run(torch.abs, abs(sc)))))
+
+
+def la_close(exact, got, s, dtype):
+    """Every value a number, off by at most the additions of its float32 sum and its own rounding: the dot
+    products over D, the walk over T, head groups, and the decays lam^n (up to 40 u where it still counts)."""
+    n = (s["q"].shape[3] + s["v"].shape[3] + s["q"].shape[1] + 16 + 64) * U
+    for name, a in got.items():
+        (b, m), a = exact[name], a.detach().cpu().double()
+        assert a.shape == b.shape, name
+        tol = n * m + (0 if "state" in name else torch.finfo(dtype).eps / 2 * b.abs() + (2.0 ** -25 if dtype == F16 else 0))
+        ok = (a - b).abs() <= tol + 1e-300
+        assert ok.all(), f"{name}: {int((~ok).sum())} of {ok.numel()} off, {int(torch.isnan(a).sum())} NaN"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T, heads", [(70, (2, 2, 2)), (70, (1, 2, 1)), (700, (2, 2, 2)), (700, (1, 1, 2))])
+def test_la_only_the_wanted_gradients(K, dtype, T, heads):
+    """Each subset of the gradients is right by itself, and nothing is computed or stored for the others."""
+    s = la_inputs(2, T, 2, heads, 40, 24, dtype, seed=T, reset=0.01, lengths=[T, T // 2 + 3])
+    exact = la_exact(s)
+    names = ("q", "k", "v", "state")
+    dev = {n: s[n].cuda() for n in names}
+    ld, rs, ln = (s[n].cuda() for n in ("ld", "reset", "lengths"))
+    raw = K.linear_attention_backward
+    for some in range(1, 16):
+        on = [bool(some >> i & 1) for i in range(4)]
+        x = {n: t.clone().requires_grad_(w) for (n, t), w in zip(dev.items(), on)}
+        out, last = K.linear_attention(x["q"], x["k"], x["v"], ld, state=x["state"], reset=rs, lengths=ln, return_state=True)
+        made = []
+        with pytest.MonkeyPatch.context() as mp:
+            mp.setattr(K, "linear_attention_backward", lambda *a, **k: made.append(raw(*a, **k)) or made[-1])
+            got = torch.autograd.grad([out, last], [t for t in x.values() if t.requires_grad],
+                                      [s["d_out"].cuda(), s["d_state"].cuda()])
+        assert [g is not None for g in made[0]] == on
+        la_close(exact, dict(zip([("d_state" if n == "state" else "d" + n) for n, w in zip(names, on) if w], got)), s, dtype)
+
+
+def test_la_raw_backward_without_any_gradient(K):
+    s = la_inputs(1, 5, 1, (1, 1, 1), 4, 4, F32, seed=1)
+    args = [s[n].cuda() for n in ("q", "k", "v", "ld")]
+    res = K.linear_attention_backward(s["d_out"].cuda(), None, *args, state=s["state"].cuda(), want=(False,) * 4)
+    assert res == (None,) * 4
