@@ -164,3 +164,44 @@ def test_la_raw_backward_without_any_gradient(K):
     args = [s[n].cuda() for n in ("q", "k", "v", "ld")]
     res = K.linear_attention_backward(s["d_out"].cuda(), None, *args, state=s["state"].cuda(), want=(False,) * 4)
     assert res == (None,) * 4
+
+
+def la_run(K, s, scale=None):
+    """{name: value} of out, state and all gradients."""
+    x = {n: s[n].cuda().requires_grad_() for n in ("q", "k", "v", "state") if s[n] is not None}
+    opt = {n: s[n].cuda() for n in ("reset", "lengths") if s[n] is not None}
+    out, last = K.linear_attention(x["q"], x["k"], x["v"], s["ld"].cuda(), scale=scale, state=x.get("state"),
+                                   return_state=True, **opt)
+    got = torch.autograd.grad([out, last], list(x.values()), [s["d_out"].cuda(), s["d_state"].cuda()])
+    return dict(out=out, state=last, **{"d_state" if n == "state" else "d" + n: g for n, g in zip(x, got)})
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B, T, H, heads, Dk, Dv", [
+    (1, 1, 1, (1, 1, 1), 1, 1), (2, 31, 2, (2, 2, 2), 5, 7), (1, 32, 3, (3, 3, 3), 32, 32),
+    (3, 33, 2, (2, 2, 2), 33, 65), (2, 64, 4, (1, 2, 4), 64, 64), (1, 65, 4, (4, 2, 1), 64, 128),
+    (1, 129, 2, (2, 2, 2), 128, 128), (2, 97, 6, (3, 2, 6), 128, 40), (1, 130, 2, (1, 1, 2), 96, 100),
+    (1, 511, 2, (2, 1, 2), 17, 128)])
+def test_la_values_of_all_shapes(K, dtype, B, T, H, heads, Dk, Dv):
+    for more in (dict(), dict(reset=0.03, time_major=True), dict(state=False, lengths=[max(0, T - 9 * b) for b in range(B)])):
+        s = la_inputs(B, T, H, heads, Dk, Dv, dtype, seed=T + Dv, **more)
+        la_close(la_exact(s), la_run(K, s), s, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T, D", [(512, 16), (700, 64), (1281, 128)])
+def test_la_values_of_split_sequences(K, dtype, T, D):
+    s = la_inputs(1, T, 2, (1, 2, 2), D, D, dtype, seed=T, reset=0.004)
+    s["reset"][0, 256] = 1
+    la_close(la_exact(s), la_run(K, s), s, dtype)
+    s["reset"], s["lengths"] = None, torch.tensor([T - 200], dtype=torch.int32)
+    la_close(la_exact(s), la_run(K, s), s, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D", [32, 128])
+def test_la_values_of_all_decays(K, dtype, D):
+    s = la_inputs(2, 150, 4, (4, 4, 4), D, D, dtype, seed=3, reset=0.02)
+    s["ld"] = torch.tensor([float("-inf"), -20.0, 0.0, -0.5])
+    la_close(la_exact(s, scale=-1.5), la_run(K, s, scale=-1.5), s, dtype)
+    la_close(la_exact(s), la_run(K, s), s, dtype)
