@@ -205,3 +205,98 @@ def test_la_values_of_all_decays(K, dtype, D):
     s["ld"] = torch.tensor([float("-inf"), -20.0, 0.0, -0.5])
     la_close(la_exact(s, scale=-1.5), la_run(K, s, scale=-1.5), s, dtype)
     la_close(la_exact(s), la_run(K, s), s, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B, H, T, Dk, Dv", [(260, 8, 100, 7, 9), (256, 8, 97, 12, 33), (130, 16, 70, 33, 20),
+                                            (64, 33, 65, 5, 50), (256, 8, 66, 70, 5)])
+def test_la_many_short_sequences(K, dtype, B, H, T, Dk, Dv):
+    """2048 blocks and more of up to 64 columns: 32 tokens a chunk on bf16, several chunks a sequence."""
+    g = torch.Generator().manual_seed(B)
+    lengths = torch.randint(0, T + 1, (B,), generator=g)
+    lengths[:6] = torch.tensor([T, 32, 33, 64, 0, 1])
+    s = la_inputs(B, T, H, (H, H, H), Dk, Dv, dtype, seed=B, reset=0.02, lengths=lengths.tolist())
+    s["reset"][0, 31] = s["reset"][0, 32] = s["reset"][1, 31] = s["reset"][3, 32] = s["reset"][3, 63] = s["reset"][6, 64] = 1
+    la_close(la_exact(s), la_run(K, s), s, dtype)
+
+
+# ---------------------------------------------------------------------------------------------
+# one token: states beyond the last-level cache
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B, H, Dk, Dv", [(4300, 4, 64, 61), (8500, 4, 64, 31), (2200, 4, 128, 62), (600, 4, 120, 128)])
+def test_la_step_past_the_caches(K, dtype, B, H, Dk, Dv):
+    """The same envs in a small call have the same bits, and those are within a few roundings of float64."""
+    g = torch.Generator(device="cuda").manual_seed(B)
+    apart = B * H * Dk * Dv * 4 <= 256 << 20             # only read and written states together are beyond it
+    q, k = (torch.randn(B, H, Dk, device="cuda", generator=g).to(dtype) for _ in range(2))
+    v = torch.randn(B, H, Dv, device="cuda", generator=g).to(dtype)
+    ld = -torch.rand(H, device="cuda", generator=g)
+    st = torch.randn(B, H, Dk, Dv, device="cuda", generator=g)
+    rs = torch.rand(B, device="cuda", generator=g) < 0.3
+    st[rs.nonzero()[0]] = float("nan")                   # dropped
+    few = torch.cat([torch.arange(100), torch.arange(B - 100, B)]).cuda()
+    small = st[few].clone()
+    old = torch.where(rs[few].view(-1, 1, 1, 1), 0.0, small).cpu().double()
+    o1 = K.linear_attention_step(q[few], k[few], v[few], ld, small, reset=rs[few])
+    new = torch.full_like(st, 7.0)
+    o2 = K.linear_attention_step(q, k, v, ld, st, reset=rs, state_out=new)
+    assert torch.equal(o2[few], o1) and torch.equal(new[few], small)
+    if not apart:
+        o3 = K.linear_attention_step(q, k, v, ld, st, reset=rs)
+        assert torch.equal(o3, o2) and torch.equal(st, new)
+    c = [t[few].cpu().double() for t in (q, k, v)]
+    lam = torch.exp(ld.cpu().double()).view(1, H, 1, 1)
+    want = lam * old + c[1].unsqueeze(-1) * c[2].unsqueeze(-2)
+    mag = lam * old.abs() + c[1].abs().unsqueeze(-1) * c[2].abs().unsqueeze(-2)
+    assert ((small.cpu().double() - want).abs() <= 8 * U * mag).all()
+    out, om = ((f(c[0]).unsqueeze(-1) * m).sum(-2) * Dk ** -0.5 for f, m in ((lambda x: x, want), (torch.abs, mag)))
+    assert ((o1.cpu().double() - out).abs() <= torch.finfo(dtype).eps / 2 * out.abs() + (Dk + 16) * U * om).all()
+
+
+# ---------------------------------------------------------------------------------------------
+# token log-probabilities: rows both split and past the caches, rows of 64 parts
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype, N, V, part", [(BF16, 300, 900001, 225280), (F32, 150, 900003, 129024)])
+@pytest.mark.parametrize("k", [0, 5])
+def test_lp_split_rows_past_the_caches(K, dtype, N, V, part, k):
+    """Fewer than 512 rows of more than 512 MB together: parts of rows, each from a multiple of 16 bytes on."""
+    g = torch.Generator(device="cuda").manual_seed(V)
+    flat = torch.empty(N * V + 1, dtype=dtype, device="cuda").normal_(0.0, 3.0, generator=g)
+    x = flat[1:].view(N, V)
+    x[9], x[9, V - 1] = float("-inf"), 0.5
+    x[10, :V // 2] = float("-inf")
+    x[11] = torch.finfo(dtype).min
+    x[12, part - 10:part + 3] = 20.0                           # ties over a part's border
+    x[13, part - 6:part + 5] = 20.0
+    pick = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, 9, 10, 11, 12, 13, N - 1])
+    tokens = torch.randint(0, V, (N,), device="cuda", generator=g)
+    tokens[5], tokens[9] = -1, V - 1
+    res = K.token_logprob(x, tokens, top_k=k)
+    rows, tk = x[pick.cuda()].cpu(), tokens[pick.cuda()].cpu()
+    r = lp_plain(rows, tk, 1.0, k)
+    base = (V / 64 + 48 + 6 * torch.nan_to_num(r["spread"])) * U
+    fin = lambda t: torch.where(torch.isfinite(t), t.abs(), torch.zeros_like(t))
+
+    def close(a, b, tol):
+        a = a[pick.cuda()].cpu().double()
+        assert (((a - b).abs() <= tol) | (a == b)).all()
+    close(res[0], r["logp"], base + 6 * U * fin(r["logp"]))
+    close(res[1], r["entropy"], base * (2 + 2 * r["spread"]))
+    if k:
+        assert torch.equal(res[3][pick.cuda()].cpu(), r["top_tokens"])
+        close(res[2], r["top_logp"], base[:, None] + 6 * U * fin(r["top_logp"]))
+
+
+@pytest.mark.parametrize("dtype, V", [(BF16, 262000), (F32, 131000)])
+@pytest.mark.parametrize("k", [0, 1, 32])
+def test_lp_rows_of_64_parts(K, dtype, V, k):
+    g = torch.Generator().manual_seed(V)
+    logits = (torch.randn(7, V, generator=g) * 3).to(dtype)
+    logits[1] = torch.randint(0, 3, (V,), generator=g).to(dtype)
+    logits[2, :-40] = float("-inf")
+    logits[3], logits[3, V // 2] = float("-inf"), 1.0
+    logits[4] = torch.arange(V).to(dtype) * 1e-4
+    tokens = torch.randint(0, V, (7,), generator=g)
+    tokens[6] = -1
+    lp_check(K, logits, tokens, k=k)
