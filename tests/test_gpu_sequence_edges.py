@@ -221,6 +221,65 @@ def test_la_many_short_sequences(K, dtype, B, H, T, Dk, Dv):
 
 
 # ---------------------------------------------------------------------------------------------
+# infs and NaNs: what they do not reach keeps its digits
+# ---------------------------------------------------------------------------------------------
+def keep_close(exact, got, s, dtype, keep):
+    """la_close of the values of keep[name]."""
+    pick = {n: (exact[n][0][k], exact[n][1][k]) for n, k in keep.items()}
+    la_close(pick, {n: got[n].detach().cpu()[k] for n, k in keep.items()}, s, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("B, H, T, D, at", [(2, 2, 200, 64, 42), (2, 2, 200, 128, 63), (2, 2, 130, 20, 31), (260, 8, 100, 10, 32),
+                                            (260, 8, 100, 10, 45), (1, 2, 700, 32, 300)])
+def test_la_other_episodes_keep_their_digits(K, dtype, bad, B, H, T, D, at):
+    """A spoilt token in an episode of ten: all other episodes' outputs and gradients as if it were not there."""
+    s = la_inputs(B, T, H, (H, 1, H), D, D, dtype, seed=at, reset=1e-9)
+    first, last = at - 3, at + 7
+    s["reset"][:, first] = s["reset"][:, last] = s["reset"][:, T - 9] = 1
+    clean = dict(s)
+    for n in ("q", "k", "v", "d_out"):
+        clean[n] = s[n].clone()
+        clean[n][0, first:last] = 0
+        s[n][0, at, 0, 3] = bad
+    exact, got = la_exact(clean), la_run(K, s)
+    rows = torch.ones(B, T, dtype=torch.bool)
+    rows[0, first:last] = False
+    keep = {n: rows for n in ("out", "dq", "dk", "dv")}
+    keep_close(exact, got, s, dtype, {**keep, "state": slice(None), "d_state": slice(None)})
+    assert not torch.isfinite(got["out"][0, at:last]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [[0], [31], [32], [33, 34], [63, 64], [20, 22, 130], [149]])
+def test_la_other_tokens_keep_their_digits(K, dtype, bad, at):
+    """A spoilt value reaches its own column from its token on, a spoilt d_out the gradients up to its token."""
+    s = la_inputs(2, 150, 2, (2, 2, 2), 33, 40, dtype, seed=15)
+    clean = {n: (x.clone() if torch.is_tensor(x) else x) for n, x in s.items()}
+    out_ok = torch.ones(2, 150, 2, 40, dtype=torch.bool)
+    for i, t in enumerate(at):
+        s["v"][0, t, 0, 5 + i], clean["v"][0, t, 0, 5 + i] = bad, 0
+        out_ok[0, t:, 0, 5 + i] = False
+    exact = la_exact(clean)
+    out, last = K.linear_attention(*(s[n].cuda() for n in "qkv"), s["ld"].cuda(), state=s["state"].cuda(), return_state=True)
+    assert torch.equal(torch.isfinite(out.cpu()), out_ok)
+    keep_close(exact, dict(out=out, state=last), s, dtype, dict(out=out_ok, state=out_ok[:, -1].unsqueeze(2).expand(2, 2, 33, 40)))
+    # backward
+    s = la_inputs(2, 150, 2, (2, 2, 2), 33, 40, dtype, seed=15)
+    clean = {n: (x.clone() if torch.is_tensor(x) else x) for n, x in s.items()}
+    dk_ok, dv_ok, dq_ok = (torch.ones(2, 150, 2, n, dtype=torch.bool) for n in (33, 40, 33))
+    for i, t in enumerate(at):
+        s["d_out"][0, t, 1, 5 + i], clean["d_out"][0, t, 1, 5 + i] = bad, 0
+        dk_ok[0, :t + 1, 1] = dq_ok[0, t, 1] = False
+        dv_ok[0, :t + 1, 1, 5 + i] = False
+    got = la_run(K, s)
+    keep_close(la_exact(clean), got, s, dtype, dict(dq=dq_ok, dk=dk_ok, dv=dv_ok))
+    assert not torch.isfinite(got["dk"].cpu()[~dk_ok]).all()
+
+
+# ---------------------------------------------------------------------------------------------
 # one token: states beyond the last-level cache
 # ---------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F32, BF16])
