@@ -52,8 +52,9 @@ struct Sums {
     float m, s, w;  // m -inf: nothing but -inf so far
 };
 
-// max(a, b, c) of numbers; a NaN is passed over (it shows in the sums). As an instruction: fmaxf puts a
-// canonicalising copy before every operand that comes from memory.
+// max(a, b, c) of numbers. With a NaN, which shows in the sums, it may be any of them: a quiet one is passed
+// over, a signalling one hides those before it. As an instruction: fmaxf puts a canonicalising copy before
+// every operand that comes from memory.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(256) void score_small_kernel(ScoreArgs a) {
             TopBuf top = {top_s[threadIdx.x >> 6], 0, a.k};
             float most = neg_inf();
 #pragma unroll
-            for (int e = 0; e < E; ++e) most = fmaxf(most, x[e]);
+            for (int e = 0; e < E; ++e) most = x[e] > most ? x[e] : most;  // passes over every NaN
             const float lim = about_kth(most, a.k);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -387,6 +388,16 @@ __global__ __launch_bounds__(256) void score_rows_kernel(ScoreArgs a) {
                 }
             }
             if (TOP) {
+                if (__any(sum.s != sum.s)) {  // a NaN in the row so far: maxima that pass over it
+                    tm = neg_inf();
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        um[u] = neg_inf();
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) um[u] = x[u][e] > um[u] ? x[u][e] : um[u];
+                        tm = fmaxf(tm, um[u]);
+                    }
+                }
                 const float others = *bound;
                 if (others > lv) lv = others, li = v1;
                 const int many = __popcll(__ballot(tm >= lv));

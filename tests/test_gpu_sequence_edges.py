@@ -359,3 +359,45 @@ def test_lp_rows_of_64_parts(K, dtype, V, k):
     tokens = torch.randint(0, V, (7,), generator=g)
     tokens[6] = -1
     lp_check(K, logits, tokens, k=k)
+
+
+@pytest.mark.parametrize("dtype, bits", [(F32, 0x7F800001), (BF16, 0x7F81), (F16, 0x7C01)])
+@pytest.mark.parametrize("V", [9, 100, 200, 300, 3000, 20000])
+@pytest.mark.parametrize("k", [1, 2, 5])
+def test_lp_alternatives_beside_nans_of_any_kind(K, dtype, bits, V, k):
+    """NaNs of either sign, quiet and signalling, beside the best logits: no alternatives, and none is lost."""
+    g = torch.Generator().manual_seed(V + k)
+    N = 600                                               # rows enough that none is split
+    logits = torch.randn(N, V, generator=g).to(dtype)
+    best = torch.randint(0, V - 1, (N,), generator=g)
+    logits[torch.arange(N), best] = 50.0
+    raw = logits.view(torch.int32 if dtype == F32 else torch.int16)
+    low = torch.iinfo(raw.dtype).min
+    for i in range(N):
+        at = int(best[i]) + 1 if i % 3 else int(torch.randint(0, V, (1,), generator=g))
+        at = at if at != int(best[i]) else at + 1
+        raw[i, at] = bits + (low if i % 2 else 0) + (torch.finfo(dtype).bits == 32 and i % 5 == 0) * 0x400000
+        if i % 4 == 0:                                    # a whole lane's vector, and the next one
+            raw[i, max(0, at - 5):at] = torch.where(logits[i, max(0, at - 5):at] == 50.0, raw[i, max(0, at - 5):at],
+                                                    torch.tensor(bits, dtype=raw.dtype))
+    assert torch.isnan(logits).any(-1).all()
+    want = lp_plain(logits, torch.zeros(N, dtype=torch.int64), 1.0, k)["top_tokens"]
+    for n in (N, 9):                                      # 9 long rows: in parts
+        logp, ent, tl, tt = K.token_logprob(logits[:n].cuda(), torch.zeros(n, dtype=torch.int64, device="cuda"), top_k=k)
+        assert torch.isnan(logp).all() and torch.isnan(ent).all() and torch.isnan(tl).all()
+        some = (~torch.isnan(logits[:n])).sum(-1, keepdim=True) > torch.arange(k)   # as many numbers as that
+        assert torch.equal(tt.cpu(), torch.where(some, want[:n], -1))
+
+
+def test_sequence_operators_in_inference_mode(K):
+    s = la_inputs(2, 40, 2, (2, 2, 2), 16, 16, F32, seed=3)
+    q, k, v, ld, st = (s[n].cuda() for n in ("q", "k", "v", "ld", "state"))
+    logits, tokens = torch.randn(3, 700, device="cuda"), torch.arange(3, device="cuda")
+    want = K.linear_attention(q, k, v, ld, state=st, return_state=True) + K.token_logprob(logits, tokens, top_k=2)
+    step = K.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, st.clone())
+    with torch.inference_mode():
+        got = K.linear_attention(q, k, v, ld, state=st, return_state=True) + K.token_logprob(logits, tokens, top_k=2)
+        mem = st.clone()
+        assert torch.equal(K.linear_attention_step(q[:, 0], k[:, 0], v[:, 0], ld, mem), step)
+        assert not torch.equal(mem, st)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
