@@ -1153,6 +1153,17 @@ int64_t workspace_bytes(const rlp_la_cfg &c, bool backward) {
     return f * 4;
 }
 
+// The bytes from the first to behind the last of B x H rows of D elements.
+struct Span {
+    const char *first, *behind;
+    Span(const void *p, int64_t B, int64_t b, int64_t H, int64_t h, int64_t D, int64_t size) {
+        const int64_t db = (B - 1) * b, dh = (H - 1) * h;
+        first = (const char *)p + size * ((db < 0 ? db : 0) + (dh < 0 ? dh : 0));
+        behind = (const char *)p + size * ((db > 0 ? db : 0) + (dh > 0 ? dh : 0) + D);
+    }
+    bool meets(const Span &o) const { return first < o.behind && o.first < behind; }
+};
+
 template <typename F>
 void by_type(int dtype, F &&f) {
     if (dtype == RLP_F32) f((float *)nullptr);
@@ -1229,6 +1240,20 @@ int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *
     RLP_REQUIRE(cfg->T == 1, "rlp_linear_attention_step: T = %d (one token)", cfg->T);
     if (cfg->B == 0) return RLP_OK;
     RLP_REQUIRE(q && k && v && log_decay && state && state_out && out, "rlp_linear_attention_step: null argument");
+    {   // blocks of other heads and columns read the inputs while one writes (out's rows may lie between q's, k's, v's)
+        const int64_t B = cfg->B, H = cfg->H, D = (int64_t)cfg->Dk * cfg->Dv, size = cfg->dtype == RLP_F32 ? 4 : 2;
+        const Span in[5] = {{q, B, cfg->q_stride[0], cfg->Hq, cfg->q_stride[2], cfg->Dk, size},
+                            {k, B, cfg->k_stride[0], cfg->Hk, cfg->k_stride[2], cfg->Dk, size},
+                            {v, B, cfg->v_stride[0], cfg->Hv, cfg->v_stride[2], cfg->Dv, size},
+                            {log_decay, 1, 0, 1, 0, H, 4},
+                            {reset, reset ? B : 0, cfg->reset_stride[0], 1, 0, reset ? 1 : 0, 1}};
+        const Span before(state, 1, 0, 1, 0, B * H * D, 4), after(state_out, 1, 0, 1, 0, B * H * D, 4);
+        const Span o(out, B, cfg->o_stride[0], H, cfg->o_stride[2], cfg->Dv, size);
+        RLP_REQUIRE(state == state_out || !after.meets(before), "rlp_linear_attention_step: state_out overlaps state");
+        RLP_REQUIRE(!o.meets(before) && !o.meets(after), "rlp_linear_attention_step: out overlaps a state");
+        for (int i = 0; i < (reset ? 5 : 4); ++i)
+            RLP_REQUIRE(!in[i].meets(after), "rlp_linear_attention_step: the updated state overlaps another argument");
+    }
     StepArgs a = {};
     a.q = q, a.k = k, a.v = v, a.out = out, a.log_decay = log_decay, a.state = state, a.state_out = state_out;
     a.qb = cfg->q_stride[0], a.qh = cfg->q_stride[2], a.kb = cfg->k_stride[0], a.kh = cfg->k_stride[2];

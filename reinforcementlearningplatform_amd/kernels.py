@@ -735,8 +735,8 @@ def linear_attention(q, k, v, log_decay, scale=None, state=None, reset=None, len
 def linear_attention_step(q, k, v, log_decay, state, reset=None, scale=None, state_out=None, out=None):
     """linear_attention for one token of every sequence, for acting: q, k [B][heads][Dk],
     v [B][heads][Dv], state float32 [B][H][Dk][Dv] contiguous, updated in place or written to state_out;
-    reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv] (in `out`, apart from the other
-    arguments, where given). Not differentiable."""
+    reset uint8 / bool [B]: state dropped first. Returns out [B][H][Dv] (in `out` where given). What is written
+    is apart from the other arguments. Not differentiable."""
     what = "linear_attention_step"
     _no_tangents(what, q, k, v, log_decay, state, state_out, out)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or

@@ -53,3 +53,33 @@ def test_forward_mode_is_refused(grad):
                 call()
     with pytest.raises(RLPError, match="forward-mode"):
         torch.func.jvp(lambda x: K.token_logprob(x, tokens)[0], (logits,), (logits,))
+
+
+def step_call(**over):
+    """rlp_linear_attention_step on made-up addresses, 1 MB apart: 2 x 4 heads, 16 x 16, float32."""
+    c = _abi.LACfg()
+    for name, x in dict(dtype=0, B=2, T=1, H=4, Hq=4, Hk=4, Hv=4, Dk=16, Dv=16, scale=1.0).items():
+        setattr(c, name, x)
+    for name in ("q_stride", "k_stride", "v_stride", "o_stride"):
+        setattr(c, name, (C.c_int64 * 3)(64, 0, 16))
+    c.reset_stride = (C.c_int64 * 2)(1, 0)
+    names = ("q", "k", "v", "log_decay", "reset", "state", "state_out", "out")
+    at = {n: (i + 1) << 20 for i, n in enumerate(names)}
+    at["state_out"] = at["state"]
+    at.update(over)
+    rc = _native.lib().rlp_linear_attention_step(C.byref(c), *(C.c_void_p(at[n]) for n in names), None)
+    return rc, _native.lib().rlp_last_error_string()
+
+
+STATE = 6 << 20   # 8192 bytes of states, 512 of the outputs, q, k and v, 16 of log_decay, 2 of reset
+
+
+@pytest.mark.parametrize("over, word", [
+    (dict(q=STATE), b"updated state"), (dict(k=STATE + 8191), b"updated state"), (dict(v=STATE - 511), b"updated state"),
+    (dict(log_decay=STATE + 100), b"updated state"), (dict(reset=STATE - 1), b"updated state"),
+    (dict(out=STATE + 8188), b"out overlaps"), (dict(out=STATE - 511), b"out overlaps"),
+    (dict(state_out=STATE + 4), b"state_out overlaps"), (dict(state_out=STATE - 8188), b"state_out overlaps")])
+def test_step_refuses_what_it_would_overwrite(over, word):
+    """The state that is updated in place is written as well as out: blocks of other heads still read the rest."""
+    rc, message = step_call(**over)
+    assert rc == _abi.RLP_EINVAL and word in message
