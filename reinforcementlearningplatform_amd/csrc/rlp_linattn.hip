@@ -987,14 +987,15 @@ void launch_walk(const WalkArgs &a, hipStream_t s) {
         constexpr int NW = decltype(nw)::value;
         if constexpr (std::is_same_v<T, __bf16>) {
             // 64 tokens a chunk: half the barriers and state steps. Up to 64 columns 32 tokens leave LDS for twice
-            // the blocks, which pays where there are blocks enough: 16384 of 128 tokens, 64 x 64, in 278 us for
-            // 302, but 512 of 2048 tokens in 182 for 149. So do sequences that end within them (8192 of 32 tokens,
-            // 128 x 128, 107 us for 147; 800 of 24 tokens 17 for 22)
+            // the blocks, which pays where there are blocks enough: 16384 of 128 tokens, 64 x 64, in 260 us for
+            // 322, 1024 of 1000 tokens in 137 for 169, 512 of 2048 tokens in 168 for 174, but 512 of 128 tokens in 16.2
+            // for 15.3, 256 of 2048 in 139 for 132, 512 parts of 65536 tokens in 260 for 255. So do sequences that end within them (8192 of 32 tokens, 128 x 128, 118 us
+            // for 165; 800 of 24 tokens 19 for 25)
             auto chunk = [&](auto c) {
                 constexpr int C = decltype(c)::value;
                 la_walk_bf16_kernel<DXB, NW, C><<<grid, 64 * NW, 0, s>>>(a);
             };
-            if ((NW <= 4 && (int64_t)grid.x * a.nseg >= 2048) || a.T <= 32) return chunk(std::integral_constant<int, 32>{});
+            if ((NW <= 4 && grid.x >= 512) || a.T <= 32) return chunk(std::integral_constant<int, 32>{});
             chunk(std::integral_constant<int, 64>{});
         } else {
             la_walk_kernel<T, DXB, NW><<<grid, 64 * NW, 0, s>>>(a);

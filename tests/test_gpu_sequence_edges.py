@@ -211,7 +211,7 @@ def test_la_values_of_all_decays(K, dtype, D):
 @pytest.mark.parametrize("B, H, T, Dk, Dv", [(260, 8, 100, 7, 9), (256, 8, 97, 12, 33), (130, 16, 70, 33, 20),
                                             (64, 33, 65, 5, 50), (256, 8, 66, 70, 5)])
 def test_la_many_short_sequences(K, dtype, B, H, T, Dk, Dv):
-    """2048 blocks and more of up to 64 columns: 32 tokens a chunk on bf16, several chunks a sequence."""
+    """Blocks enough, of up to 64 columns: 32 tokens a chunk on bf16, several chunks a sequence."""
     g = torch.Generator().manual_seed(B)
     lengths = torch.randint(0, T + 1, (B,), generator=g)
     lengths[:6] = torch.tensor([T, 32, 33, 64, 0, 1])
