@@ -653,7 +653,8 @@ int rlp_sac_update(const rlp_sac_nets *nets, const rlp_sac_cfg *cfg, const float
  * token and head axes ([T][B] rollout buffers and slices need no copy); the Dk / Dv axis is
  * contiguous. Dk, Dv: 1 to 128. log_decay [H] f32 device, <= 0 (-inf: no memory).
  * reset [B][T] u8 (nullable), strides reset_stride: a token with a nonzero entry begins an episode,
- * nothing of what came before reaches it, infs and NaNs included.
+ * nothing of what came before reaches it, infs and NaNs included. What they do reach by the formula is
+ * inf or NaN, not always the one that float arithmetic gives.
  * lengths [B] i32 device (nullable): tokens of each sequence, clamped to [0, T]; rows behind them
  * are not read, their outputs and gradients are 0.
  * state / state_out [B][H][Dk][Dv] f32 contiguous (nullable): the state before the first token (0)

@@ -86,8 +86,8 @@ __device__ __forceinline__ T anew(T v) {
 // The sequence of a grid's slot-th H blocks, of up to 64 by their lengths. A sequence's chunks follow one another,
 // so that the longest ends last. Up to two blocks a CU all start at once: the longest get a CU alone, the
 // others share theirs with the shortest, the longer with the shorter. More start in order, the longest
-// first. 24 of 256 .. 2047 tokens with 16 heads, 128 x 128 bf16: 204 us, 231 as they stand (212 longest
-// first); 60 of 125 .. 1000 with 8, 64 x 64 f32: 119 for 143.
+// first. 24 of 256 .. 2047 tokens with 16 heads, 128 x 128 bf16: 213 us, 238 as they stand (221 longest
+// first); 60 of 125 .. 1000 with 8, 64 x 64 f32: 112 for 140.
 __device__ __forceinline__ int by_length(const WalkArgs &a, int slot) {
     if (!a.lengths || a.nseg > 1 || a.B > 64 || gridDim.x <= 256) return slot;
     const int lane = threadIdx.x & 63, n = lane < a.B ? a.lengths[lane] : 0;
@@ -107,7 +107,7 @@ typedef floatx4 floatx4_any __attribute__((aligned(4)));
 
 // A wave's 16 columns of a state, rows row0 + 16 at .. + 3 a lane. Of a transposed one these four are 16 bytes;
 // and without the masks of narrower states the loads are all in flight together (1611 x 16 states of 64 x 128
-// through training on 6 tokens 1280 us for 1650).
+// through training on 6 tokens 1158 us for 1556).
 template <int DZ, int N>
 __device__ __forceinline__ void load_state(floatx4 (&S)[N], const float *src, int64_t ia, int64_t in, int dx, int dz,
                                            int row0, int col) {
@@ -555,9 +555,9 @@ __device__ __forceinline__ uintx4 column32(const unsigned short (*t)[P], int j0,
 // 16 columns a wave, not 32: with 32x32 tiles at two waves a SIMD the same work waited on LDS and on
 // its own products (9 us a chunk of 128 x 128); half the registers a wave let four waves run.
 //
-// Bound by issue: of the cycles of 16 sequences of 65536 tokens, 128 x 128 (outputs in 278 us for 1.07 GB),
-// vector instructions take 44 % and matrix instructions 28 %, and they seldom run at once. Without
-// the check for infs and NaNs it takes 1 to 2 % less, without the second piece of S 3 to 6 %.
+// Bound by issue: of the cycles of 16 sequences of 65536 tokens, 128 x 128 (outputs in 335 us for 1.07 GB),
+// vector instructions take 44 % and matrix instructions 34 %, and they seldom run at once. Without
+// the check for infs and NaNs it takes 1 to 2 % less.
 template <int DXB, int NW, int C>
 __global__ __launch_bounds__(64 * NW, 32 * DXB <= 32 * NW ? 4 : 2) void la_walk_bf16_kernel(WalkArgs a) {
     constexpr int CT = C / 16, NP = CT * (CT + 1) / 2, SLOTS = C == 64 ? 6 : 2;  // token tiles, P's, their operands
@@ -961,8 +961,8 @@ constexpr int kMaxD = 128;
 // A sequence is split where batch x heads leave most CUs idle, into as many segments as fill the card
 // with the two blocks a CU holds at D = 128. A segment has 256 tokens at least, so that its state's way
 // through memory stays below the walk. The split walk reads y and z twice: 384 sequences of up to 2047
-// tokens took 322 us in two parts each, 236 us whole (128 x 128 bf16); 16 of 65536 tokens 504 us in 512
-// blocks, 571 in 256 and 535 in 768.
+// tokens take 305 us in two parts each, 213 us whole (128 x 128 bf16); 16 of 65536 tokens 480 us in 512
+// blocks, 552 in 256 and 502 in 768.
 int segments(int64_t bh, int T, int *seglen) {
     *seglen = T > 0 ? T : 1;
     if (bh < 1 || bh > 128 || T < 512) return 1;

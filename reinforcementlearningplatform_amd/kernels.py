@@ -881,7 +881,7 @@ def token_logprob(logits, tokens, temperature=1.0, top_k=0):
     row (0 everywhere, no gradient). -inf logits are actions that are not allowed.
     Returns (logp, entropy), float32 of tokens' shape; with top_k (1 to 32) also the top_k most
     probable tokens, (logp, entropy, top_logp, top_tokens [...][top_k]), ties to the lower token; those
-    two carry no gradient."""
+    two carry no gradient. In a captured HIP graph: as linear_attention."""
     what = "token_logprob"
     _no_tangents(what, logits)
     shape, top_k, temperature = tokens.shape, int(top_k), float(temperature)
