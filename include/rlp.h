@@ -684,8 +684,8 @@ int rlp_linear_attention_backward(const rlp_la_cfg *cfg, const void *q, const vo
                                   float *d_state, void *workspace, int64_t workspace_bytes,
                                   rlp_stream_t stream);
 /* One token for every sequence (T = 1): state_out = reset ? 0 : lam state, + k v^T; state_out may be
- * state, and must not overlap it otherwise; state_out and out are apart from the other arguments. reset [B], stride
- * reset_stride[0]. */
+ * state, and must not overlap it otherwise; state_out and out are apart from the other arguments. reset
+ * [B], stride reset_stride[0]. */
 int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *k, const void *v,
                               const float *log_decay, const uint8_t *reset, const float *state,
                               float *state_out, void *out, rlp_stream_t stream);

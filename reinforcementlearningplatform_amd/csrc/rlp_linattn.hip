@@ -989,8 +989,8 @@ void launch_walk(const WalkArgs &a, hipStream_t s) {
             // 64 tokens a chunk: half the barriers and state steps. Up to 64 columns 32 tokens leave LDS for twice
             // the blocks, which pays where there are blocks enough: 16384 of 128 tokens, 64 x 64, in 260 us for
             // 322, 1024 of 1000 tokens in 137 for 169, 512 of 2048 tokens in 168 for 174, but 512 of 128 tokens in 16.2
-            // for 15.3, 256 of 2048 in 139 for 132, 512 parts of 65536 tokens in 260 for 255. So do sequences that end within them (8192 of 32 tokens, 128 x 128, 118 us
-            // for 165; 800 of 24 tokens 19 for 25)
+            // for 15.3, 256 of 2048 in 139 for 132, 512 parts of 65536 tokens in 260 for 255. So do sequences that end
+            // within them (8192 of 32 tokens, 128 x 128, 118 us for 165; 800 of 24 tokens 19 for 25)
             auto chunk = [&](auto c) {
                 constexpr int C = decltype(c)::value;
                 la_walk_bf16_kernel<DXB, NW, C><<<grid, 64 * NW, 0, s>>>(a);
@@ -1241,7 +1241,7 @@ int rlp_linear_attention_step(const rlp_la_cfg *cfg, const void *q, const void *
     RLP_REQUIRE(cfg->T == 1, "rlp_linear_attention_step: T = %d (one token)", cfg->T);
     if (cfg->B == 0) return RLP_OK;
     RLP_REQUIRE(q && k && v && log_decay && state && state_out && out, "rlp_linear_attention_step: null argument");
-    {   // blocks of other heads and columns read the inputs while one writes (out's rows may lie between q's, k's, v's)
+    {   // blocks of other heads and columns read the inputs while one writes; out's rows may lie between theirs
         const int64_t B = cfg->B, H = cfg->H, D = (int64_t)cfg->Dk * cfg->Dv, size = cfg->dtype == RLP_F32 ? 4 : 2;
         const Span in[5] = {{q, B, cfg->q_stride[0], cfg->Hq, cfg->q_stride[2], cfg->Dk, size},
                             {k, B, cfg->k_stride[0], cfg->Hk, cfg->k_stride[2], cfg->Dk, size},
